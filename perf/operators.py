@@ -115,7 +115,7 @@ def draw(rng):
     ctx = _log(rng, rows[1], 60000 if kind != "prompt" else 6000)
     # bounded by the cache and by the scores of the largest listed cases
     seqs = _log(rng, 1, 128 if kind != "prompt" else 6)
-    seqs = max(1, min(seqs, int(4e8 // (ctx * hkv * dim)), int(8e10 // (ctx * rows[1] * hkv * group * dim))))
+    seqs = max(1, min(seqs, int(1.3e8 // (ctx * hkv * dim)), int(8e10 // (ctx * rows[1] * hkv * group * dim))))
     c.update(seqs=seqs, rows_lo=rows[0], rows_hi=rows[1], ctx_lo=max(rows[1], ctx // rng.choice((1, 4, 50))), ctx_hi=ctx)
     return c
 
