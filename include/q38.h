@@ -699,6 +699,119 @@ int q38_verify_chain_hc_mapped(q38_moe_layer* const* layers, q38_hc* const* mixe
 int q38_hc_initialize_stream(const uint16_t* embedding, int32_t rows, int32_t hidden, int32_t streams, uint16_t* out,
                              void* hip_stream);
 
+/* ------------------------------------------------------------------ batched token mixing
+ * The two token mixers of the decoder for many requests of ragged lengths at once: causal
+ * attention over a paged key-value cache, and the gated delta rule over a pool of states. No
+ * counterpart in the reference, which serves one request at a time (its decoder keeps one
+ * SelfAttentionState or GatedDeltaNetState, include/qwen38/self_attention.hpp:12-30,
+ * include/qwen38/gated_delta_net.hpp:28-37). These calls take the operands behind the
+ * projections, norms and RoPE (attention) or behind the convolution, SiLU and norms (delta
+ * rule), and hold softmax sums and states in 32 bits; q38_attn_verify and q38_gdn_verify remain
+ * the whole single-request steps with the reference's bf16 rounding points.
+ *
+ * A batch lays the new rows of its sequences one after the other: sequence i owns rows
+ * row_offsets[i] .. row_offsets[i + 1] - 1 of every [rows, ...] tensor, possibly none. Rows that
+ * no sequence owns are read and written by nobody. Lengths, slots and page numbers live in
+ * device memory, so a captured graph is replayed with new ones; `max_rows` is the host's word on
+ * the rows of the longest sequence and only chooses kernels: any true lengths give right results.
+ * Device integers are checked where they are used: row offsets are clamped to [0, rows], and a
+ * page number or slot out of range is never followed (see each call). Calls run on ctx's device
+ * whatever device is current, on a stream of that device. Workspaces and graphs: as elsewhere, a
+ * workspace serves one call at a time and is left dirty; calls (or graph replays) that overlap
+ * need one each. All-zero batches (rows or sequences 0) return Q38_OK. */
+
+/* A layer's pages (caller's device memory, 16-byte aligned). Q38_KV_Q8 keeps int8 codes and one
+ * float scale per (token, kv head): value = code * scale. */
+enum { Q38_KV_BF16 = 0, Q38_KV_Q8 = 1 };
+typedef struct q38_paged_cache {
+    void* keys;            /* [pages][kv_heads][page_tokens][head_dim] bf16 or int8            */
+    void* values;          /* the same                                                         */
+    float* key_scales;     /* [pages][kv_heads][page_tokens] (Q38_KV_Q8), else null             */
+    float* value_scales;
+    int32_t format;        /* Q38_KV_BF16 or Q38_KV_Q8                                         */
+    int32_t pages;
+    int32_t page_tokens;   /* a power of two, 16..1024                                         */
+    int32_t kv_heads;      /* 1..64                                                            */
+    int32_t head_dim;      /* 64, 128 or 256                                                   */
+} q38_paged_cache;
+/* tokens[i]: the tokens of sequence i with its new rows: row r of its n rows is token
+ * tokens[i] - n + r. Token t lies in page page_table[i][t / page_tokens]. Sequences may share
+ * pages (a common prefix) that no call writes. */
+typedef struct q38_paged_batch {
+    int32_t sequences;          /* 0..4096                                                     */
+    int32_t rows;               /* rows of the call's tensors, at most 2^24                     */
+    int32_t max_rows;           /* rows of the longest sequence (a hint), 1..rows               */
+    int32_t table_pages;        /* columns of page_table; table_pages * page_tokens < 2^30     */
+    const int32_t* row_offsets; /* device [sequences + 1], ascending                           */
+    const int32_t* tokens;      /* device [sequences]                                          */
+    const int32_t* page_table;  /* device [sequences][table_pages]                             */
+} q38_paged_batch;
+/* Writes the rows' keys and values into their pages. k, v: device, row r at k + r * k_stride
+ * elements, [kv_heads][head_dim] bf16 each (slices of a projection's output); 16-byte aligned,
+ * strides multiples of 8 and at least kv_heads * head_dim. Q38_KV_Q8: with a = max|x| of the
+ * head's row, code = rint(x * 127 / a) (ties to even; the product is exact and no rounded
+ * quotient crosses a tie, so the codes are those of exact arithmetic) and scale = a / 127; a row
+ * of zeros has scale 0, a row with an infinity or NaN scale NaN, which attention then shows. A
+ * row whose token is negative or behind the table, or whose page is out of range, is not
+ * written. Two rows must not share a token's place. */
+int q38_paged_append(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged_batch* batch, const uint16_t* k,
+                     int64_t k_stride, const uint16_t* v, int64_t v_stride, void* stream);
+/* Attention of the rows over the cache, which already holds them (q38_paged_append): row r of
+ * sequence i sees tokens 0 .. tokens[i] - n + r, and out = sum_t p_t v_t with p the softmax of
+ * scale * (q . k_t); query head h reads kv head h / (q_heads / kv_heads). q and out: device bf16,
+ * [q_heads][head_dim] per row at their strides (alignment as for k); they may not overlap. Scores,
+ * softmax sums and the output's sums are float, p is rounded to bf16 for the product with V (in a
+ * Q8 cache p times the value's scale), out is rounded once. A row that sees no token gives zeros;
+ * what unseen places of the cache hold, infinities and NaN too, has no effect. A sequence with
+ * tokens behind its table or a seen page out of range gives NaN. Results do not depend on the
+ * other sequences' values, but on their lengths within float rounding (they move the points
+ * where the cache is split). */
+size_t q38_paged_attention_workspace_size(const q38_paged_cache* cache, const q38_paged_batch* batch, int32_t q_heads);
+int q38_paged_attention(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged_batch* batch, const uint16_t* q,
+                        int64_t q_stride, int32_t q_heads, float scale, uint16_t* out, int64_t out_stride,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gated delta rule per value head, with the state S [value_dim][key_dim] in float:
+ *   S <- exp(g) S,  S <- S + beta (v - S k) k^T,  o = scale * S q       for every row in turn.
+ * q, k: device bf16 [key_heads][key_dim] per row (value head h reads key head h / (value_heads /
+ * key_heads)), v [value_heads][value_dim], each at its row stride (slices of one convolved row;
+ * 16-byte aligned, strides multiples of 8); log_decay (g <= 0; -inf clears the state) and beta:
+ * device float [rows][value_heads]; out: device bf16 [rows][value_heads][value_dim]. q and k are
+ * taken as given (the layer normalises them before: |k| = 1 keeps the rule stable). Long
+ * sequences run in chunks on the matrix cores with float accuracy (operands split into three
+ * bf16 parts), short ones and calls with checkpoints row by row.
+ * States: a pool [slots][value_heads][value_dim][key_dim] of floats, 16-byte aligned. origin[i]:
+ * the slot a sequence starts from, negative (or a null array) for the zero state; final_slots[i]:
+ * the slot its last state goes to, negative (or null) for none, its own origin for an update in
+ * place; checkpoints[r]: the slot of the state after row r, negative (or null) for none: a
+ * verification keeps a state per row and commits by naming one as the next origin. A sequence
+ * without rows copies its origin to its final slot. A slot that one call writes must not be read
+ * or written by another sequence (or row) of the call; origins may be shared. An origin >= slots
+ * makes the sequence's outputs and states NaN; a written slot >= slots is not written. */
+typedef struct q38_delta_desc {
+    int32_t key_heads;
+    int32_t value_heads;   /* a multiple of key_heads, at most 256                             */
+    int32_t key_dim;       /* 64, 128 or 256                                                   */
+    int32_t value_dim;     /* 64, 128 or 256                                                   */
+    float scale;           /* of the outputs (1 / sqrt(key_dim) in the decoder)                */
+} q38_delta_desc;
+typedef struct q38_delta_batch {
+    int32_t sequences;           /* 0..4096                                                    */
+    int32_t rows;                /* at most 2^24                                               */
+    int32_t max_rows;            /* rows of the longest sequence (a hint), 1..rows             */
+    int32_t slots;
+    const int32_t* row_offsets;  /* device [sequences + 1], ascending                          */
+    const int32_t* origin;       /* device [sequences] or null                                 */
+    const int32_t* final_slots;  /* device [sequences] or null                                 */
+    const int32_t* checkpoints;  /* device [rows] or null                                      */
+    float* states;
+} q38_delta_batch;
+size_t q38_delta_workspace_size(const q38_delta_desc* desc, const q38_delta_batch* batch);
+int q38_delta_rule(q38_ctx* ctx, const q38_delta_desc* desc, const q38_delta_batch* batch, const uint16_t* q,
+                   int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
+                   const float* log_decay, const float* beta, uint16_t* out, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@
 
 #include "q38_device.hpp"
 #include "q38_internal.hpp"
+#include "q38_paged.hpp"
 #include "q38_private.h"
 
 #include <algorithm>
@@ -2167,6 +2168,200 @@ int q38_hc_initialize_stream(const uint16_t* embedding, int32_t rows, int32_t hi
     if ((reinterpret_cast<uintptr_t>(embedding) | reinterpret_cast<uintptr_t>(out)) % 16)
         return fail(Q38_EINVAL, "q38_hc_initialize_stream: embedding and out must be 16-byte aligned");
     Q38_HIP(launch_hc_tile(hidden, streams, rows, embedding, out, static_cast<hipStream_t>(st)));
+    return Q38_OK;
+}
+
+// ------------------------------------------------------------------ batched token mixing
+namespace {
+
+// The calls run on their context's device, whichever is current, and put the caller's back.
+class DeviceScope {
+public:
+    hipError_t enter(int device) {
+        int now = 0;
+        hipError_t e = hipGetDevice(&now);
+        if (e != hipSuccess || now == device) return e;
+        e = hipSetDevice(device);
+        if (e == hipSuccess) back_ = now;
+        return e;
+    }
+    ~DeviceScope() {
+        if (back_ >= 0) (void)hipSetDevice(back_);
+    }
+
+private:
+    int back_ = -1;
+};
+
+int enter_device(const char* name, const q38_ctx* ctx, void* stream, DeviceScope& scope) {
+    if (!ctx) return fail(Q38_EINVAL, std::string(name) + ": null context");
+    Q38_HIP(scope.enter(ctx->device));
+    if (stream) {
+        hipDevice_t dev = 0;
+        Q38_HIP(hipStreamGetDevice(static_cast<hipStream_t>(stream), &dev));
+        if (dev != ctx->device) return fail(Q38_EINVAL, std::string(name) + ": the stream is another device's");
+    }
+    return Q38_OK;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// A [rows, heads * dim] bf16 operand at a row stride.
+int check_rows_operand(const char* name, const char* what, const void* p, int64_t stride, int64_t width) {
+    if (!p) return fail(Q38_EINVAL, std::string(name) + ": null " + what);
+    if (!aligned16(p)) return fail(Q38_EINVAL, std::string(name) + ": " + what + " must be 16-byte aligned");
+    if (stride < width || stride % 8 || stride > (int64_t{1} << 32))
+        return fail(Q38_EINVAL, std::string(name) + ": " + what + " stride must be a multiple of 8, at least the row");
+    return Q38_OK;
+}
+
+int check_paged(const char* name, const q38_paged_cache* c, const q38_paged_batch* b, PagedCacheDev* C,
+                PagedBatchDev* B) {
+    const std::string at = std::string(name) + ": ";
+    if (!c || !b) return fail(Q38_EINVAL, at + "null cache or batch");
+    if (c->format != Q38_KV_BF16 && c->format != Q38_KV_Q8) return fail(Q38_EINVAL, at + "cache format must be bf16 or Q8");
+    if (c->page_tokens < 16 || c->page_tokens > 1024 || (c->page_tokens & (c->page_tokens - 1)))
+        return fail(Q38_EINVAL, at + "page_tokens must be a power of two, 16..1024");
+    if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 64) return fail(Q38_EINVAL, at + "pages must be positive, kv_heads 1..64");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(Q38_EINVAL, at + "head_dim must be 64, 128 or 256");
+    if (b->sequences < 0 || b->sequences > kBatchMaxSeqs || b->rows < 0 || b->rows > kBatchMaxRows)
+        return fail(Q38_EINVAL, at + "sequences must be 0..4096, rows 0..2^24");
+    if (b->rows > 0 && b->sequences > 0 && (b->max_rows < 1 || b->max_rows > b->rows))
+        return fail(Q38_EINVAL, at + "max_rows must be 1..rows");
+    if (b->table_pages < 1 || static_cast<int64_t>(b->table_pages) * c->page_tokens >= (int64_t{1} << 30))
+        return fail(Q38_EINVAL, at + "table_pages must be positive and the table hold less than 2^30 tokens");
+    *C = PagedCacheDev{c->keys, c->values, c->key_scales, c->value_scales, c->pages,
+                       __builtin_ctz(static_cast<unsigned>(c->page_tokens)), c->kv_heads, c->head_dim};
+    *B = PagedBatchDev{b->row_offsets, b->tokens, b->page_table, b->sequences, b->rows, b->table_pages};
+    return Q38_OK;
+}
+
+int check_paged_pointers(const char* name, const q38_paged_cache& c, const q38_paged_batch& b) {
+    const std::string at = std::string(name) + ": ";
+    if (!c.keys || !c.values || !b.row_offsets || !b.tokens || !b.page_table) return fail(Q38_EINVAL, at + "null cache or batch tensor");
+    if (!aligned16(c.keys) || !aligned16(c.values)) return fail(Q38_EINVAL, at + "keys and values must be 16-byte aligned");
+    if ((c.format == Q38_KV_Q8) != (c.key_scales != nullptr) || (c.format == Q38_KV_Q8) != (c.value_scales != nullptr))
+        return fail(Q38_EINVAL, at + "a Q8 cache has scales, a bf16 cache has none");
+    return Q38_OK;
+}
+
+} // namespace
+
+int q38_paged_append(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged_batch* batch, const uint16_t* k,
+                     int64_t k_stride, const uint16_t* v, int64_t v_stride, void* stream) {
+    const char* name = "q38_paged_append";
+    PagedCacheDev C;
+    PagedBatchDev B;
+    if (int rc = check_paged(name, cache, batch, &C, &B)) return rc;
+    if (!B.rows || !B.seqs) return Q38_OK;
+    if (int rc = check_paged_pointers(name, *cache, *batch)) return rc;
+    const int64_t width = static_cast<int64_t>(C.hkv) * C.d;
+    if (int rc = check_rows_operand(name, "k", k, k_stride, width)) return rc;
+    if (int rc = check_rows_operand(name, "v", v, v_stride, width)) return rc;
+    DeviceScope scope;
+    if (int rc = enter_device(name, ctx, stream, scope)) return rc;
+    Q38_HIP(launch_paged_append(C, cache->format == Q38_KV_Q8, B, k, k_stride, v, v_stride, static_cast<hipStream_t>(stream)));
+    return Q38_OK;
+}
+
+static int check_q_heads(const char* name, const PagedCacheDev& C, int32_t q_heads) {
+    if (q_heads < 1 || q_heads > 256 || q_heads % C.hkv)
+        return fail(Q38_EINVAL, std::string(name) + ": q_heads must be a multiple of kv_heads, at most 256");
+    return Q38_OK;
+}
+
+size_t q38_paged_attention_workspace_size(const q38_paged_cache* cache, const q38_paged_batch* batch, int32_t q_heads) {
+    const char* name = "q38_paged_attention_workspace_size";
+    PagedCacheDev C;
+    PagedBatchDev B;
+    if (check_paged(name, cache, batch, &C, &B) || check_q_heads(name, C, q_heads) || !B.rows || !B.seqs) return 0;
+    return paged_attention_ws(C, B, batch->max_rows, q_heads);
+}
+
+int q38_paged_attention(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged_batch* batch, const uint16_t* q,
+                        int64_t q_stride, int32_t q_heads, float scale, uint16_t* out, int64_t out_stride,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+    const char* name = "q38_paged_attention";
+    PagedCacheDev C;
+    PagedBatchDev B;
+    if (int rc = check_paged(name, cache, batch, &C, &B)) return rc;
+    if (int rc = check_q_heads(name, C, q_heads)) return rc;
+    if (!std::isfinite(scale)) return fail(Q38_EINVAL, "q38_paged_attention: scale must be finite");
+    if (!B.rows || !B.seqs) return Q38_OK;
+    if (int rc = check_paged_pointers(name, *cache, *batch)) return rc;
+    const int64_t width = static_cast<int64_t>(q_heads) * C.d;
+    if (int rc = check_rows_operand(name, "q", q, q_stride, width)) return rc;
+    if (int rc = check_rows_operand(name, "out", out, out_stride, width)) return rc;
+    const size_t need = paged_attention_ws(C, B, batch->max_rows, q_heads);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+        return fail(Q38_ESPACE, "q38_paged_attention: workspace too small or not 16-byte aligned");
+    DeviceScope scope;
+    if (int rc = enter_device(name, ctx, stream, scope)) return rc;
+    Q38_HIP(launch_paged_attention(C, cache->format == Q38_KV_Q8, B, batch->max_rows, q, q_stride, q_heads, scale, out,
+                                   out_stride, workspace, static_cast<hipStream_t>(stream)));
+    return Q38_OK;
+}
+
+static int check_delta(const char* name, const q38_delta_desc* d, const q38_delta_batch* b, DeltaDev* D,
+                       DeltaBatchDev* B) {
+    const std::string at = std::string(name) + ": ";
+    if (!d || !b) return fail(Q38_EINVAL, at + "null description or batch");
+    auto dim_ok = [](int32_t n) { return n == 64 || n == 128 || n == 256; };
+    if (!dim_ok(d->key_dim) || !dim_ok(d->value_dim)) return fail(Q38_EINVAL, at + "key_dim and value_dim must be 64, 128 or 256");
+    if (d->key_heads < 1 || d->value_heads < 1 || d->value_heads > 256 || d->value_heads % d->key_heads)
+        return fail(Q38_EINVAL, at + "value heads must be divisible by key heads, at most 256");
+    if (!std::isfinite(d->scale)) return fail(Q38_EINVAL, at + "scale must be finite");
+    if (b->sequences < 0 || b->sequences > kBatchMaxSeqs || b->rows < 0 || b->rows > kBatchMaxRows || b->slots < 0)
+        return fail(Q38_EINVAL, at + "sequences must be 0..4096, rows 0..2^24, slots not negative");
+    if (b->rows > 0 && b->sequences > 0 && (b->max_rows < 1 || b->max_rows > b->rows))
+        return fail(Q38_EINVAL, at + "max_rows must be 1..rows");
+    *D = DeltaDev{};
+    D->hk = d->key_heads;
+    D->hv = d->value_heads;
+    D->dk = d->key_dim;
+    D->dv = d->value_dim;
+    D->scale = d->scale;
+    *B = DeltaBatchDev{b->row_offsets, b->origin, b->final_slots, b->checkpoints, b->states, b->sequences, b->rows, b->slots};
+    return Q38_OK;
+}
+
+size_t q38_delta_workspace_size(const q38_delta_desc* desc, const q38_delta_batch* batch) {
+    DeltaDev D;
+    DeltaBatchDev B;
+    if (check_delta("q38_delta_workspace_size", desc, batch, &D, &B) || !B.seqs) return 0;
+    return delta_ws(D, B, batch->max_rows);
+}
+
+int q38_delta_rule(q38_ctx* ctx, const q38_delta_desc* desc, const q38_delta_batch* batch, const uint16_t* q,
+                   int64_t q_stride, const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
+                   const float* log_decay, const float* beta, uint16_t* out, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+    const char* name = "q38_delta_rule";
+    DeltaDev D;
+    DeltaBatchDev B;
+    if (int rc = check_delta(name, desc, batch, &D, &B)) return rc;
+    if (!B.seqs) return Q38_OK;
+    if (!B.off) return fail(Q38_EINVAL, "q38_delta_rule: null row_offsets");
+    if ((B.origin || B.last || B.ckpt) && B.slots > 0 && !B.states)
+        return fail(Q38_EINVAL, "q38_delta_rule: slots without states");
+    if (!aligned16(B.states)) return fail(Q38_EINVAL, "q38_delta_rule: states must be 16-byte aligned");
+    if (B.rows) {
+        const int64_t kw = static_cast<int64_t>(D.hk) * D.dk, vw = static_cast<int64_t>(D.hv) * D.dv;
+        if (int rc = check_rows_operand(name, "q", q, q_stride, kw)) return rc;
+        if (int rc = check_rows_operand(name, "k", k, k_stride, kw)) return rc;
+        if (int rc = check_rows_operand(name, "v", v, v_stride, vw)) return rc;
+        if (int rc = check_rows_operand(name, "out", out, vw, vw)) return rc;
+        if (!log_decay || !beta) return fail(Q38_EINVAL, "q38_delta_rule: null log_decay or beta");
+    }
+    const size_t need = delta_ws(D, B, batch->max_rows);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+        return fail(Q38_ESPACE, "q38_delta_rule: workspace too small or not 16-byte aligned");
+    D.q = q, D.k = k, D.v = v, D.g = log_decay, D.beta = beta, D.out = out;
+    D.qs = q_stride, D.ks = k_stride, D.vs = v_stride;
+    DeviceScope scope;
+    if (int rc = enter_device(name, ctx, stream, scope)) return rc;
+    Q38_HIP(launch_delta(D, B, batch->max_rows, workspace, static_cast<hipStream_t>(stream)));
     return Q38_OK;
 }
 

@@ -226,6 +226,37 @@ _sig("q38_verify_chain_hc_workspace_size", SZ, C.POINTER(MoeDesc), C.POINTER(HcD
 _sig("q38_verify_chain_hc", C.c_int, P, P, I32, P, I32, P, SZ, P)
 
 
+Q38_KV_BF16, Q38_KV_Q8 = 0, 1
+
+
+class PagedCacheDesc(C.Structure):  # include/q38.h q38_paged_cache
+    _fields_ = [(n, P) for n in ("keys", "values", "key_scales", "value_scales")] + [
+        (n, I32) for n in ("format", "pages", "page_tokens", "kv_heads", "head_dim")]
+
+
+class PagedBatchDesc(C.Structure):  # include/q38.h q38_paged_batch
+    _fields_ = [(n, I32) for n in ("sequences", "rows", "max_rows", "table_pages")] + [
+        (n, P) for n in ("row_offsets", "tokens", "page_table")]
+
+
+class DeltaDesc(C.Structure):  # include/q38.h q38_delta_desc
+    _fields_ = [(n, I32) for n in ("key_heads", "value_heads", "key_dim", "value_dim")] + [("scale", F32)]
+
+
+class DeltaBatchDesc(C.Structure):  # include/q38.h q38_delta_batch
+    _fields_ = [(n, I32) for n in ("sequences", "rows", "max_rows", "slots")] + [
+        (n, P) for n in ("row_offsets", "origin", "final_slots", "checkpoints", "states")]
+
+
+_sig("q38_paged_append", C.c_int, P, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), P, I64, P, I64, P)
+_sig("q38_paged_attention_workspace_size", SZ, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), I32)
+_sig("q38_paged_attention", C.c_int, P, C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), P, I64, I32, F32, P, I64,
+     P, SZ, P)
+_sig("q38_delta_workspace_size", SZ, C.POINTER(DeltaDesc), C.POINTER(DeltaBatchDesc))
+_sig("q38_delta_rule", C.c_int, P, C.POINTER(DeltaDesc), C.POINTER(DeltaBatchDesc), P, I64, P, I64, P, I64, P, P, P, P,
+     SZ, P)
+
+
 def check(rc: int) -> int:
     if rc != Q38_OK:
         raise Q38Error(rc, lib.q38_last_error().decode())
@@ -386,3 +417,128 @@ class Hc:
         if self.h:
             lib.q38_hc_destroy(self.h)
             self.h = None
+
+
+def _opt(t):
+    return None if t is None else ptr(t)
+
+
+def _int32(what: str, *tensors):
+    for t in tensors:
+        if t is not None and (str(t.dtype) != "torch.int32" or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous int32 tensors")
+
+
+def _row_stride(t, heads: int, dim: int) -> int:
+    """Row stride in elements of a [rows, heads, dim] bf16 tensor whose rows are contiguous."""
+    rows_ok = t.dim() == 3 and tuple(t.shape[1:]) == (heads, dim) and t.stride(2) == 1 and (
+        heads == 1 or t.stride(1) == dim)
+    if not rows_ok or str(t.dtype) not in ("torch.bfloat16", "torch.int16", "torch.uint16"):
+        raise ValueError(f"expected a bf16 tensor [rows, {heads}, {dim}] with contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+class PagedBatch:
+    """The ragged rows of a batch of sequences over a paged cache (q38_paged_batch): int32
+    tensors row_offsets [n + 1], tokens [n] and page_table [n, pages] of the device, read by every
+    call made with the batch; max_rows: the rows of the longest sequence."""
+
+    def __init__(self, row_offsets, tokens, page_table, rows: int, max_rows: int):
+        _int32("row_offsets, tokens and page_table", row_offsets, tokens, page_table)
+        n = tokens.numel()
+        if row_offsets.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+            raise ValueError("row_offsets [n + 1], tokens [n] and page_table [n, pages] disagree")
+        self._keep = (row_offsets, tokens, page_table)
+        self.desc = PagedBatchDesc(n, rows, max_rows, page_table.shape[1], ptr(row_offsets), ptr(tokens),
+                                   ptr(page_table))
+
+
+class PagedCache:
+    """A layer's paged keys and values (q38_paged_cache) over device tensors [pages, kv_heads,
+    page_tokens, head_dim]: bf16, or int8 with float scales [pages, kv_heads, page_tokens]."""
+
+    def __init__(self, ctx: "Ctx", keys, values, key_scales=None, value_scales=None):
+        q8 = key_scales is not None
+        if keys.dim() != 4 or keys.shape != values.shape or not (keys.is_contiguous() and values.is_contiguous()):
+            raise ValueError("keys and values must be contiguous [pages, kv_heads, page_tokens, head_dim] tensors")
+        for t in (keys, values):
+            if t.element_size() != (1 if q8 else 2):
+                raise ValueError("a Q8 cache holds int8 codes, a bf16 cache 16-bit values")
+        if q8 != (value_scales is not None):
+            raise ValueError("a Q8 cache has both scales, a bf16 cache none")
+        for t in (key_scales, value_scales):
+            if q8 and (t.shape != keys.shape[:3] or str(t.dtype) != "torch.float32" or not t.is_contiguous()):
+                raise ValueError("scales must be contiguous float32 [pages, kv_heads, page_tokens] tensors")
+        self._ctx, self._keep = ctx, (keys, values, key_scales, value_scales)
+        pages, heads, page, dim = keys.shape
+        self.desc = PagedCacheDesc(ptr(keys), ptr(values), _opt(key_scales), _opt(value_scales),
+                                   Q38_KV_Q8 if q8 else Q38_KV_BF16, pages, page, heads, dim)
+
+    def append(self, batch: PagedBatch, k, v, st=None):
+        """k, v: [rows, kv_heads, head_dim] bf16, any row stride."""
+        d = self.desc
+        ks, vs = _row_stride(k, d.kv_heads, d.head_dim), _row_stride(v, d.kv_heads, d.head_dim)
+        if min(k.shape[0], v.shape[0]) < batch.desc.rows:
+            raise ValueError("k and v have fewer rows than the batch")
+        check(lib.q38_paged_append(self._ctx.h, C.byref(d), C.byref(batch.desc), ptr(k), ks, ptr(v), vs, st))
+
+    def workspace_size(self, batch: PagedBatch, q_heads: int) -> int:
+        return lib.q38_paged_attention_workspace_size(C.byref(self.desc), C.byref(batch.desc), q_heads)
+
+    def attend(self, batch: PagedBatch, q, out, scale: float, ws, st=None):
+        """q, out: [rows, q_heads, head_dim] bf16, any row stride."""
+        d, heads = self.desc, q.shape[1]
+        qs, os_ = _row_stride(q, heads, d.head_dim), _row_stride(out, heads, d.head_dim)
+        if min(q.shape[0], out.shape[0]) < batch.desc.rows:
+            raise ValueError("q and out have fewer rows than the batch")
+        check(lib.q38_paged_attention(self._ctx.h, C.byref(d), C.byref(batch.desc), ptr(q), qs, heads, scale, ptr(out),
+                                      os_, _opt(ws), 0 if ws is None else ws.numel() * ws.element_size(), st))
+
+
+class DeltaBatch:
+    """The ragged rows of a batch of sequences over a pool of delta-rule states (q38_delta_batch):
+    states [slots, value_heads, value_dim, key_dim] float32; int32 tensors row_offsets [n + 1],
+    origin, final_slots [n] and checkpoints [rows] (or None) of the device."""
+
+    def __init__(self, states, row_offsets, origin, final_slots, rows: int, max_rows: int, checkpoints=None):
+        _int32("row_offsets, origin, final_slots and checkpoints", row_offsets, origin, final_slots, checkpoints)
+        n = row_offsets.numel() - 1
+        if any(t is not None and t.numel() != n for t in (origin, final_slots)):
+            raise ValueError("row_offsets [n + 1], origin [n] and final_slots [n] disagree")
+        if checkpoints is not None and checkpoints.numel() < rows:
+            raise ValueError("checkpoints has fewer entries than the batch rows")
+        if states is not None and (states.dim() != 4 or str(states.dtype) != "torch.float32" or not states.is_contiguous()):
+            raise ValueError("states must be a contiguous float32 [slots, value_heads, value_dim, key_dim] tensor")
+        self._keep = (states, row_offsets, origin, final_slots, checkpoints)
+        self.desc = DeltaBatchDesc(n, rows, max_rows, 0 if states is None else states.shape[0], ptr(row_offsets),
+                                   _opt(origin), _opt(final_slots), _opt(checkpoints), _opt(states))
+
+
+class DeltaRule:
+    """The gated delta rule of one layer geometry (q38_delta_rule)."""
+
+    def __init__(self, ctx: "Ctx", key_heads: int, value_heads: int, key_dim: int, value_dim: int, scale: float):
+        self._ctx = ctx
+        self.desc = DeltaDesc(key_heads, value_heads, key_dim, value_dim, scale)
+
+    def workspace_size(self, batch: DeltaBatch) -> int:
+        return lib.q38_delta_workspace_size(C.byref(self.desc), C.byref(batch.desc))
+
+    def run(self, batch: DeltaBatch, q, k, v, log_decay, beta, out, ws, st=None):
+        """q, k: [rows, key_heads, key_dim], v: [rows, value_heads, value_dim] bf16 at any row
+        stride; log_decay, beta: contiguous [rows, value_heads] float32; out: contiguous, as v."""
+        d = self.desc
+        if batch._keep[0] is not None and tuple(batch._keep[0].shape[1:]) != (d.value_heads, d.value_dim, d.key_dim):
+            raise ValueError("states do not have this rule's heads and dims")
+        strides = [_row_stride(t, h, n) for t, h, n in ((q, d.key_heads, d.key_dim), (k, d.key_heads, d.key_dim),
+                                                        (v, d.value_heads, d.value_dim))]
+        if _row_stride(out, d.value_heads, d.value_dim) != d.value_heads * d.value_dim:
+            raise ValueError("out must be contiguous")
+        for t in (log_decay, beta):
+            if str(t.dtype) != "torch.float32" or not t.is_contiguous() or t.shape[1:] != (d.value_heads,):
+                raise ValueError("log_decay and beta must be contiguous float32 [rows, value_heads] tensors")
+        if min(t.shape[0] for t in (q, k, v, log_decay, beta, out)) < batch.desc.rows:
+            raise ValueError("an operand has fewer rows than the batch")
+        check(lib.q38_delta_rule(self._ctx.h, C.byref(d), C.byref(batch.desc), ptr(q), strides[0], ptr(k), strides[1],
+                                 ptr(v), strides[2], ptr(log_decay), ptr(beta), ptr(out), _opt(ws),
+                                 0 if ws is None else ws.numel() * ws.element_size(), st))

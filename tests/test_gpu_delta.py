@@ -1,0 +1,215 @@
+"""The gated delta rule on the GPU (q38_delta_rule) against its float64 recurrence, bounds from
+delta_cases.DeltaCase.exact. Slots that a call does not read hold NaN."""
+import math
+
+import pytest
+import torch
+
+import gpu_util as G
+from delta_cases import BF16, DeltaCase
+
+pytestmark = pytest.mark.gpu
+
+CHUNK = 32  # rows of a chunk of the long form
+
+
+def run(q38, gpu, c, states=None, ws=None, out=None, max_rows=None):
+    states = c.states.cuda() if states is None else states
+    rule = q38.DeltaRule(gpu, c.hk, c.hv, c.dk, c.dv, c.scale)
+    batch = q38.DeltaBatch(states, c.off.cuda(), c.origin.cuda(), c.last.cuda(), c.rows, max_rows or c.max_rows,
+                           None if c.ckpt is None else c.ckpt.cuda())
+    if ws is None:  # dirty
+        ws = torch.full((max(16, rule.workspace_size(batch)),), 0xff, dtype=torch.uint8, device="cuda")
+    out = torch.full((c.rows, c.hv, c.dv), 7.0, dtype=BF16, device="cuda") if out is None else out
+    rule.run(batch, *c.operands("cuda"), out, ws, G.stream())
+    torch.cuda.synchronize()
+    return out.cpu(), states.cpu()
+
+
+def check(c, out, states):
+    # (either form may run: the bounds are the larger ones of the chunked form for long sequences)
+    want, ob, S, sb = c.exact(CHUNK if c.max_rows > 8 and c.ckpt is None else 0)
+    lo, hi = int(c.off[0]), int(c.off[-1])
+    owned = torch.zeros(c.rows, dtype=torch.bool)
+    owned[lo:hi] = True
+    assert (out[~owned] == 7.0).all(), "rows of nobody were written"
+    err = (out.double() - want)[owned].abs()
+    assert bool((err <= ob[owned]).all()), float((err / ob[owned]).max())
+    touched = torch.zeros(c.slots, dtype=torch.bool)
+    for i, n in enumerate(c.lens):
+        got = states[int(c.last[i])].double()
+        touched[int(c.last[i])] = True
+        if n == 0:
+            o = int(c.origin[i])
+            assert torch.equal(got.float(), c.states[o] if o >= 0 else torch.zeros_like(c.states[0]))
+            continue
+        r = int(c.off[i + 1]) - 1
+        off = (got - S[r]).norm(dim=-1)
+        assert bool((off <= sb[r]).all()), float((off / sb[r]).max())
+    if c.ckpt is not None:
+        for r in range(lo, hi):
+            off = (states[int(c.ckpt[r])].double() - S[r]).norm(dim=-1)
+            touched[int(c.ckpt[r])] = True
+            assert bool((off <= sb[r]).all()), (r, float((off / sb[r]).max()))
+    assert torch.equal(states[~touched].nan_to_num(123.0), c.states[~touched].nan_to_num(123.0))
+
+
+HEADS = {"family": (2, 4, 128, 128), "small": (1, 1, 64, 64), "wide": (2, 2, 256, 256), "uneven": (1, 3, 128, 64),
+         "tall": (2, 2, 64, 256), "many": (4, 16, 64, 128)}
+LENGTHS = {"one": [1], "decode": [1] * 9, "verify": [4, 1, 3, 7], "empty": [0, 2, 0, 0, 5, 0],
+           "prompt_33": [33], "prompt": [70, 1, 0, 129, 32, 64], "prompt_long": [515, 40], "edge": [31, 32, 33, 63, 64, 65]}
+
+
+@pytest.mark.parametrize("lengths", list(LENGTHS))
+@pytest.mark.parametrize("heads", list(HEADS))
+def test_delta(gpu, q38, heads, lengths):
+    hk, hv, dk, dv = HEADS[heads]
+    c = DeltaCase(LENGTHS[lengths], hk, hv, dk, dv, seed=len(heads) * 7 + len(lengths), gap=2)
+    check(c, *run(q38, gpu, c))
+
+
+@pytest.mark.parametrize("lengths", ["one", "verify", "empty", "prompt_33"])
+def test_checkpoints(gpu, q38, lengths):
+    c = DeltaCase(LENGTHS[lengths], 2, 4, 128, 128, seed=3, checkpoints=True)
+    check(c, *run(q38, gpu, c))
+
+
+@pytest.mark.parametrize("rows", [[3, 1], [90, 40, 33]])
+def test_zero_origin_and_no_results(gpu, q38, rows):
+    c = DeltaCase(rows, 2, 2, 64, 64, seed=4, origin="zero")
+    out, states = run(q38, gpu, c)
+    check(c, out, states)
+    rule = q38.DeltaRule(gpu, 2, 2, 64, 64, c.scale)
+    for pool in (None, torch.full((1, 2, 64, 64), math.nan, device="cuda")):  # null arrays: no slot is read or written
+        batch = q38.DeltaBatch(pool, c.off.cuda(), None, None, c.rows, c.max_rows)
+        o2 = torch.zeros(c.rows, 2, 64, dtype=BF16, device="cuda")
+        rule.run(batch, *c.operands("cuda"), o2, G.workspace(max(16, rule.workspace_size(batch))), G.stream())
+        torch.cuda.synchronize()
+        assert torch.equal(o2.cpu(), out)
+
+
+@pytest.mark.parametrize("rows", [[2, 5], [70, 140]])
+@pytest.mark.parametrize("decay", [0.0, 1.0, 40.0, math.inf])
+def test_decays(gpu, q38, rows, decay):
+    """No decay, strong decay (sums of a chunk far below the smallest exponent) and rows that clear
+    the state (log decay -inf)."""
+    c = DeltaCase(rows, 1, 2, 64, 64, seed=5, decay=0.05 if decay == math.inf else decay)
+    if decay == math.inf:
+        c.g_log[3::7] = -math.inf
+    if decay == 40.0:  # one strong row among weak ones: the weak ones' differences must survive its size
+        c.g_log[torch.arange(c.rows) % 9 != 4] *= 1e-3
+    check(c, *run(q38, gpu, c))
+
+
+def test_in_place_and_shared_origins(gpu, q38):
+    c = DeltaCase([3, 40, 2], 2, 4, 64, 64, seed=6)
+    want_out, want = run(q38, gpu, c)
+    d = DeltaCase([3, 40, 2], 2, 4, 64, 64, seed=6)
+    d.last = d.origin.clone()
+    out, states = run(q38, gpu, d)
+    assert torch.equal(out, want_out)
+    assert torch.equal(states[d.origin.long()], want[c.last.long()])
+    e = DeltaCase([3, 40, 2], 2, 4, 64, 64, seed=6)
+    e.origin[:] = e.origin[0]
+    check(e, *run(q38, gpu, e))
+
+
+@pytest.mark.parametrize("rows", [[2, 1, 3], [50, 40, 90]])
+def test_bad_slots(gpu, q38, rows):
+    c = DeltaCase(rows, 1, 2, 64, 64, seed=7)
+    clean_out, clean = run(q38, gpu, c)
+    c.origin[1] = c.slots
+    last = c.last.clone()
+    c.last[2] = c.slots + 5
+    out, states = run(q38, gpu, c)
+    a, b = int(c.off[1]), int(c.off[2])
+    assert torch.isnan(out[a:b].float()).all() and torch.isnan(states[int(last[1])]).all()
+    assert torch.equal(out[:a], clean_out[:a]) and torch.equal(out[b:], clean_out[b:])
+    assert torch.equal(states[int(last[0])], clean[int(last[0])])
+    assert torch.isnan(states[int(last[2])]).all()  # as it was
+
+
+@pytest.mark.parametrize("hint", [1, 3, 200, 10 ** 9])
+def test_max_rows_is_a_hint(gpu, q38, hint):
+    c = DeltaCase([200, 1, 3, 50], 2, 4, 128, 128, seed=8)
+    check(c, *run(q38, gpu, c, max_rows=min(hint, c.rows)))
+
+
+def test_offsets_outside_the_rows_are_clamped(gpu, q38):
+    c = DeltaCase([40, 50], 1, 2, 64, 64, seed=9)
+    want = run(q38, gpu, c)
+    c.off[2] = 10 ** 6
+    got = run(q38, gpu, c)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1][c.last.long()], want[1][c.last.long()])
+
+
+def test_prompt_in_pieces_then_tokens(gpu, q38):
+    """A prompt in two calls, then single tokens, then a verification of four rows committed at its
+    second: the same as the rows in one float64 recurrence."""
+    n = 150
+    c = DeltaCase([n], 2, 4, 128, 128, seed=10, origin="zero", spare=8)
+    want, ob, S, sb = c.exact(CHUNK)
+    pool = c.states.cuda()
+    at, origin = 0, -1
+    for size in (97, 45, 1, 1, 1, 1, 4):
+        d = DeltaCase([size], 2, 4, 128, 128, checkpoints=size == 4)
+        d.qkv, d.g_log, d.beta = c.qkv[at:at + size], c.g_log[at:at + size], c.beta[at:at + size]
+        d.origin, d.last = torch.tensor([origin], dtype=torch.int32), torch.tensor([0], dtype=torch.int32)
+        if size == 4:
+            d.ckpt = torch.arange(1, 5, dtype=torch.int32)
+            d.last[:] = -1
+        out, states = run(q38, gpu, d, states=pool)
+        assert bool(((out.double() - want[at:at + size]).abs() <= 2 * ob[at:at + size]).all())
+        at, origin = at + size, 0
+    assert at == n
+    for r in range(4):
+        off = (states[1 + r].double() - S[n - 4 + r]).norm(dim=-1)
+        assert bool((off <= 2 * sb[n - 4 + r]).all())
+
+
+def test_captured_and_on_streams(gpu, q38):
+    """Graphs of the long and the short form over one pool, replayed with new values, against eager
+    calls on another stream with another workspace."""
+    for rows in ([1, 1, 1], [64, 33, 100]):
+        c = DeltaCase(rows, 2, 4, 128, 128, seed=11)
+        rule = q38.DeltaRule(gpu, 2, 4, 128, 128, c.scale)
+        pool = c.states.cuda()
+        batch = q38.DeltaBatch(pool, c.off.cuda(), c.origin.cuda(), c.last.cuda(), c.rows, c.max_rows)
+        q, k, v, g, beta = c.operands("cuda")
+        qkv = q._base if q._base is not None else q
+        out = torch.zeros(c.rows, 4, 128, dtype=BF16, device="cuda")
+        ws = G.workspace(max(16, rule.workspace_size(batch)))
+        rule.run(batch, q, k, v, g, beta, out, ws, G.stream())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            rule.run(batch, q, k, v, g, beta, out, ws, torch.cuda.current_stream().cuda_stream)
+        side = torch.cuda.Stream()
+        for i in range(3):
+            d = DeltaCase(rows, 2, 4, 128, 128, seed=20 + i)
+            qkv.copy_(d.qkv)
+            g.copy_(d.g_log)
+            beta.copy_(d.beta)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got, st = out.clone(), pool[c.last.long().cuda()].clone()
+            with torch.cuda.stream(side):
+                o2, w2 = torch.zeros_like(out), torch.zeros_like(ws)
+                rule.run(batch, q, k, v, g, beta, o2, w2, side.cuda_stream)
+            torch.cuda.synchronize()
+            assert torch.equal(got, o2) and torch.equal(st, pool[c.last.long().cuda()])
+
+
+def test_rows_of_a_batch_do_not_depend_on_each_other(gpu, q38):
+    """A sequence's bits are the same alone and beside others of its own form."""
+    for rows in ([3, 1, 5], [200, 70, 41]):
+        c = DeltaCase(rows, 2, 4, 128, 128, seed=12)
+        out, states = run(q38, gpu, c)
+        for i, n in enumerate(rows):
+            d = DeltaCase([n], 2, 4, 128, 128, spare=c.slots - 2)
+            a = int(c.off[i])
+            d.qkv, d.g_log, d.beta = c.qkv[a:a + n], c.g_log[a:a + n], c.beta[a:a + n]
+            d.states, d.slots, d.origin, d.last = c.states, c.slots, c.origin[i:i + 1], c.last[i:i + 1]
+            o, s = run(q38, gpu, d)
+            assert torch.equal(o, out[a:a + n]) and torch.equal(s[int(c.last[i])], states[int(c.last[i])])
