@@ -3,11 +3,15 @@
 //
 //   k_paged_append   per (row, kv head, keys / values): the copy into the token's place, or its
 //                    8-bit codes and scale
-//   k_paged_attn     per (row, query head): one pass over the row's tokens with the running
-//                    maximum and sum of the softmax
+//   k_paged_split    attention of few queries per sequence: equal shares of all sequences' tokens,
+//                    one pass with the running maximum and sum of the softmax
+//   k_paged_join     the shares' pieces of a sequence joined
 #include "q38_device.hpp"
 #include "q38_paged.hpp"
 #include "q38_internal.hpp"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace q38 {
 
@@ -67,55 +71,526 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedCacheDev C, PagedBatc
     }
 }
 
-// One wave per (row, query head); lane l holds dims l D/64 .. of the query, the output and each
-// token's key and value.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){lo, hi}, bf16x2));
+}
+__device__ __forceinline__ float code_f(uint32_t w, int b) { return static_cast<float>(static_cast<int8_t>(w >> (8 * b))); }
+__device__ __forceinline__ floatx4 mfma(uintx4 a, uintx4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+constexpr float kNan = __builtin_nanf("");
+
+// ---- the register layout of the attention products.
+// A wave works transposed, on 32 tokens and 16 queries (a column each) at a time: S^T = K Q^T,
+// then O^T += V^T P^T, with 16x16x32 products (A: row lane % 16, k 8 (lane / 16) + j; B the same by
+// column; result: column lane % 16, rows 4 (lane / 16) + r). The order of a product's rows and of
+// its k index is free as long as both operands agree, and it is chosen so that nothing has to
+// move between lanes, with u = lane % 16, w = lane / 16:
+//   scores   two products per 32 dims: product a (0, 1) has token 8 (u / 4) + 4 a + u % 4 in row u,
+//            so that a lane's results, rows 4 w + r of both, are tokens 8 w .. 8 w + 7 of its query:
+//            just the k index that the second product wants of its B operand. Keys are read as
+//            16-byte runs of a row straight into the operand.
+//   values   lane (u, w) reads the rows of tokens 8 w .. 8 w + 7, E = D / 16 dims of each, 16 bytes at
+//            a time; pairs of rows are interleaved by byte permutes into E operands of 8 tokens,
+//            operand o covering dim o of every lane's run. Results: dims of 4 w + r's runs.
+// The softmax statistics of a query live in its column's lanes: rescaling is lane-local too.
 template <int D, bool Q8>
-__global__ __launch_bounds__(64) void k_paged_attn(PagedCacheDev C, PagedBatchDev B, const uint16_t* __restrict__ q,
-                                                   int64_t qs, int hq, float scale, uint16_t* __restrict__ out,
-                                                   int64_t os) {
-    constexpr int E = D / 64;
-    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int s = row_sequence(B.off, B.seqs, row);
-    if (s < 0) return;
-    const RowSpan span = row_span(B.off, s, B.rows);
-    const int head = h / (hq / C.hkv);
-    int64_t see = static_cast<int64_t>(B.tokens[s]) - (span.end - row) + 1;
-    bool bad = false;
-    if (B.tokens[s] > (static_cast<int64_t>(B.width) << C.shift)) bad = true, see = 0;
-    float qv[E], o[E] = {};
-#pragma unroll
-    for (int e = 0; e < E; ++e) qv[e] = bf2f(q[row * qs + h * D + lane * E + e]);
-    float m = -INFINITY, sum = 0.0f;
-    for (int64_t t = 0; t < see; ++t) {
-        const int32_t page = B.table[static_cast<int64_t>(s) * B.width + (t >> C.shift)];
-        const int64_t at = cache_row(page, C.pages, C.hkv, head, C.shift, static_cast<int>(t));
-        if (at < 0) {
-            bad = true;
-            break;
-        }
-        float kv[E], vv[E], dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int64_t i = at * D + lane * E + e;
-            kv[e] = Q8 ? static_cast<const int8_t*>(C.keys)[i] : bf2f(static_cast<const uint16_t*>(C.keys)[i]);
-            vv[e] = Q8 ? static_cast<const int8_t*>(C.values)[i] : bf2f(static_cast<const uint16_t*>(C.values)[i]);
-            dot = fmaf(qv[e], kv[e], dot);
-        }
-        dot = wave_sum_xor(dot) * scale;
-        if (Q8) dot *= C.ks[at];
-        const float top = fmaxf(m, dot);
-        // (a score of -inf leaves the row as it was; NaN reaches the sum)
-        const float keep = top == -INFINITY ? 1.0f : expf(m - top);
-        const float p = dot == -INFINITY ? 0.0f : expf(dot - top);
-        m = top;
-        sum = sum * keep + p;
-        const float pv = Q8 ? p * C.vs[at] : p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(pv, vv[e], o[e] * keep);
+struct AttnGeo {
+    static constexpr int E = D / 16;                  // dims of a lane's run in the values
+    static constexpr int VD = Q8 ? E / 4 : E / 2;     // its dwords
+    static constexpr int KS = D / 32;                 // 32-dim products of a score
+    static constexpr int KD = Q8 ? D / 64 : D / 32;   // 16-byte loads of a key row and lane
+    static constexpr int EC = (Q8 ? 16 : 8) < E ? (Q8 ? 16 : 8) : E;  // dims of one load of the values
+    // dim of operand o in the run of lane u (or result row u)
+    __device__ static int dim(int u, int o) { return (o / EC) * 16 * EC + EC * u + o % EC; }
+};
+
+// 32 tokens' keys of a lane (with their scales), or their values.
+template <int D, bool Q8>
+struct KeyTile {
+    uintx4 k[2][AttnGeo<D, Q8>::KD];
+    floatx4 s[2];
+};
+template <int D, bool Q8>
+struct ValueTile {
+    uint32_t v[8][AttnGeo<D, Q8>::VD];
+    floatx4 s[2];
+};
+
+// First cache rows (head rows) of the two 16-token halves of 32 tokens.
+struct HalfRows {
+    int64_t lo, hi;
+    __device__ __forceinline__ int64_t of(int half) const {
+        const int64_t a = lo, b = hi;  // (values: a select of addresses would put them in memory)
+        return half ? b : a;
     }
-    const float inv = bad ? __uint_as_float(0x7fc00000u) : see > 0 ? 1.0f / sum : 0.0f;
+};
+// A sequence's pages. The 32 tokens from `base` lie in the pages of their two 16-token halves (one
+// page, for pages of 32 and more): the numbers are uniform over the wave.
+struct PageWalk {
+    const int32_t* table;  // the sequence's row
+    int shift, pages, hkv, head, see;
+    bool bad;
+    // (a page out of range counts as page 0, a half behind the last seen token as that token's page)
+    __device__ __forceinline__ int64_t half(int t) {
+        int page = table[min(t, see - 1) >> shift];
+        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(pages)) {
+            bad = true;
+            page = 0;
+        }
+        return ((static_cast<int64_t>(page) * hkv + head) << shift) + (t & ((1 << shift) - 1));
+    }
+    __device__ __forceinline__ HalfRows rows(int base) { return HalfRows{half(base), half(base + 16)}; }
+};
+
+template <int D, bool Q8>
+__device__ __forceinline__ void load_keys(const PagedCacheDev& C, HalfRows at, int lane, KeyTile<D, Q8>& t) {
+    using Geo = AttnGeo<D, Q8>;
+    const int u = lane & 15, w = lane >> 4;
+    const int64_t row = at.of(u >> 3) + (8 * (u >> 2) & 15) + (u & 3);
+    const char* p = static_cast<const char*>(C.keys) + row * (D * (Q8 ? 1 : 2)) + 16 * w;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[row * os + h * D + lane * E + e] = f2bf(see > 0 || bad ? o[e] * inv : 0.0f);
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int c = 0; c < Geo::KD; ++c)
+            t.k[a][c] = *reinterpret_cast<const uintx4*>(p + 4 * a * D * (Q8 ? 1 : 2) + 64 * c);
+    if constexpr (Q8) {
+        const float* s = C.ks + at.of(w >> 1) + (8 * w & 15);
+        t.s[0] = *reinterpret_cast<const floatx4*>(s);
+        t.s[1] = *reinterpret_cast<const floatx4*>(s + 4);
+    }
+}
+template <int D, bool Q8>
+__device__ __forceinline__ void load_values(const PagedCacheDev& C, HalfRows at, int lane, ValueTile<D, Q8>& t) {
+    using Geo = AttnGeo<D, Q8>;
+    const int u = lane & 15, w = lane >> 4;
+    const int64_t row = at.of(w >> 1) + (8 * w & 15);
+    constexpr int B = Q8 ? 1 : 2;
+    const char* p = static_cast<const char*>(C.values) + row * (D * B) + Geo::EC * B * u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (Geo::VD == 1) {
+            t.v[j][0] = *reinterpret_cast<const uint32_t*>(p + j * D * B);
+        } else if constexpr (Geo::VD == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p + j * D * B);
+            t.v[j][0] = x.x, t.v[j][1] = x.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < Geo::VD / 4; ++c) {
+                const uintx4 x = *reinterpret_cast<const uintx4*>(p + j * D * B + 256 * c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t.v[j][4 * c + i] = x[i];
+            }
+        }
+    }
+    if constexpr (Q8) {
+        t.s[0] = *reinterpret_cast<const floatx4*>(C.vs + row);
+        t.s[1] = *reinterpret_cast<const floatx4*>(C.vs + row + 4);
+    }
+}
+
+// The queries of a tile as B operands: column lane % 16 of each group of 16.
+template <int D, bool Q8, int MT>
+struct QueryTile {
+    uintx4 q[MT][AttnGeo<D, Q8>::KS];
+    __device__ __forceinline__ void load(const uint16_t* q0, int64_t qs, const AttnItem& it, const AttnSplit& S, int head,
+                                         int m0, int lane) {
+        const int u = lane & 15, w = lane >> 4;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int idx = it.tile * S.M + m0 + 16 * m + u;
+            const bool live = idx < it.rows * S.G;
+            const uint16_t* p = q0 + (it.first + (live ? idx / S.G : 0)) * qs + (head * S.G + (live ? idx % S.G : 0)) * D;
+#pragma unroll
+            for (int c = 0; c < AttnGeo<D, Q8>::KS; ++c) {
+                // (the keys' 16-byte loads hold 16 dims of an 8-bit row, 8 of a bf16 one)
+                const int d = Q8 ? 64 * (c >> 1) + 16 * w + 8 * (c & 1) : 32 * c + 8 * w;
+                q[m][c] = live ? *reinterpret_cast<const uintx4*>(p + d) : (uintx4){0, 0, 0, 0};
+            }
+        }
+    }
+};
+
+// The running softmax of a wave's queries and its sum of the values.
+template <int D, bool Q8, int MT>
+struct AttnState {
+    using Geo = AttnGeo<D, Q8>;
+    floatx4 o[MT][Geo::E];
+    float top[MT], sum[MT];  // sum: of the lane's own tokens
+    int lim[MT];             // tokens that the query sees
+
+    __device__ __forceinline__ void clear(const AttnItem& it, const AttnSplit& S, int m0, int lane) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int idx = it.tile * S.M + m0 + 16 * m + (lane & 15);
+            lim[m] = idx < it.rows * S.G ? attn_see(it, idx / S.G) : 0;
+            top[m] = -INFINITY;
+            sum[m] = 0.0f;
+#pragma unroll
+            for (int o_ = 0; o_ < Geo::E; ++o_) o[m][o_] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    // Scores of the 32 tokens from `base`, the new maxima, and the probabilities as the second
+    // product's B operand. MASKED: some query of the wave does not see all of them.
+    __device__ __forceinline__ void scores(const KeyTile<D, Q8>& k, const QueryTile<D, Q8, MT>& q, float c, int base,
+                                           bool masked, int lane, float (&p)[MT][8]) {
+        const int w = lane >> 4;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            floatx4 s[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                s[a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (!Q8) {
+#pragma unroll
+                    for (int i = 0; i < Geo::KS; ++i) s[a] = mfma(k.k[a][i], q.q[m][i], s[a]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < Geo::KS; ++i) {
+                        // codes are integers of at most 8 bits: exact in bf16
+                        const uint32_t x = k.k[a][i >> 1][2 * (i & 1)], y = k.k[a][i >> 1][2 * (i & 1) + 1];
+                        const uintx4 b = {pack_bf16(code_f(x, 0), code_f(x, 1)), pack_bf16(code_f(x, 2), code_f(x, 3)),
+                                          pack_bf16(code_f(y, 0), code_f(y, 1)), pack_bf16(code_f(y, 2), code_f(y, 3))};
+                        s[a] = mfma(b, q.q[m][i], s[a]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+            float best = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float x = s[j >> 2][j & 3] * c;
+                if constexpr (Q8) x *= k.s[j >> 2][j & 3];
+                if (masked) x = base + 8 * w + j < lim[m] ? x : -INFINITY;
+                p[m][j] = x;
+                best = fmaxf(best, x);
+            }
+            best = fmaxf(best, xor_lane_f<16>(best));
+            best = fmaxf(best, xor_lane_f<32>(best));
+            if (__any(best > top[m])) {  // rare after the first tokens: the sums are brought to the new maximum
+                const float now = fmaxf(best, top[m]);
+                const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[m] - now);
+                top[m] = now;
+                sum[m] *= keep;
+#pragma unroll
+                for (int o_ = 0; o_ < Geo::E; ++o_) o[m][o_] *= keep;
+            }
+            // (no seen token yet: the scores are -inf, and so are their differences from 0)
+            const float ref = top[m] == -INFINITY ? 0.0f : top[m];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[m][j] = __builtin_amdgcn_exp2f(p[m][j] - ref);
+                sum[m] += p[m][j];
+            }
+        }
+    }
+
+    // O^T += V^T P^T; the probabilities, at most 1, are rounded to bf16 for it (with the value's
+    // scale in a Q8 cache): half a step of each against the value it multiplies, as the output's
+    // own rounding; their sum is taken unrounded.
+    __device__ __forceinline__ void values(const ValueTile<D, Q8>& t, const float (&p)[MT][8], int base, int lane) {
+        uintx4 b[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = p[m][j];
+                // (an unseen token's scale may be anything)
+                if constexpr (Q8) x[j] = base + 8 * (lane >> 4) + j < lim[m] ? x[j] * t.s[j >> 2][j & 3] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[m][j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+        }
+#pragma unroll
+        for (int o_ = 0; o_ < Geo::E; ++o_) {
+            uintx4 a;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (Q8)
+                    a[j] = pack_bf16(code_f(t.v[2 * j][o_ >> 2], o_ & 3), code_f(t.v[2 * j + 1][o_ >> 2], o_ & 3));
+                else
+                    a[j] = __builtin_amdgcn_perm(t.v[2 * j + 1][o_ >> 1], t.v[2 * j][o_ >> 1],
+                                                 o_ & 1 ? 0x07060302u : 0x05040100u);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) o[m][o_] = mfma(a, b[m], o[m][o_]);
+            // (an operand or two at a time: formed all at once they would take the tile's size again)
+            if (o_ & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+// bf16 values in steps that not every query of a tile sees whole. A product of a probability 0 and
+// an infinity or NaN is NaN, so tokens that nobody sees and elements that are not finite are
+// cleared; true where a seen one was not finite (add_special then gives it to the queries that see it).
+__device__ __forceinline__ uint32_t special_mask(uint32_t x) {
+    return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+template <int D>
+__device__ __forceinline__ bool clean_values(ValueTile<D, false>& t, int base, int see, int lane) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const bool dead = base + 8 * (lane >> 4) + j >= see;
+#pragma unroll
+        for (int i = 0; i < AttnGeo<D, false>::VD; ++i) {
+            const uint32_t x = dead ? 0u : t.v[j][i], m = special_mask(x);
+            any |= m;
+            t.v[j][i] = x & ~m;
+        }
+    }
+    return __any(any != 0);
+}
+// To the wave's sums in LDS (row u: its queries): the non-finite values of the 32 tokens from base
+// times their probabilities. Never needed by a healthy model; lanes take turns, so that the sums
+// have one order.
+template <int D, int MT>
+__device__ __forceinline__ void add_special(const PagedCacheDev& C, HalfRows at, int base,
+                                            const float (&p)[MT][8], const int (&lim)[MT], float* sums, int stride,
+                                            int lane) {
+    const int u = lane & 15, w = lane >> 4;
+    const uint16_t* v = static_cast<const uint16_t*>(C.values) + (at.of(w >> 1) + (8 * w & 15)) * D;
+    for (int turn = 0; turn < 4; ++turn)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (turn == w && base + 8 * w + j < lim[m])
+                    for (int d = 0; d < D; ++d) {
+                        const uint16_t x = v[j * D + d];
+                        if ((x & 0x7f80u) == 0x7f80u) sums[(16 * m + u) * stride + d] += p[m][j] * bf2f(x);
+                    }
+}
+
+constexpr int kSplitWaves = 4;                 // waves of a workgroup
+constexpr int kSplitTokens = 32 * kSplitWaves; // tokens of a step
+
+// Where the share's first step lies: the sequence that holds step w * share of the list, and that
+// sequence's first step. Returns the list's length. All threads take part; seqs <= 256 are weighed once.
+__device__ __forceinline__ int64_t find_share(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t w, int64_t W,
+                                              int* seq, int64_t* seq_start, int64_t* share) {
+    __shared__ int64_t sums[4], hit_start;
+    __shared__ int hit;
+    const int tid = threadIdx.x, lane = tid & 63;
+    int64_t total = 0, mine = 0;
+    for (int s0 = 0; s0 < B.seqs; s0 += 256) {
+        mine = s0 + tid < B.seqs ? attn_weight(S, B, shift, s0 + tid) : 0;
+        int64_t sum = mine;
+        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) sums[tid >> 6] = sum;
+        __syncthreads();
+        total += sums[0] + sums[1] + sums[2] + sums[3];
+        __syncthreads();
+    }
+    *share = (total + W - 1) / W;
+    const int64_t want = w * *share;
+    if (want >= total) return total;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < B.seqs; s0 += 256) {
+        if (B.seqs > 256) mine = s0 + tid < B.seqs ? attn_weight(S, B, shift, s0 + tid) : 0;
+        int64_t upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
+        }
+        if (lane == 63) sums[tid >> 6] = upto;
+        __syncthreads();
+        int64_t start = before + upto - mine;
+        for (int i = 0; i < (tid >> 6); ++i) start += sums[i];
+        before += sums[0] + sums[1] + sums[2] + sums[3];
+        if (want >= start && want < start + mine) {
+            hit = s0 + tid;
+            hit_start = start;
+        }
+        __syncthreads();
+        if (before > want) break;
+    }
+    *seq = hit;
+    *seq_start = hit_start;
+    return total;
+}
+
+// A workgroup's share of a kv head's steps; wave i takes tokens 32 i .. 32 i + 31 of every step, the
+// next step's keys and values in flight, and the waves' sums are joined through LDS at the end of
+// a piece. Few queries per token: bound by the cache's bytes.
+template <int D, bool Q8, int MT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCacheDev C, PagedBatchDev B, int G,
+                                                                           const uint16_t* __restrict__ q, int64_t qs,
+                                                                           float c, uint16_t* __restrict__ out, int64_t os,
+                                                                           float* __restrict__ part) {
+    using Geo = AttnGeo<D, Q8>;
+    constexpr int M = 16 * MT, LR = D + 4;  // (rows of the waves' sums padded: 16 bytes move the banks)
+    extern __shared__ float lds[];          // [waves][M][LR], then [waves][M] maxima and sums
+    const AttnSplit S{G, M, kSplitTokens};
+    const int w = blockIdx.x, W = gridDim.x, head = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int seq = 0;
+    int64_t seq_start = 0, share = 0;
+    const int64_t total = find_share(S, B, C.shift, w, W, &seq, &seq_start, &share);
+    int64_t pos = w * share;
+    const int64_t end = min(total, pos + share);
+    AttnPiece pc;
+    while (attn_next(S, B, C.shift, end, &seq, &seq_start, &pos, &pc)) {
+        const AttnItem& it = pc.it;
+        PageWalk walk{B.table + static_cast<int64_t>(it.seq) * B.width, C.shift, C.pages, C.hkv, head, it.see, it.bad};
+        // tokens that every query of the tile sees: steps below need no mask
+        const int all = attn_see(it, it.tile * M / G);
+        QueryTile<D, Q8, MT> qt;
+        AttnState<D, Q8, MT> st;
+        qt.load(q, qs, it, S, head, 0, lane);
+        st.clear(it, S, 0, lane);
+        KeyTile<D, Q8> kt;
+        ValueTile<D, Q8> vt;
+        int base = pc.from * kSplitTokens + 32 * wave;
+        const int stop = min(pc.to * kSplitTokens, it.see);
+        HalfRows at{0, 0};
+        float p[MT][8];
+        // (a tile's rows are at most M apart: a masked step is the wave's last of the piece, so `p` and
+        // `base` are still its own after the loop)
+        static_assert(M <= 32, "one masked step per wave");
+        bool special = false;
+        if (base < stop) {
+            at = walk.rows(base);
+            load_keys<D, Q8>(C, at, lane, kt);
+            load_values<D, Q8>(C, at, lane, vt);
+            if (base + kSplitTokens < stop) at = walk.rows(base + kSplitTokens);
+        }
+        for (; base < stop; base += kSplitTokens) {
+            const bool more = base + kSplitTokens < stop, masked = base + 32 > all;
+            st.scores(kt, qt, c, base, masked, lane, p);
+            if (more) load_keys<D, Q8>(C, at, lane, kt);
+            if constexpr (!Q8)
+                if (masked) special = clean_values<D>(vt, base, it.see, lane);
+            st.values(vt, p, base, lane);
+            if (more) load_values<D, Q8>(C, at, lane, vt);
+            if (base + 2 * kSplitTokens < stop) at = walk.rows(base + 2 * kSplitTokens);
+        }
+        // join the waves
+        float* stats = lds + kSplitWaves * M * LR;
+        __syncthreads();  // (the previous piece's sums have been read)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float sum = st.sum[m];
+            sum += xor_lane_f<16>(sum);
+            sum += xor_lane_f<32>(sum);
+            if (walk.bad) sum = kNan;
+            const int row = 16 * m + (lane & 15);
+            if (lane < 16) {
+                stats[wave * M + row] = st.top[m];
+                stats[(kSplitWaves + wave) * M + row] = sum;
+            }
+            float* dst = lds + (wave * M + row) * LR;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int o = 0; o < Geo::E; o += 4)
+                    *reinterpret_cast<floatx4*>(dst + Geo::dim(4 * (lane >> 4) + r, o)) =
+                        (floatx4){st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
+        }
+        if constexpr (!Q8)
+            if (special) {
+                at = walk.rows(base - kSplitTokens);
+                add_special<D, MT>(C, at, base - kSplitTokens, p, st.lim, lds + wave * M * LR, LR, lane);
+            }
+        __syncthreads();
+        const bool whole = pc.to - pc.from == it.steps;
+        float* pd = nullptr;
+        if (!whole) pd = part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(pc.start, share, w)) * (M * (D + 2));
+        for (int e = threadIdx.x; e < M * D / 4; e += 256) {
+            const int row = e / (D / 4), d = e % (D / 4) * 4, idx = it.tile * M + row;
+            if (idx >= it.rows * G) continue;
+            float top = stats[row];
+#pragma unroll
+            for (int i = 1; i < kSplitWaves; ++i) top = fmaxf(top, stats[i * M + row]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+            floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kSplitWaves; ++i) {
+                const float f = __builtin_amdgcn_exp2f(stats[i * M + row] - ref);
+                sum += stats[(kSplitWaves + i) * M + row] * f;
+                o += *reinterpret_cast<const floatx4*>(lds + (i * M + row) * LR + d) * f;
+            }
+            if (whole) {
+                const float inv = it.bad || attn_see(it, idx / G) > 0 ? 1.0f / sum : 0.0f;
+                const uint2 x = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+                *reinterpret_cast<uint2*>(out + (it.first + idx / G) * os + (head * G + idx % G) * D + d) = x;
+            } else {
+                *reinterpret_cast<floatx4*>(pd + row * D + d) = o;
+                if (d == 0) pd[M * D + row] = top, pd[M * D + M + row] = sum;
+            }
+        }
+    }
+}
+
+// Joins the pieces of the items that more than one share worked on: a wave per (row, query head).
+template <int D>
+__global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchDev B, AttnSplit S, int hq, int W,
+                                                    const float* __restrict__ part, uint16_t* __restrict__ out, int64_t os) {
+    const int row = blockIdx.x, lane = threadIdx.x & 63, G = S.G, M = S.M;
+    const int h = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const int seq = row_sequence(B.off, B.seqs, row);
+    if (seq < 0) return;
+    // the list's length, and the steps in front of the sequence
+    int64_t total = 0, start = 0;
+    for (int s = lane; s < B.seqs; s += 64) {
+        const int n = attn_weight(S, B, C.shift, s);
+        total += n;
+        if (s < seq) start += n;
+    }
+    for (int d = 32; d >= 1; d >>= 1) {
+        total += __shfl_xor(total, d);
+        start += __shfl_xor(start, d);
+    }
+    if (h >= hq) return;
+    const int64_t share = (total + W - 1) / W;
+    AttnItem it;
+    attn_sequence(B, C.shift, seq, &it);
+    const int idx = (row - it.first) * G + h % G, head = h / G;
+    for (int j = 0; j < idx / M; ++j) {
+        attn_tile(S, j, &it);
+        start += it.steps;
+    }
+    attn_tile(S, idx / M, &it);
+    const int w0 = static_cast<int>(start / share), w1 = static_cast<int>((start + it.steps - 1) / share);
+    if (w0 == w1) return;
+    const int at = idx % M;
+    auto piece = [&](int w) {
+        return part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(start, share, w)) * (M * (D + 2));
+    };
+    constexpr int E = D / 64;
+    float top = -INFINITY, sum = 0.0f, o[E] = {};
+    for (int p0 = w0; p0 <= w1; p0 += 64) {
+        const bool live = p0 + lane <= w1;
+        const float* mine = piece(live ? p0 + lane : w1);
+        const float mt = live ? mine[M * D + at] : -INFINITY, ms = live ? mine[M * D + M + at] : 0.0f;
+        const float now = fmaxf(top, wave_max(mt)), ref = now == -INFINITY ? 0.0f : now;
+        const float keep = __builtin_amdgcn_exp2f(top - ref), f = live ? __builtin_amdgcn_exp2f(mt - ref) : 0.0f;
+        top = now;
+        sum = sum * keep + wave_sum_xor(ms * f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= keep;
+        const int n = min(64, w1 - p0 + 1);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float* src = piece(p0 + i) + at * D + lane * E;
+            const float fi = __shfl(f, i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], fi, o[e]);
+        }
+    }
+    const float inv = it.bad || attn_see(it, idx / G) > 0 ? 1.0f / sum : 0.0f;
+    uint16_t* dst = out + row * os + h * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = f2bf(o[e] * inv);
 }
 
 } // namespace
@@ -130,14 +605,60 @@ hipError_t launch_paged_append(const PagedCacheDev& C, bool q8, const PagedBatch
     return C.d == 64 ? go(k_paged_append<64, false>) : C.d == 128 ? go(k_paged_append<128, false>) : go(k_paged_append<256, false>);
 }
 
-size_t paged_attention_ws(const PagedCacheDev&, const PagedBatchDev&, int, int) { return 0; }
+namespace {
 
-hipError_t launch_paged_attention(const PagedCacheDev& C, bool q8, const PagedBatchDev& B, int, const uint16_t* q,
-                                  int64_t qs, int hq, float scale, uint16_t* out, int64_t os, void*, hipStream_t st) {
-    const dim3 grid(B.rows, hq);
-    auto go = [&](auto kern) { return launch(kern, grid, dim3(64), 0, st, C, B, q, qs, hq, scale, out, os); };
-    if (q8) return C.d == 64 ? go(k_paged_attn<64, true>) : C.d == 128 ? go(k_paged_attn<128, true>) : go(k_paged_attn<256, true>);
-    return C.d == 64 ? go(k_paged_attn<64, false>) : C.d == 128 ? go(k_paged_attn<128, false>) : go(k_paged_attn<256, false>);
+// Workgroups per kv head of the split kernel: the chip's 256 CUs at the kernel's occupancy.
+struct SplitPlan {
+    int mt, W;
+    bool joined;
+};
+SplitPlan split_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
+    SplitPlan p;
+    p.mt = static_cast<int64_t>(max_rows) * (hq / C.hkv) <= 16 ? 1 : 2;
+    const int per_cu = C.d == 256 ? 1 : 2;
+    p.W = std::max(1, 256 * per_cu / C.hkv);
+    // no sequence of the table is longer than a step: nothing is ever split
+    p.joined = (static_cast<int64_t>(B.width) << C.shift) > kSplitTokens;
+    return p;
+}
+
+template <int D, bool Q8, int MT>
+hipError_t launch_split(const PagedCacheDev& C, const PagedBatchDev& B, const SplitPlan& p, const uint16_t* q, int64_t qs,
+                        int hq, float scale, uint16_t* out, int64_t os, float* part, hipStream_t st) {
+    constexpr int M = 16 * MT;
+    constexpr size_t lds = (static_cast<size_t>(kSplitWaves) * M * (D + 4) + 2 * kSplitWaves * M) * 4;
+    const float c = scale * 1.44269504088896341f;  // exponents of 2
+    const int G = hq / C.hkv;
+    hipError_t e = ensure_lds<k_paged_split<D, Q8, MT>>(lds);
+    if (e != hipSuccess) return e;
+    e = launch(k_paged_split<D, Q8, MT>, dim3(p.W, C.hkv), dim3(256), lds, st, C, B, G, q, qs, c, out, os, part);
+    if (e != hipSuccess || !p.joined) return e;
+    return launch(k_paged_join<D>, dim3(B.rows, (hq + 3) / 4), dim3(256), 0, st, C, B, AttnSplit{G, M, kSplitTokens}, hq,
+                  p.W, part, out, os);
+}
+
+} // namespace
+
+size_t paged_attention_ws(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
+    const SplitPlan p = split_plan(C, B, max_rows, hq);
+    return p.joined ? static_cast<size_t>(C.hkv) * p.W * 2 * 16 * p.mt * (C.d + 2) * 4 : 0;
+}
+
+hipError_t launch_paged_attention(const PagedCacheDev& C, bool q8, const PagedBatchDev& B, int max_rows, const uint16_t* q,
+                                  int64_t qs, int hq, float scale, uint16_t* out, int64_t os, void* ws, hipStream_t st) {
+    const SplitPlan p = split_plan(C, B, max_rows, hq);
+    auto go = [&](auto d, auto c8) {
+        constexpr int D = decltype(d)::value;
+        constexpr bool Q8 = decltype(c8)::value;
+        auto* kern = p.mt == 1 ? launch_split<D, Q8, 1> : launch_split<D, Q8, 2>;
+        return kern(C, B, p, q, qs, hq, scale, out, os, static_cast<float*>(ws), st);
+    };
+    auto dims = [&](auto c8) {
+        return C.d == 64    ? go(std::integral_constant<int, 64>{}, c8)
+               : C.d == 128 ? go(std::integral_constant<int, 128>{}, c8)
+                            : go(std::integral_constant<int, 256>{}, c8);
+    };
+    return q8 ? dims(std::true_type{}) : dims(std::false_type{});
 }
 
 } // namespace q38
