@@ -739,7 +739,7 @@ typedef struct q38_paged_cache {
  * pages (a common prefix) that no call writes. */
 typedef struct q38_paged_batch {
     int32_t sequences;          /* 0..4096                                                     */
-    int32_t rows;               /* rows of the call's tensors, at most 2^24                     */
+    int32_t rows;               /* rows of the call's tensors, at most 2^19                     */
     int32_t max_rows;           /* rows of the longest sequence (a hint), 1..rows               */
     int32_t table_pages;        /* columns of page_table; table_pages * page_tokens < 2^30     */
     const int32_t* row_offsets; /* device [sequences + 1], ascending                           */
@@ -797,7 +797,7 @@ typedef struct q38_delta_desc {
 } q38_delta_desc;
 typedef struct q38_delta_batch {
     int32_t sequences;           /* 0..4096                                                    */
-    int32_t rows;                /* at most 2^24                                               */
+    int32_t rows;                /* at most 2^19                                               */
     int32_t max_rows;            /* rows of the longest sequence (a hint), 1..rows             */
     int32_t slots;
     const int32_t* row_offsets;  /* device [sequences + 1], ascending                          */

@@ -2226,7 +2226,7 @@ int check_paged(const char* name, const q38_paged_cache* c, const q38_paged_batc
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return fail(Q38_EINVAL, at + "head_dim must be 64, 128 or 256");
     if (b->sequences < 0 || b->sequences > kBatchMaxSeqs || b->rows < 0 || b->rows > kBatchMaxRows)
-        return fail(Q38_EINVAL, at + "sequences must be 0..4096, rows 0..2^24");
+        return fail(Q38_EINVAL, at + "sequences must be 0..4096, rows 0..2^19");
     if (b->rows > 0 && b->sequences > 0 && (b->max_rows < 1 || b->max_rows > b->rows))
         return fail(Q38_EINVAL, at + "max_rows must be 1..rows");
     if (b->table_pages < 1 || static_cast<int64_t>(b->table_pages) * c->page_tokens >= (int64_t{1} << 30))
@@ -2313,7 +2313,7 @@ static int check_delta(const char* name, const q38_delta_desc* d, const q38_delt
         return fail(Q38_EINVAL, at + "value heads must be divisible by key heads, at most 256");
     if (!std::isfinite(d->scale)) return fail(Q38_EINVAL, at + "scale must be finite");
     if (b->sequences < 0 || b->sequences > kBatchMaxSeqs || b->rows < 0 || b->rows > kBatchMaxRows || b->slots < 0)
-        return fail(Q38_EINVAL, at + "sequences must be 0..4096, rows 0..2^24, slots not negative");
+        return fail(Q38_EINVAL, at + "sequences must be 0..4096, rows 0..2^19, slots not negative");
     if (b->rows > 0 && b->sequences > 0 && (b->max_rows < 1 || b->max_rows > b->rows))
         return fail(Q38_EINVAL, at + "max_rows must be 1..rows");
     *D = DeltaDev{};

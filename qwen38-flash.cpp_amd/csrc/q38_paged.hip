@@ -5,13 +5,14 @@
 //                    8-bit codes and scale
 //   k_paged_split    attention of few queries per sequence: equal shares of all sequences' tokens,
 //                    one pass with the running maximum and sum of the softmax
-//   k_paged_join     the shares' pieces of a sequence joined
+//   k_paged_tile     attention of many queries per sequence: tiles of 128 or 256 of them over keys
+//                    and values staged in LDS
+//   k_paged_join     the pieces of a sequence that several workgroups worked on
 #include "q38_device.hpp"
 #include "q38_paged.hpp"
 #include "q38_internal.hpp"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace q38 {
 
@@ -199,8 +200,9 @@ __device__ __forceinline__ void load_values(const PagedCacheDev& C, HalfRows at,
 template <int D, bool Q8, int MT>
 struct QueryTile {
     uintx4 q[MT][AttnGeo<D, Q8>::KS];
+    // (a negative scale turns the queries' signs, so that the softmax's factor is not negative)
     __device__ __forceinline__ void load(const uint16_t* q0, int64_t qs, const AttnItem& it, const AttnSplit& S, int head,
-                                         int m0, int lane) {
+                                         int m0, bool negate, int lane) {
         const int u = lane & 15, w = lane >> 4;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -211,7 +213,7 @@ struct QueryTile {
             for (int c = 0; c < AttnGeo<D, Q8>::KS; ++c) {
                 // (the keys' 16-byte loads hold 16 dims of an 8-bit row, 8 of a bf16 one)
                 const int d = Q8 ? 64 * (c >> 1) + 16 * w + 8 * (c & 1) : 32 * c + 8 * w;
-                q[m][c] = live ? *reinterpret_cast<const uintx4*>(p + d) : (uintx4){0, 0, 0, 0};
+                q[m][c] = live ? *reinterpret_cast<const uintx4*>(p + d) ^ (negate ? 0x80008000u : 0u) : (uintx4){0, 0, 0, 0};
             }
         }
     }
@@ -237,11 +239,48 @@ struct AttnState {
         }
     }
 
-    // Scores of the 32 tokens from `base`, the new maxima, and the probabilities as the second
-    // product's B operand. MASKED: some query of the wave does not see all of them.
+    // From the 32 tokens' products of query group m: the new maximum, the probabilities as the
+    // second product's B operand, and their sum. MASKED steps: some query does not see all tokens.
+    __device__ __forceinline__ void soften(int m, const floatx4 (&s)[2], const floatx4 (&ks)[2], float c, int base,
+                                           bool masked, int lane, float (&p)[8]) {
+        const int first = base + 8 * (lane >> 4);
+        float best = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = s[j >> 2][j & 3];
+            if constexpr (Q8) p[j] *= ks[j >> 2][j & 3];
+        }
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = first + j < lim[m] ? p[j] : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) best = fmaxf(best, p[j]);
+        best = fmaxf(best, xor_lane_f<16>(best));
+        best = fmaxf(best, xor_lane_f<32>(best));
+        best = best == -INFINITY ? best : best * c;  // (c may be 0)
+        if (__any(best > top[m])) {  // rare after the first tokens: the sums are brought to the new maximum
+            const float now = fmaxf(best, top[m]);
+            const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[m] - now);
+            top[m] = now;
+            sum[m] *= keep;
+#pragma unroll
+            for (int o_ = 0; o_ < Geo::E; ++o_) o[m][o_] *= keep;
+        }
+        // (no seen token yet: the scores are -inf, and so are their differences from 0)
+        const float ref = top[m] == -INFINITY ? 0.0f : top[m];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], c, -ref));
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = first + j < lim[m] ? p[j] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[m] += p[j];
+    }
+
     __device__ __forceinline__ void scores(const KeyTile<D, Q8>& k, const QueryTile<D, Q8, MT>& q, float c, int base,
                                            bool masked, int lane, float (&p)[MT][8]) {
-        const int w = lane >> 4;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             floatx4 s[2];
@@ -263,40 +302,15 @@ struct AttnState {
                     }
                 }
             }
-            float best = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float x = s[j >> 2][j & 3] * c;
-                if constexpr (Q8) x *= k.s[j >> 2][j & 3];
-                if (masked) x = base + 8 * w + j < lim[m] ? x : -INFINITY;
-                p[m][j] = x;
-                best = fmaxf(best, x);
-            }
-            best = fmaxf(best, xor_lane_f<16>(best));
-            best = fmaxf(best, xor_lane_f<32>(best));
-            if (__any(best > top[m])) {  // rare after the first tokens: the sums are brought to the new maximum
-                const float now = fmaxf(best, top[m]);
-                const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[m] - now);
-                top[m] = now;
-                sum[m] *= keep;
-#pragma unroll
-                for (int o_ = 0; o_ < Geo::E; ++o_) o[m][o_] *= keep;
-            }
-            // (no seen token yet: the scores are -inf, and so are their differences from 0)
-            const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p[m][j] = __builtin_amdgcn_exp2f(p[m][j] - ref);
-                sum[m] += p[m][j];
-            }
+            soften(m, s, k.s, c, base, masked, lane, p[m]);
         }
     }
 
     // O^T += V^T P^T; the probabilities, at most 1, are rounded to bf16 for it (with the value's
     // scale in a Q8 cache): half a step of each against the value it multiplies, as the output's
     // own rounding; their sum is taken unrounded.
-    __device__ __forceinline__ void values(const ValueTile<D, Q8>& t, const float (&p)[MT][8], int base, int lane) {
-        uintx4 b[MT];
+    __device__ __forceinline__ void weights(const float (&p)[MT][8], const floatx4 (&vs)[2], int base, int lane,
+                                            uintx4 (&b)[MT]) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float x[8];
@@ -304,17 +318,20 @@ struct AttnState {
             for (int j = 0; j < 8; ++j) {
                 x[j] = p[m][j];
                 // (an unseen token's scale may be anything)
-                if constexpr (Q8) x[j] = base + 8 * (lane >> 4) + j < lim[m] ? x[j] * t.s[j >> 2][j & 3] : 0.0f;
+                if constexpr (Q8) x[j] = base + 8 * (lane >> 4) + j < lim[m] ? x[j] * vs[j >> 2][j & 3] : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) b[m][j] = pack_bf16(x[2 * j], x[2 * j + 1]);
         }
+    }
+    template <bool CODES>  // the values as 8-bit codes, not as bf16
+    __device__ __forceinline__ void products(const ValueTile<D, CODES>& t, const uintx4 (&b)[MT]) {
 #pragma unroll
         for (int o_ = 0; o_ < Geo::E; ++o_) {
             uintx4 a;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (Q8)
+                if constexpr (CODES)
                     a[j] = pack_bf16(code_f(t.v[2 * j][o_ >> 2], o_ & 3), code_f(t.v[2 * j + 1][o_ >> 2], o_ & 3));
                 else
                     a[j] = __builtin_amdgcn_perm(t.v[2 * j + 1][o_ >> 1], t.v[2 * j][o_ >> 1],
@@ -326,11 +343,24 @@ struct AttnState {
             if (o_ & 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
+    __device__ __forceinline__ void values(const ValueTile<D, Q8>& t, const float (&p)[MT][8], int base, int lane) {
+        uintx4 b[MT];
+        weights(p, t.s, base, lane, b);
+        products<Q8>(t, b);
+    }
+    // the same for values widened to bf16 on their way, with their scales beside them
+    __device__ __forceinline__ void values16(const ValueTile<D, false>& t, const floatx4 (&vs)[2], const float (&p)[MT][8],
+                                             int base, int lane) {
+        uintx4 b[MT];
+        weights(p, vs, base, lane, b);
+        products<false>(t, b);
+    }
 };
 
 // bf16 values in steps that not every query of a tile sees whole. A product of a probability 0 and
 // an infinity or NaN is NaN, so tokens that nobody sees and elements that are not finite are
-// cleared; true where a seen one was not finite (add_special then gives it to the queries that see it).
+// cleared; true where a seen one was not finite (never, in a healthy model): the outputs of the
+// queries that see it take it at the end (add_special).
 __device__ __forceinline__ uint32_t special_mask(uint32_t x) {
     return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
@@ -349,25 +379,21 @@ __device__ __forceinline__ bool clean_values(ValueTile<D, false>& t, int base, i
     }
     return __any(any != 0);
 }
-// To the wave's sums in LDS (row u: its queries): the non-finite values of the 32 tokens from base
-// times their probabilities. Never needed by a healthy model; lanes take turns, so that the sums
-// have one order.
-template <int D, int MT>
-__device__ __forceinline__ void add_special(const PagedCacheDev& C, HalfRows at, int base,
-                                            const float (&p)[MT][8], const int (&lim)[MT], float* sums, int stride,
-                                            int lane) {
-    const int u = lane & 15, w = lane >> 4;
-    const uint16_t* v = static_cast<const uint16_t*>(C.values) + (at.of(w >> 1) + (8 * w & 15)) * D;
-    for (int turn = 0; turn < 4; ++turn)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (turn == w && base + 8 * w + j < lim[m])
-                    for (int d = 0; d < D; ++d) {
-                        const uint16_t x = v[j * D + d];
-                        if ((x & 0x7f80u) == 0x7f80u) sums[(16 * m + u) * stride + d] += p[m][j] * bf2f(x);
-                    }
+// The first token of the steps that a tile's queries do not see whole.
+__device__ __forceinline__ int special_from(int all) { return all & ~31; }
+// Dims d .. d + 3 of a query's sum, with the non-finite values of the tokens t0 .. lim - 1 (their
+// weights are positive: an infinity or NaN comes out whatever they are).
+template <int D>
+__device__ __forceinline__ floatx4 add_special(const PagedCacheDev& C, const int32_t* table, int head, int t0, int lim,
+                                               int d, floatx4 x) {
+    for (int t = t0; t < lim; ++t) {
+        const int64_t at = cache_row(table[t >> C.shift], C.pages, C.hkv, head, C.shift, t);
+        if (at < 0) continue;
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(C.values) + at * D + d);
+        const uint32_t m0 = special_mask(v.x), m1 = special_mask(v.y);
+        x[0] += bflo(v.x & m0), x[1] += bfhi(v.x & m0), x[2] += bflo(v.y & m1), x[3] += bfhi(v.y & m1);
+    }
+    return x;
 }
 
 constexpr int kSplitWaves = 4;                 // waves of a workgroup
@@ -429,6 +455,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
     using Geo = AttnGeo<D, Q8>;
     constexpr int M = 16 * MT, LR = D + 4;  // (rows of the waves' sums padded: 16 bytes move the banks)
     extern __shared__ float lds[];          // [waves][M][LR], then [waves][M] maxima and sums
+    __shared__ int flags[kSplitWaves];
     const AttnSplit S{G, M, kSplitTokens};
     const int w = blockIdx.x, W = gridDim.x, head = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -445,17 +472,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         const int all = attn_see(it, it.tile * M / G);
         QueryTile<D, Q8, MT> qt;
         AttnState<D, Q8, MT> st;
-        qt.load(q, qs, it, S, head, 0, lane);
+        qt.load(q, qs, it, S, head, 0, c < 0.0f, lane);
         st.clear(it, S, 0, lane);
         KeyTile<D, Q8> kt;
         ValueTile<D, Q8> vt;
         int base = pc.from * kSplitTokens + 32 * wave;
         const int stop = min(pc.to * kSplitTokens, it.see);
         HalfRows at{0, 0};
-        float p[MT][8];
-        // (a tile's rows are at most M apart: a masked step is the wave's last of the piece, so `p` and
-        // `base` are still its own after the loop)
-        static_assert(M <= 32, "one masked step per wave");
         bool special = false;
         if (base < stop) {
             at = walk.rows(base);
@@ -465,10 +488,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         }
         for (; base < stop; base += kSplitTokens) {
             const bool more = base + kSplitTokens < stop, masked = base + 32 > all;
-            st.scores(kt, qt, c, base, masked, lane, p);
+            float p[MT][8];
+            st.scores(kt, qt, fabsf(c), base, masked, lane, p);
             if (more) load_keys<D, Q8>(C, at, lane, kt);
             if constexpr (!Q8)
-                if (masked) special = clean_values<D>(vt, base, it.see, lane);
+                if (masked) special |= clean_values<D>(vt, base, it.see, lane);
             st.values(vt, p, base, lane);
             if (more) load_values<D, Q8>(C, at, lane, vt);
             if (base + 2 * kSplitTokens < stop) at = walk.rows(base + 2 * kSplitTokens);
@@ -495,12 +519,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
                     *reinterpret_cast<floatx4*>(dst + Geo::dim(4 * (lane >> 4) + r, o)) =
                         (floatx4){st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
         }
-        if constexpr (!Q8)
-            if (special) {
-                at = walk.rows(base - kSplitTokens);
-                add_special<D, MT>(C, at, base - kSplitTokens, p, st.lim, lds + wave * M * LR, LR, lane);
-            }
+        if (lane == 0) flags[wave] = special;
         __syncthreads();
+        special = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
         const bool whole = pc.to - pc.from == it.steps;
         float* pd = nullptr;
         if (!whole) pd = part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(pc.start, share, w)) * (M * (D + 2));
@@ -519,6 +540,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
                 sum += stats[(kSplitWaves + i) * M + row] * f;
                 o += *reinterpret_cast<const floatx4*>(lds + (i * M + row) * LR + d) * f;
             }
+            if constexpr (!Q8)
+                if (special)
+                    o = add_special<D>(C, walk.table, head, max(special_from(all), pc.from * kSplitTokens),
+                                       min(stop, attn_see(it, idx / G)), d, o);
             if (whole) {
                 const float inv = it.bad || attn_see(it, idx / G) > 0 ? 1.0f / sum : 0.0f;
                 const uint2 x = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
@@ -531,18 +556,258 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
     }
 }
 
-// Joins the pieces of the items that more than one share worked on: a wave per (row, query head).
+// ---- many queries per sequence. A workgroup takes M = 32 x waves queries of one item and one of
+// `splits` equal ranges of its tokens; keys and values go through LDS, TB tokens at a time and the
+// next ones in flight (an 8-bit cache is converted on the way: its codes are exact in bf16), and
+// every wave multiplies them with its own 32 queries. Bound by the matrix cores, by the
+// exponentials beside them (8 per lane for 16 products of 128 dims) and by LDS reads, which 32
+// queries per wave bring to the matrix cores' own time.
 template <int D>
+struct TileGeo {
+    static constexpr int WAVES = D == 256 ? 4 : 8;  // 256 dims: twice the registers, one wave per SIMD
+    static constexpr int M = 32 * WAVES;
+    static constexpr int TB = D == 256 ? 32 : 64;
+    static constexpr int CH = D / 8;                            // 16-byte chunks of a bf16 row
+    static constexpr int PIECES = TB * CH / (64 * WAVES);       // chunks per thread
+    static constexpr size_t kLds = 2 * (2 * static_cast<size_t>(TB) * D * 2 + 2 * TB * 4);
+};
+// Place of a token's chunk in its tile: a wave's 16-byte reads of the keys go down 16 rows, 8 of
+// which (token % 4, token / 8 % 2) get chunks of their own banks.
+template <int D>
+__device__ __forceinline__ int tile_at(int token, int chunk) {
+    return token * (D / 8) + (chunk ^ ((token & 3) | ((token >> 1) & 4)));
+}
+
+// Which item a workgroup takes: the sequences' tiles in order, a sequence's last (longest) first.
+__device__ __forceinline__ bool find_tile(const AttnSplit& S, const PagedBatchDev& B, int shift, int want, AttnItem* it) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = 0; s0 < B.seqs; s0 += 64) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < B.seqs) {
+            const RowSpan span = row_span(B.off, s, B.rows);
+            n = attn_tiles(S, span.end - span.begin);
+        }
+        int upto = n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
+        }
+        const uint64_t past = __ballot(before + upto > want);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            attn_sequence(B, shift, s0 + l, it);
+            const int tiles = __shfl(n, l), start = before + __shfl(upto, l) - tiles;
+            attn_tile(S, tiles - 1 - (want - start), it);
+            return true;
+        }
+        before += __shfl(upto, 63);
+    }
+    return false;
+}
+
+template <int D, bool Q8>
+__global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_paged_tile(
+    PagedCacheDev C, PagedBatchDev B, int G, const uint16_t* __restrict__ q, int64_t qs, float c, uint16_t* __restrict__ out,
+    int64_t os, float* __restrict__ part) {
+    using Geo = AttnGeo<D, false>;
+    using TG = TileGeo<D>;
+    constexpr int TB = TG::TB, NT = 64 * TG::WAVES, CH = TG::CH, PC = TG::PIECES, MT = 2;
+    extern __shared__ uintx4 tiles[];  // [2][keys, values][TB][CH], then [2][key, value scales][TB]
+    float* const scales = reinterpret_cast<float*>(tiles + 4 * TB * CH);
+    const AttnSplit S{G, TG::M, TB};
+    const int head = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int u = lane & 15, w = lane >> 4;
+    AttnItem it;
+    if (!find_tile(S, B, C.shift, blockIdx.x, &it)) return;
+    const int per = (it.steps + gridDim.z - 1) / gridDim.z, from = blockIdx.z * per, to = min(it.steps, from + per);
+    if (from >= to) return;
+    const int m0 = wave * 32, i0 = it.tile * TG::M + m0, rows = it.rows * G;
+    QueryTile<D, false, MT> qt;
+    AttnState<D, Q8, MT> st;
+    qt.load(q, qs, it, S, head, m0, c < 0.0f, lane);
+    st.clear(it, S, m0, lane);
+    c = fabsf(c);
+    // tokens that all, and any, of the wave's queries see
+    const int all = i0 < rows ? attn_see(it, i0 / G) : 0;
+    const int any = i0 < rows ? attn_see(it, min(i0 + 31, rows - 1) / G) : 0;
+    const int stop = min(to * TB, it.see);
+    const int32_t* table = B.table + static_cast<int64_t>(it.seq) * B.width;
+    bool bad = it.bad, special = false;
+
+    // staging: chunk (token, ch) of the tile from thread's piece; pages a tile ahead of the loads
+    int32_t page[PC];
+    uintx4 kr[PC], vr[PC];
+    float sr[2] = {0.0f, 0.0f};
+    auto token_of = [&](int i) { return (static_cast<int>(threadIdx.x) + i * NT) / CH; };
+    const int ch = threadIdx.x % CH;
+    auto pages = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < PC; ++i) page[i] = t0 + token_of(i) < stop ? table[(t0 + token_of(i)) >> C.shift] : 0;
+    };
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int t = t0 + token_of(i);
+            kr[i] = vr[i] = (uintx4){0, 0, 0, 0};
+            if (t >= stop) continue;
+            const int64_t at = cache_row(page[i], C.pages, C.hkv, head, C.shift, t);
+            if (at < 0) {
+                bad = true;
+                continue;
+            }
+            if constexpr (Q8) {
+                const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(C.keys) + at * D + 8 * ch);
+                const uint2 y = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(C.values) + at * D + 8 * ch);
+                kr[i][0] = x.x, kr[i][1] = x.y;
+                vr[i][0] = y.x, vr[i][1] = y.y;
+            } else {
+                kr[i] = *reinterpret_cast<const uintx4*>(static_cast<const uint16_t*>(C.keys) + at * D + 8 * ch);
+                vr[i] = *reinterpret_cast<const uintx4*>(static_cast<const uint16_t*>(C.values) + at * D + 8 * ch);
+            }
+        }
+        if constexpr (Q8) {
+            sr[0] = sr[1] = 0.0f;
+            const int t = t0 + threadIdx.x;
+            if (threadIdx.x < TB && t < stop) {
+                const int64_t at = cache_row(table[t >> C.shift], C.pages, C.hkv, head, C.shift, t);
+                if (at >= 0) sr[0] = C.ks[at], sr[1] = C.vs[at];
+            }
+        }
+    };
+    auto widen = [](uintx4 x) {
+        return (uintx4){pack_bf16(code_f(x[0], 0), code_f(x[0], 1)), pack_bf16(code_f(x[0], 2), code_f(x[0], 3)),
+                        pack_bf16(code_f(x[1], 0), code_f(x[1], 1)), pack_bf16(code_f(x[1], 2), code_f(x[1], 3))};
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int at = tile_at<D>(token_of(i), ch);
+            tiles[(2 * buf) * TB * CH + at] = Q8 ? widen(kr[i]) : kr[i];
+            tiles[(2 * buf + 1) * TB * CH + at] = Q8 ? widen(vr[i]) : vr[i];
+        }
+        if constexpr (Q8)
+            if (threadIdx.x < TB) {
+                scales[2 * buf * TB + threadIdx.x] = sr[0];
+                scales[(2 * buf + 1) * TB + threadIdx.x] = sr[1];
+            }
+    };
+    pages(from * TB);
+    fetch(from * TB);
+    if (from + 1 < to) pages((from + 1) * TB);
+    stage(0);
+    __syncthreads();
+    for (int step = from; step < to; ++step) {
+        const int buf = (step - from) & 1;
+        if (step + 1 < to) {
+            fetch((step + 1) * TB);
+            if (step + 2 < to) pages((step + 2) * TB);
+        }
+        const uintx4* kt = tiles + (2 * buf) * TB * CH;
+        const uintx4* vt = kt + TB * CH;
+#pragma unroll 1
+        for (int sub = 0; sub < TB / 32; ++sub) {
+            const int base = step * TB + 32 * sub;
+            if (base >= any) break;
+            const bool masked = base + 32 > all;
+            floatx4 s[MT][2], ks[2], vs[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) s[m][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+                const int t = 32 * sub + 8 * (u >> 2) + 4 * a + (u & 3);
+#pragma unroll
+                for (int i = 0; i < Geo::KS; ++i) {
+                    const uintx4 k = kt[tile_at<D>(t, 4 * i + w)];
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) s[m][a] = mfma(k, qt.q[m][i], s[m][a]);
+                }
+                if constexpr (Q8) {
+                    const float* sc = scales + 2 * buf * TB + 32 * sub + 8 * w + 4 * a;
+                    ks[a] = *reinterpret_cast<const floatx4*>(sc);
+                    vs[a] = *reinterpret_cast<const floatx4*>(sc + TB);
+                }
+            }
+            float p[MT][8];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) st.soften(m, s[m], ks, c, base, masked, lane, p[m]);
+            ValueTile<D, false> v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int t = 32 * sub + 8 * w + j;
+                if constexpr (D == 64) {
+                    const uint2 x = reinterpret_cast<const uint2*>(vt + tile_at<D>(t, u >> 1))[u & 1];
+                    v.v[j][0] = x.x, v.v[j][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int b = 0; b < D / 128; ++b) {
+                        const uintx4 x = vt[tile_at<D>(t, 16 * b + u)];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v.v[j][4 * b + i] = x[i];
+                    }
+                }
+            }
+            if constexpr (!Q8)
+                if (masked) special |= clean_values<D>(v, base, any, lane);
+            st.values16(v, vs, p, base, lane);
+        }
+        if (step + 1 < to) stage(buf ^ 1);
+        __syncthreads();
+    }
+    bad = __syncthreads_or(bad);
+    const bool whole = per >= it.steps;
+    float* pd = nullptr;
+    if (!whole) pd = part + ((static_cast<int64_t>(blockIdx.x) * C.hkv + head) * gridDim.z + blockIdx.z) * (TG::M * (D + 2));
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        float sum = st.sum[m];
+        sum += xor_lane_f<16>(sum);
+        sum += xor_lane_f<32>(sum);
+        if (bad) sum = kNan;
+        const int idx = i0 + 16 * m + u;
+        if (idx >= rows) continue;
+        const float inv = bad || st.lim[m] > 0 ? 1.0f / sum : 0.0f;
+        const int row = m0 + 16 * m + u;
+        uint16_t* dst = out + (it.first + idx / G) * os + (head * G + idx % G) * D;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int o = 0; o < Geo::E; o += 4) {
+                const int d = Geo::dim(4 * w + r, o);
+                floatx4 x = {st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
+                if constexpr (!Q8)
+                    if (special)
+                        x = add_special<D>(C, table, head, max(special_from(all), from * TB), min(stop, st.lim[m]), d, x);
+                if (whole)
+                    *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
+                else
+                    *reinterpret_cast<floatx4*>(pd + row * D + d) = x;
+            }
+        if (!whole && w == 0) pd[TG::M * D + row] = st.top[m], pd[TG::M * D + TG::M + row] = sum;
+    }
+}
+
+// Joins the pieces of an item that several workgroups worked on, one wave per (row, query head):
+// TILES: those of k_paged_tile, W ranges per item; else those of k_paged_split, W shares.
+template <int D, bool TILES>
 __global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchDev B, AttnSplit S, int hq, int W,
-                                                    const float* __restrict__ part, uint16_t* __restrict__ out, int64_t os) {
+                                                    int items, const float* __restrict__ part,
+                                                    uint16_t* __restrict__ out, int64_t os) {
     const int row = blockIdx.x, lane = threadIdx.x & 63, G = S.G, M = S.M;
     const int h = blockIdx.y * 4 + (threadIdx.x >> 6);
     const int seq = row_sequence(B.off, B.seqs, row);
     if (seq < 0) return;
-    // the list's length, and the steps in front of the sequence
+    // what lies in front of the sequence: steps (and the list's length), or tiles
     int64_t total = 0, start = 0;
-    for (int s = lane; s < B.seqs; s += 64) {
-        const int n = attn_weight(S, B, C.shift, s);
+    for (int s = lane; s < (TILES ? seq : B.seqs); s += 64) {
+        int n;
+        if constexpr (TILES) {
+            const RowSpan span = row_span(B.off, s, B.rows);
+            n = attn_tiles(S, span.end - span.begin);
+        } else {
+            n = attn_weight(S, B, C.shift, s);
+        }
         total += n;
         if (s < seq) start += n;
     }
@@ -551,26 +816,39 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchD
         start += __shfl_xor(start, d);
     }
     if (h >= hq) return;
-    const int64_t share = (total + W - 1) / W;
     AttnItem it;
     attn_sequence(B, C.shift, seq, &it);
-    const int idx = (row - it.first) * G + h % G, head = h / G;
-    for (int j = 0; j < idx / M; ++j) {
-        attn_tile(S, j, &it);
-        start += it.steps;
+    const int idx = (row - it.first) * G + h % G, head = h / G, at = idx % M;
+    int64_t first, step;  // the first piece, and from one to the next
+    int n;
+    if constexpr (TILES) {
+        attn_tile(S, idx / M, &it);
+        const int per = (it.steps + W - 1) / W;
+        n = (it.steps + per - 1) / per;
+        const int64_t item = start + attn_tiles(S, it.rows) - 1 - it.tile;
+        if (item >= items) return;  // (offsets that do not ascend: more tiles than rows)
+        first = (item * C.hkv + head) * W;
+        step = 1;
+    } else {
+        const int64_t share = (total + W - 1) / W;
+        for (int j = 0; j < idx / M; ++j) {
+            attn_tile(S, j, &it);
+            start += it.steps;
+        }
+        attn_tile(S, idx / M, &it);
+        const int64_t w0 = start / share, w1 = (start + it.steps - 1) / share;
+        n = static_cast<int>(w1 - w0) + 1;
+        // (an item goes on behind its first share, whose second slot it takes; it began before the others)
+        first = (static_cast<int64_t>(head) * W + w0) * 2 + 1;
+        step = 2;
     }
-    attn_tile(S, idx / M, &it);
-    const int w0 = static_cast<int>(start / share), w1 = static_cast<int>((start + it.steps - 1) / share);
-    if (w0 == w1) return;
-    const int at = idx % M;
-    auto piece = [&](int w) {
-        return part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(start, share, w)) * (M * (D + 2));
-    };
+    if (n == 1) return;
+    auto piece = [&](int i) { return part + (first + i * step - (!TILES && i > 0)) * (M * (D + 2)); };
     constexpr int E = D / 64;
     float top = -INFINITY, sum = 0.0f, o[E] = {};
-    for (int p0 = w0; p0 <= w1; p0 += 64) {
-        const bool live = p0 + lane <= w1;
-        const float* mine = piece(live ? p0 + lane : w1);
+    for (int p0 = 0; p0 < n; p0 += 64) {
+        const bool live = p0 + lane < n;
+        const float* mine = piece(live ? p0 + lane : n - 1);
         const float mt = live ? mine[M * D + at] : -INFINITY, ms = live ? mine[M * D + M + at] : 0.0f;
         const float now = fmaxf(top, wave_max(mt)), ref = now == -INFINITY ? 0.0f : now;
         const float keep = __builtin_amdgcn_exp2f(top - ref), f = live ? __builtin_amdgcn_exp2f(mt - ref) : 0.0f;
@@ -578,9 +856,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchD
         sum = sum * keep + wave_sum_xor(ms * f);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] *= keep;
-        const int n = min(64, w1 - p0 + 1);
+        const int left = min(64, n - p0);
 #pragma unroll 4
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < left; ++i) {
             const float* src = piece(p0 + i) + at * D + lane * E;
             const float fi = __shfl(f, i);
 #pragma unroll
@@ -607,58 +885,84 @@ hipError_t launch_paged_append(const PagedCacheDev& C, bool q8, const PagedBatch
 
 namespace {
 
-// Workgroups per kv head of the split kernel: the chip's 256 CUs at the kernel's occupancy.
-struct SplitPlan {
-    int mt, W;
+// Up to 32 queries per sequence and kv head the split kernel reads every token once; above, the tile
+// kernel does so once per 128 or 256 queries.
+struct AttnPlan {
+    bool tiles;
+    int mt;         // split: 16-query groups
+    int W;          // split: workgroups per kv head; tiles: ranges per item
+    int items;      // tiles: items at most
     bool joined;
+    int M;
 };
-SplitPlan split_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
-    SplitPlan p;
-    p.mt = static_cast<int64_t>(max_rows) * (hq / C.hkv) <= 16 ? 1 : 2;
-    const int per_cu = C.d == 256 ? 1 : 2;
-    p.W = std::max(1, 256 * per_cu / C.hkv);
-    // no sequence of the table is longer than a step: nothing is ever split
-    p.joined = (static_cast<int64_t>(B.width) << C.shift) > kSplitTokens;
+AttnPlan attn_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
+    AttnPlan p{};
+    const int64_t G = hq / C.hkv, queries = max_rows * G, span = static_cast<int64_t>(B.width) << C.shift;
+    p.tiles = queries > 32;
+    if (!p.tiles) {
+        p.mt = queries <= 16 ? 1 : 2;
+        p.M = 16 * p.mt;
+        p.W = std::max(1, 256 * (C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernel's occupancy
+        p.joined = span > kSplitTokens;  // (no sequence of the table is longer than a step: nothing is split)
+    } else {
+        p.M = C.d == 256 ? 128 : 256;
+        p.items = static_cast<int>(std::min<int64_t>(B.rows * G / p.M + B.seqs, B.rows * G));
+        // ranges of at least 256 tokens, until there are about two workgroups per CU
+        const int64_t blocks = std::max<int64_t>(1, static_cast<int64_t>(p.items) * C.hkv);
+        p.W = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / blocks, (span + 255) / 256)));
+        p.joined = p.W > 1;
+    }
     return p;
 }
 
 template <int D, bool Q8, int MT>
-hipError_t launch_split(const PagedCacheDev& C, const PagedBatchDev& B, const SplitPlan& p, const uint16_t* q, int64_t qs,
-                        int hq, float scale, uint16_t* out, int64_t os, float* part, hipStream_t st) {
-    constexpr int M = 16 * MT;
-    constexpr size_t lds = (static_cast<size_t>(kSplitWaves) * M * (D + 4) + 2 * kSplitWaves * M) * 4;
-    const float c = scale * 1.44269504088896341f;  // exponents of 2
-    const int G = hq / C.hkv;
-    hipError_t e = ensure_lds<k_paged_split<D, Q8, MT>>(lds);
+hipError_t launch_split(const PagedCacheDev& C, const PagedBatchDev& B, const AttnPlan& p, const uint16_t* q, int64_t qs,
+                        int hq, float c, uint16_t* out, int64_t os, float* part, hipStream_t st) {
+    constexpr size_t lds = (static_cast<size_t>(kSplitWaves) * 16 * MT * (D + 4) + 2 * kSplitWaves * 16 * MT) * 4;
+    const hipError_t e = ensure_lds<k_paged_split<D, Q8, MT>>(lds);
     if (e != hipSuccess) return e;
-    e = launch(k_paged_split<D, Q8, MT>, dim3(p.W, C.hkv), dim3(256), lds, st, C, B, G, q, qs, c, out, os, part);
+    return launch(k_paged_split<D, Q8, MT>, dim3(p.W, C.hkv), dim3(256), lds, st, C, B, hq / C.hkv, q, qs, c, out, os, part);
+}
+template <int D, bool Q8>
+hipError_t launch_attention(const PagedCacheDev& C, const PagedBatchDev& B, const AttnPlan& p, const uint16_t* q, int64_t qs,
+                            int hq, float scale, uint16_t* out, int64_t os, float* part, hipStream_t st) {
+    const float c = scale * 1.44269504088896341f;  // exponents of 2
+    hipError_t e;
+    if (!p.tiles) {
+        e = p.mt == 1 ? launch_split<D, Q8, 1>(C, B, p, q, qs, hq, c, out, os, part, st)
+                      : launch_split<D, Q8, 2>(C, B, p, q, qs, hq, c, out, os, part, st);
+    } else {
+        e = ensure_lds<k_paged_tile<D, Q8>>(TileGeo<D>::kLds);
+        if (e == hipSuccess)
+            e = launch(k_paged_tile<D, Q8>, dim3(p.items, C.hkv, p.W), dim3(64 * TileGeo<D>::WAVES), TileGeo<D>::kLds, st, C, B,
+                       hq / C.hkv, q, qs, c, out, os, part);
+    }
     if (e != hipSuccess || !p.joined) return e;
-    return launch(k_paged_join<D>, dim3(B.rows, (hq + 3) / 4), dim3(256), 0, st, C, B, AttnSplit{G, M, kSplitTokens}, hq,
-                  p.W, part, out, os);
+    const AttnSplit S{hq / C.hkv, p.M, p.tiles ? TileGeo<D>::TB : kSplitTokens};
+    const dim3 grid(B.rows, (hq + 3) / 4);
+    return p.tiles ? launch(k_paged_join<D, true>, grid, dim3(256), 0, st, C, B, S, hq, p.W, p.items, part, out, os)
+                   : launch(k_paged_join<D, false>, grid, dim3(256), 0, st, C, B, S, hq, p.W, p.items, part, out, os);
 }
 
 } // namespace
 
 size_t paged_attention_ws(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
-    const SplitPlan p = split_plan(C, B, max_rows, hq);
-    return p.joined ? static_cast<size_t>(C.hkv) * p.W * 2 * 16 * p.mt * (C.d + 2) * 4 : 0;
+    const AttnPlan p = attn_plan(C, B, max_rows, hq);
+    const size_t pieces = static_cast<size_t>(C.hkv) * p.W * (p.tiles ? p.items : 2);
+    return p.joined ? pieces * p.M * (C.d + 2) * 4 : 0;
 }
 
 hipError_t launch_paged_attention(const PagedCacheDev& C, bool q8, const PagedBatchDev& B, int max_rows, const uint16_t* q,
                                   int64_t qs, int hq, float scale, uint16_t* out, int64_t os, void* ws, hipStream_t st) {
-    const SplitPlan p = split_plan(C, B, max_rows, hq);
-    auto go = [&](auto d, auto c8) {
-        constexpr int D = decltype(d)::value;
-        constexpr bool Q8 = decltype(c8)::value;
-        auto* kern = p.mt == 1 ? launch_split<D, Q8, 1> : launch_split<D, Q8, 2>;
-        return kern(C, B, p, q, qs, hq, scale, out, os, static_cast<float*>(ws), st);
-    };
-    auto dims = [&](auto c8) {
-        return C.d == 64    ? go(std::integral_constant<int, 64>{}, c8)
-               : C.d == 128 ? go(std::integral_constant<int, 128>{}, c8)
-                            : go(std::integral_constant<int, 256>{}, c8);
-    };
-    return q8 ? dims(std::true_type{}) : dims(std::false_type{});
+    const AttnPlan p = attn_plan(C, B, max_rows, hq);
+    auto go = [&](auto kern) { return kern(C, B, p, q, qs, hq, scale, out, os, static_cast<float*>(ws), st); };
+    if (q8)
+        return C.d == 64    ? go(launch_attention<64, true>)
+               : C.d == 128 ? go(launch_attention<128, true>)
+                            : go(launch_attention<256, true>);
+    return C.d == 64    ? go(launch_attention<64, false>)
+           : C.d == 128 ? go(launch_attention<128, false>)
+                        : go(launch_attention<256, false>);
 }
 
 } // namespace q38

@@ -9,7 +9,7 @@
 namespace q38 {
 
 constexpr int kBatchMaxSeqs = 4096;
-constexpr int kBatchMaxRows = 1 << 24;
+constexpr int kBatchMaxRows = 1 << 19;  // (a launch has less than 2^32 threads)
 
 struct PagedCacheDev {
     void *keys, *values;   // [pages][hkv][1 << shift][d] bf16 or int8

@@ -32,7 +32,7 @@ def attend(q38, c, b, q=X, qs=512, heads=8, scale=0.1, out=X, os=512, ws=X, ws_b
 BAD_CACHE = [dict(format=2), dict(format=-1), dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=2048),
              dict(pages=0), dict(kv_heads=0), dict(kv_heads=65), dict(head_dim=96), dict(keys=None), dict(values=None),
              dict(keys=X + 8), dict(values=X + 2), dict(key_scales=X), dict(format=1), dict(format=1, key_scales=X)]
-BAD_BATCH = [dict(sequences=-1), dict(sequences=4097), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(max_rows=0),
+BAD_BATCH = [dict(sequences=-1), dict(sequences=4097), dict(rows=-1), dict(rows=(1 << 19) + 1), dict(max_rows=0),
              dict(max_rows=4), dict(table_pages=0), dict(table_pages=1 << 26), dict(row_offsets=None),
              dict(tokens=None), dict(page_table=None)]
 
@@ -114,7 +114,7 @@ def test_bad_delta_desc(q38, kw):
     assert "context" not in q38.last_error()
 
 
-@pytest.mark.parametrize("kw", [dict(sequences=-1), dict(sequences=4097), dict(rows=-1), dict(rows=(1 << 24) + 1),
+@pytest.mark.parametrize("kw", [dict(sequences=-1), dict(sequences=4097), dict(rows=-1), dict(rows=(1 << 19) + 1),
                                 dict(max_rows=0), dict(max_rows=4), dict(slots=-1), dict(row_offsets=None),
                                 dict(states=None), dict(states=X + 4)])
 def test_bad_delta_batch(q38, kw):
