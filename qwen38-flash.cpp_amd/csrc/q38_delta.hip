@@ -1,7 +1,9 @@
 // q38_delta.hip — the gated delta rule of many requests over a pool of float states:
 //   S <- exp(g) S,  S <- S + beta (v - S k) k^T,  o = scale * S q      per row and value head.
 //
-//   k_delta_rows   row by row, the state in registers across a sequence's rows
+//   k_delta_rows     row by row, the state in registers across a sequence's rows
+//   k_delta_system   the long form, chunks of 32 rows: each chunk's triangular system and scores
+//   k_delta_chunks   its walk over a sequence's chunks, the state in registers
 #include "q38_device.hpp"
 #include "q38_paged.hpp"
 #include "q38_internal.hpp"
@@ -94,11 +96,498 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B)
     if (B.last) store(B.last[s]);
 }
 
+// ---- the chunked form. Within a chunk of C rows, with G_i the sums of its log decays up to row i,
+// A_ij = beta_i (k_i . k_j) exp(G_i - G_j) for j < i and T = (I + A)^-1, the rows' updates
+// u_i = beta_i (v_i - S k_i) solve a triangular system:
+//   U   = T diag(beta) Y,  Y_i = v_i - exp(G_i) S k_i           (S: the state before the chunk)
+//   o_i = exp(G_i) S q_i + sum_{j <= i} (q_i . k_j) exp(G_i - G_j) U_j
+//   S  <- exp(G_C) S + sum_j exp(G_C - G_j) U_j k_j^T
+// k_delta_system forms T diag(beta), the scores and the decays of every chunk at once;
+// k_delta_chunks walks a sequence's chunks with the state in registers.
+//
+// The products run on the bf16 matrix cores. q, k and v are bf16 already: k . k and q . k are exact
+// products with float sums. Float operands of products that the state depends on (S, Y, U and T)
+// are split into three bf16 parts, x = hi + mid + lo with 24 bits kept, multiplied part by part
+// (for two split operands the six products down to 2^-24). Outputs are rounded to bf16 anyway: for
+// them S, U and the scores keep two parts, 16 bits (with one part the outputs' error was 1.5 times that
+// of their own rounding).
+constexpr int kChunk = 32;
+constexpr double kFloor = -1e4;  // exp() of it is 0; log decays below (-inf) are taken as this
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){lo, hi}, bf16x2));
+}
+__device__ __forceinline__ floatx4 mfma(uintx4 a, uintx4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Eight floats as an operand, in P parts.
+template <int P>
+struct Parts {
+    uintx4 p[P];
+    __device__ __forceinline__ void split(const float (&x)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+            for (int n = 0; n < P; ++n) {
+                const uint32_t w = pack_bf16(a, b);
+                p[n][i] = w;
+                if (n + 1 < P) a -= bflo(w), b -= bfhi(w);
+            }
+        }
+    }
+};
+
+// What k_delta_system leaves of a (chunk, value head): T diag(beta) in three parts and the scores,
+// both as operands (16 bytes per lane, two row tiles), then exp(G_i) and exp(G_C - G_i).
+struct alignas(16) ChunkSystem {
+    uintx4 t[3][2][64];
+    uintx4 m[2][2][64];
+    float into[kChunk], left[kChunk];
+};
+
+// Row of tile a's operand row (or result row) u: a lane's result rows 4 w + r of both tiles are the
+// chunk's rows 8 w .. 8 w + 7, the k index that the next product wants of it.
+__device__ __forceinline__ int chunk_row(int u, int a) { return 8 * (u >> 2) + 4 * a + (u & 3); }
+
+// The chunk of the whole batch's list, and its sequence's first row and rows from the chunk's on.
+__device__ __forceinline__ bool find_chunk(const DeltaBatchDev& B, int want, int* row, int* rows) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = 0; s0 < B.seqs; s0 += 64) {
+        RowSpan span{0, 0};
+        if (s0 + lane < B.seqs) span = row_span(B.off, s0 + lane, B.rows);
+        const int n = (span.end - span.begin + kChunk - 1) / kChunk;
+        int upto = n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
+        }
+        const uint64_t past = __ballot(before + upto > want);
+        if (past) {
+            const int l = __builtin_ctzll(past), at = want - before - __shfl(upto, l) + __shfl(n, l);
+            *row = __shfl(span.begin, l) + at * kChunk;
+            *rows = min(kChunk, __shfl(span.end, l) - *row);
+            return true;
+        }
+        before += __shfl(upto, 63);
+    }
+    return false;
+}
+// The sequence's first chunk in the list.
+__device__ __forceinline__ int first_chunk(const DeltaBatchDev& B, int seq) {
+    int n = 0;
+    for (int s = threadIdx.x & 63; s < seq; s += 64) {
+        const RowSpan span = row_span(B.off, s, B.rows);
+        n += (span.end - span.begin + kChunk - 1) / kChunk;
+    }
+    for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d);
+    return n;
+}
+
+// One wave per (chunk, value head).
+template <int DK>
+__global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B, ChunkSystem* __restrict__ sys) {
+    constexpr int KS = DK / 32, LD = kChunk + 4;
+    __shared__ __align__(16) float As[kChunk][LD], Ts[kChunk][LD], Ws[16][20];
+    __shared__ double Gs[kChunk];
+    __shared__ float Bs[kChunk];
+    const int h = blockIdx.y, lane = threadIdx.x, u = lane & 15, w = lane >> 4, hk = h / (D.hv / D.hk);
+    int r0 = 0, n = 0;
+    if (!find_chunk(B, blockIdx.x, &r0, &n)) return;
+    // the decay sums, in double: differences of far sums must keep a weak decay's digits
+    const bool mine = lane < n;
+    const float g = mine ? D.g[static_cast<size_t>(r0 + lane) * D.hv + h] : 0.0f;
+    double G = g < kFloor ? kFloor : g;
+    for (int d = 1; d < kChunk; d <<= 1) {
+        const double x = __shfl_up(G, d);
+        if (lane >= d) G += x;
+    }
+    if (lane < kChunk) {
+        Gs[lane] = G;
+        Bs[lane] = mine ? D.beta[static_cast<size_t>(r0 + lane) * D.hv + h] : 0.0f;
+    }
+    // operands: row 16 t + u, dims 32 s + 8 w ..; rows behind the sequence are zeros
+    uintx4 kop[2][KS], qop[2][KS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int r = 16 * t + u;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            kop[t][s] = qop[t][s] = (uintx4){0, 0, 0, 0};
+            if (r < n) {
+                kop[t][s] = *reinterpret_cast<const uintx4*>(D.k + (r0 + r) * D.ks + hk * DK + 32 * s + 8 * w);
+                qop[t][s] = *reinterpret_cast<const uintx4*>(D.q + (r0 + r) * D.qs + hk * DK + 32 * s + 8 * w);
+            }
+        }
+    }
+    __syncthreads();
+    floatx4 qk[2][2];
+#pragma unroll
+    for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+        for (int tj = 0; tj <= ti; ++tj) {
+            floatx4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
+            qk[ti][tj] = kk;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                kk = mfma(kop[ti][s], kop[tj][s], kk);
+                qk[ti][tj] = mfma(qop[ti][s], kop[tj][s], qk[ti][tj]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * ti + 4 * w + r, j = 16 * tj + u;
+                const float d = j <= i ? expf(static_cast<float>(Gs[i] - Gs[j])) : 0.0f;
+                As[i][j] = j < i ? Bs[i] * kk[r] * d : 0.0f;
+                qk[ti][tj][r] *= d;
+                if (j > i) qk[ti][tj][r] = 0.0f;
+            }
+        }
+    __syncthreads();
+    // the two diagonal blocks' inverses, a column per lane, by substitution
+    {
+        const int b = 16 * (w & 1);
+        float t[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float x = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                if (j >= i) break;
+                const floatx4 a = *reinterpret_cast<const floatx4*>(&As[b + i][b + j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j + e < i) x = fmaf(a[e], t[j + e], x);
+            }
+            t[i] = i == u ? 1.0f : -x;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            Ts[b + i][b + u] = t[i];
+            Ts[i][16 + u] = 0.0f;
+        }
+    }
+    __syncthreads();
+    // the block below them: -T22 (A21 T11), float products
+    floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) x = __builtin_amdgcn_mfma_f32_16x16x4f32(As[16 + u][k + w], Ts[k + w][u], x, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) Ws[4 * w + r][u] = x[r];
+    __syncthreads();
+    x = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) x = __builtin_amdgcn_mfma_f32_16x16x4f32(Ts[16 + u][16 + k + w], Ws[k + w][u], x, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) Ts[16 + 4 * w + r][u] = -x[r];
+    // (As has been read) the scores
+#pragma unroll
+    for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+        for (int tj = 0; tj < 2; ++tj)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) As[16 * ti + 4 * w + r][16 * tj + u] = tj <= ti ? qk[ti][tj][r] : 0.0f;
+    __syncthreads();
+    ChunkSystem& out = sys[static_cast<size_t>(blockIdx.x) * D.hv + h];
+    float beta[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) beta[j] = Bs[8 * w + j];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        float row[8];
+        Parts<3> t;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) row[j] = Ts[chunk_row(u, a)][8 * w + j] * beta[j];
+        t.split(row);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) out.t[p][a][lane] = t.p[p];
+        Parts<2> m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) row[j] = As[16 * a + u][8 * w + j];
+        m.split(row);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) out.m[p][a][lane] = m.p[p];
+    }
+    if (lane < kChunk) {
+        out.into[lane] = expf(static_cast<float>(Gs[lane]));
+        out.left[lane] = expf(static_cast<float>(Gs[kChunk - 1] - Gs[lane]));
+    }
+}
+
+// A wave holds 16 NC value columns of a head's state, transposed: S^T tile o (o < E = DK / 16) has
+// key dim E (4 w + r) + o in its result row 4 w + r and the value dim in its column. Lane (u, w) thus
+// holds key dims 4 E w .. 4 E (w + 1) - 1 of value dim u, eight of them in a row being an operand of
+// S k and S q with keys and queries read as stored, and the update's operand, K^T, is formed from 16-byte
+// runs of eight keys by byte permutes. No value moves between lanes, and waves share nothing but
+// the keys and queries in LDS.
+template <int DK, int NW, int NC>
+__global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatchDev B,
+                                                          const ChunkSystem* __restrict__ sys, int bound) {
+    constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8, NT = 64 * NW, PC = kChunk * CH / NT;
+    __shared__ uintx4 rows_lds[2][2][kChunk * CH];  // [buffer][keys, queries]
+    const int lane = threadIdx.x & 63, u = lane & 15, w = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.y, s = blockIdx.z, hk = h / (D.hv / D.hk);
+    const int dv = (blockIdx.x * NW + wave) * 16 * NC;  // the wave's first value dim
+    const RowSpan span = row_span(B.off, s, B.rows);
+    const int c0 = __builtin_amdgcn_readfirstlane(first_chunk(B, s));
+    // (offsets that do not ascend could name more chunks than the workspace holds)
+    const int chunks = min((span.end - span.begin + kChunk - 1) / kChunk, bound - c0);
+    const size_t elems = static_cast<size_t>(D.hv) * D.dv * DK;
+    const int from = B.origin ? B.origin[s] : -1;
+    floatx4 st[NC][E];
+    auto state_at = [&](int slot, int c, int r) {  // E consecutive key dims
+        return B.states + slot * elems + (static_cast<size_t>(h) * D.dv + dv + 16 * c + u) * DK + E * (4 * w + r);
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int o = 0; o < E; o += 4) {
+                floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (from >= B.slots) x = x + __builtin_nanf("");
+                else if (from >= 0) x = *reinterpret_cast<const floatx4*>(state_at(from, c, r) + o);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st[c][o + e][r] = x[e];
+            }
+    // keys: swizzled for reads down chunk_row()'s rows; queries: for reads down consecutive rows
+    auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
+    auto query_at = [](int row, int ch) { return row * CH + (ch ^ (row & 7)); };
+    uintx4 kr[PC], qr[PC];
+    auto fetch = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int piece = threadIdx.x + i * NT, r = span.begin + chunk * kChunk + piece / CH;
+            kr[i] = qr[i] = (uintx4){0, 0, 0, 0};
+            if (r < span.end) {
+                kr[i] = *reinterpret_cast<const uintx4*>(D.k + r * D.ks + hk * DK + 8 * (piece % CH));
+                qr[i] = *reinterpret_cast<const uintx4*>(D.q + r * D.qs + hk * DK + 8 * (piece % CH));
+            }
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int piece = threadIdx.x + i * NT;
+            rows_lds[buf][0][key_at(piece / CH, piece % CH)] = kr[i];
+            rows_lds[buf][1][query_at(piece / CH, piece % CH)] = qr[i];
+        }
+    };
+    uint16_t vr[NC][8];
+    auto fetch_v = [&](int chunk) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = span.begin + chunk * kChunk + 8 * w + j;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) vr[c][j] = r < span.end ? D.v[r * D.vs + h * D.dv + dv + 16 * c + u] : 0;
+        }
+    };
+    // a chunk's system in registers, every part loaded anew as soon as its chunk is done with it
+    uintx4 top[3][2], mop[2][2];
+    floatx4 into[2], left[2];
+    float eg[2], whole = 1.0f;
+    auto load_t = [&](const ChunkSystem& cs) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) top[p][a] = cs.t[p][a][lane];
+    };
+    auto load_m = [&](const ChunkSystem& cs) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) mop[p][a] = cs.m[p][a][lane];
+            eg[a] = cs.into[16 * a + u];
+        }
+    };
+    auto load_into = [&](const ChunkSystem& cs) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) into[a] = *reinterpret_cast<const floatx4*>(cs.into + 8 * w + 4 * a);
+    };
+    auto load_left = [&](const ChunkSystem& cs) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) left[a] = *reinterpret_cast<const floatx4*>(cs.left + 8 * w + 4 * a);
+        whole = cs.into[kChunk - 1];
+    };
+    if (chunks > 0) {
+        const ChunkSystem& cs = sys[static_cast<size_t>(c0) * D.hv + h];
+        fetch(0);
+        fetch_v(0);
+        load_into(cs);
+        load_t(cs);
+        load_m(cs);
+        load_left(cs);
+        stage(0);
+    }
+    __syncthreads();
+    for (int n = 0; n < chunks; ++n) {
+        const uintx4* kt = rows_lds[n & 1][0];
+        const uintx4* qt = rows_lds[n & 1][1];
+        const ChunkSystem& next = sys[static_cast<size_t>(c0 + min(n + 1, chunks - 1)) * D.hv + h];
+        if (n + 1 < chunks) fetch(n + 1);
+        // P = K S^T (chunk rows by value dims), and the outputs' S q, transposed (value dims by chunk rows)
+        floatx4 pr[NC][2], ot[NC][2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) pr[c][a] = ot[c][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uintx4 ka[2], qa[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                ka[a] = kt[key_at(chunk_row(u, a), KS * w + k)];
+                qa[a] = qt[query_at(16 * a + u, KS * w + k)];
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = st[c][(8 * k + j) % E][(8 * k + j) / E];
+                Parts<3> sp;
+                sp.split(x);
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+#pragma unroll
+                    for (int p = 2; p >= 0; --p) pr[c][a] = mfma(ka[a], sp.p[p], pr[c][a]);
+                    ot[c][a] = mfma(sp.p[1], qa[a], ot[c][a]);
+                    ot[c][a] = mfma(sp.p[0], qa[a], ot[c][a]);
+                }
+            }
+        }
+        // U = T diag(beta) (V - exp(G) P)
+        floatx4 un[NC][2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = bf2f(vr[c][j]) - into[j >> 2][j & 3] * pr[c][j >> 2][j & 3];
+            Parts<3> yp;
+            yp.split(y);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                x = mfma(top[2][a], yp.p[0], x);
+                x = mfma(top[1][a], yp.p[1], x);
+                x = mfma(top[0][a], yp.p[2], x);
+                x = mfma(top[1][a], yp.p[0], x);
+                x = mfma(top[0][a], yp.p[1], x);
+                un[c][a] = mfma(top[0][a], yp.p[0], x);
+            }
+        }
+        if (n + 1 < chunks) {
+            fetch_v(n + 1);
+            load_into(next);
+            load_t(next);
+        }
+        // O^T = exp(G) S q + U^T M^T
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = un[c][j >> 2][j & 3];
+            Parts<2> up;
+            up.split(x);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                ot[c][a] *= eg[a];
+                ot[c][a] = mfma(up.p[0], mop[1][a], ot[c][a]);
+                ot[c][a] = mfma(up.p[1], mop[0][a], ot[c][a]);
+                ot[c][a] = mfma(up.p[0], mop[0][a], ot[c][a]) * D.scale;
+                const int r = span.begin + n * kChunk + 16 * a + u;
+                if (r < span.end)
+                    *reinterpret_cast<uint2*>(D.out + (static_cast<size_t>(r) * D.hv + h) * D.dv + dv + 16 * c + 4 * w) =
+                        make_uint2(pack_bf16(ot[c][a][0], ot[c][a][1]), pack_bf16(ot[c][a][2], ot[c][a][3]));
+            }
+        }
+        if (n + 1 < chunks) load_m(next);
+        // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U)
+        Parts<3> zp[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float z[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = left[j >> 2][j & 3] * un[c][j >> 2][j & 3];
+            zp[c].split(z);
+#pragma unroll
+            for (int o = 0; o < E; ++o) st[c][o] *= whole;
+        }
+        if (n + 1 < chunks) load_left(next);
+        uint32_t kv[8][E / 2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (E == 4) {
+                const uint2 x = reinterpret_cast<const uint2*>(kt + key_at(8 * w + j, u >> 1))[u & 1];
+                kv[j][0] = x.x, kv[j][1] = x.y;
+            } else {
+#pragma unroll
+                for (int b = 0; b < E / 8; ++b) {
+                    const uintx4 x = kt[key_at(8 * w + j, E / 8 * u + b)];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) kv[j][4 * b + i] = x[i];
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 0; o < E; ++o) {
+            uintx4 a;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                a[j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], o & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int p = 2; p >= 0; --p) st[c][o] = mfma(a, zp[c].p[p], st[c][o]);
+        }
+        if (n + 1 < chunks) stage((n + 1) & 1);
+        __syncthreads();
+    }
+    const int to = B.last ? B.last[s] : -1;
+    if (to < 0 || to >= B.slots) return;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int o = 0; o < E; o += 4)
+                *reinterpret_cast<floatx4*>(state_at(to, c, r) + o) =
+                    (floatx4){st[c][o][r], st[c][o + 1][r], st[c][o + 2][r], st[c][o + 3][r]};
+}
+
+// Sequences of up to so many rows go row by row.
+constexpr int kRowsForm = 16;
+bool by_rows(const DeltaBatchDev& B, int max_rows) { return B.ckpt || B.rows == 0 || max_rows <= kRowsForm; }
+int chunk_bound(const DeltaBatchDev& B) { return B.rows / kChunk + (B.seqs < B.rows ? B.seqs : B.rows); }
+
+template <int DK>
+hipError_t launch_chunks(const DeltaDev& D, const DeltaBatchDev& B, ChunkSystem* sys, hipStream_t st) {
+    const int bound = chunk_bound(B);
+    const hipError_t e = launch(k_delta_system<DK>, dim3(bound, D.hv), dim3(64), 0, st, D, B, sys);
+    if (e != hipSuccess) return e;
+    return launch(k_delta_chunks<DK, 4, 1>, dim3(D.dv / 64, D.hv, B.seqs), dim3(256), 0, st, D, B,
+                  static_cast<const ChunkSystem*>(sys), bound);
+}
+
 } // namespace
 
-size_t delta_ws(const DeltaDev&, const DeltaBatchDev&, int) { return 0; }
+size_t delta_ws(const DeltaDev& D, const DeltaBatchDev& B, int max_rows) {
+    return by_rows(B, max_rows) ? 0 : static_cast<size_t>(chunk_bound(B)) * D.hv * sizeof(ChunkSystem);
+}
 
-hipError_t launch_delta(const DeltaDev& D, const DeltaBatchDev& B, int, void*, hipStream_t st) {
+hipError_t launch_delta(const DeltaDev& D, const DeltaBatchDev& B, int max_rows, void* ws, hipStream_t st) {
+    if (!by_rows(B, max_rows)) {
+        ChunkSystem* sys = static_cast<ChunkSystem*>(ws);
+        return D.dk == 64    ? launch_chunks<64>(D, B, sys, st)
+               : D.dk == 128 ? launch_chunks<128>(D, B, sys, st)
+                             : launch_chunks<256>(D, B, sys, st);
+    }
     const dim3 grid(D.dv / 32, D.hv, B.seqs);
     return D.dk == 64    ? launch(k_delta_rows<64>, grid, dim3(256), 0, st, D, B)
            : D.dk == 128 ? launch(k_delta_rows<128>, grid, dim3(256), 0, st, D, B)
