@@ -106,11 +106,12 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B)
 // k_delta_chunks walks a sequence's chunks with the state in registers.
 //
 // The products run on the bf16 matrix cores. q, k and v are bf16 already: k . k and q . k are exact
-// products with float sums. Float operands of products that the state depends on (S, Y, U and T)
-// are split into three bf16 parts, x = hi + mid + lo with 24 bits kept, multiplied part by part
-// (for two split operands the six products down to 2^-24). Outputs are rounded to bf16 anyway: for
-// them S, U and the scores keep two parts, 16 bits (with one part the outputs' error was 1.5 times that
-// of their own rounding).
+// products with float sums. Float operands are split into bf16 parts, x = hi + mid + lo: three parts
+// (24 bits) of Y, U and T, which the state's new terms are made of, multiplied part by part (for two
+// split operands the six products down to 2^-24); two (16 bits) of the state where it is multiplied with
+// k and q (the state itself stays in float), of the scores and of U in the outputs. Against 64 bits
+// the states are off by 1.2e-7 (7e-8 row by row in float, 4e-6 with two parts everywhere), the
+// outputs by their own rounding.
 constexpr int kChunk = 32;
 constexpr double kFloor = -1e4;  // exp() of it is 0; log decays below (-inf) are taken as this
 
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 // runs of eight keys by byte permutes. No value moves between lanes, and waves share nothing but
 // the keys and queries in LDS.
 template <int DK, int NW, int NC>
-__global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatchDev B,
+__global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(DeltaDev D, DeltaBatchDev B,
                                                           const ChunkSystem* __restrict__ sys, int bound) {
     constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8, NT = 64 * NW, PC = kChunk * CH / NT;
     __shared__ uintx4 rows_lds[2][2][kChunk * CH];  // [buffer][keys, queries]
@@ -357,6 +358,8 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st[c][o + e][r] = x[e];
             }
+    // Loads of the next chunk are made always, of the last row again where there is none: its update is
+    // nothing (beta 0 in the system), and without branches a wait counts the loads that it needs alone.
     // keys: swizzled for reads down chunk_row()'s rows; queries: for reads down consecutive rows
     auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
     auto query_at = [](int row, int ch) { return row * CH + (ch ^ (row & 7)); };
@@ -364,12 +367,9 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
     auto fetch = [&](int chunk) {
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int piece = threadIdx.x + i * NT, r = span.begin + chunk * kChunk + piece / CH;
-            kr[i] = qr[i] = (uintx4){0, 0, 0, 0};
-            if (r < span.end) {
-                kr[i] = *reinterpret_cast<const uintx4*>(D.k + r * D.ks + hk * DK + 8 * (piece % CH));
-                qr[i] = *reinterpret_cast<const uintx4*>(D.q + r * D.qs + hk * DK + 8 * (piece % CH));
-            }
+            const int piece = threadIdx.x + i * NT, r = min(span.begin + chunk * kChunk + piece / CH, span.end - 1);
+            kr[i] = *reinterpret_cast<const uintx4*>(D.k + r * D.ks + hk * DK + 8 * (piece % CH));
+            qr[i] = *reinterpret_cast<const uintx4*>(D.q + r * D.qs + hk * DK + 8 * (piece % CH));
         }
     };
     auto stage = [&](int buf) {
@@ -384,9 +384,9 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
     auto fetch_v = [&](int chunk) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int r = span.begin + chunk * kChunk + 8 * w + j;
+            const int r = min(span.begin + chunk * kChunk + 8 * w + j, span.end - 1);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) vr[c][j] = r < span.end ? D.v[r * D.vs + h * D.dv + dv + 16 * c + u] : 0;
+            for (int c = 0; c < NC; ++c) vr[c][j] = D.v[r * D.vs + h * D.dv + dv + 16 * c + u];
         }
     };
     // a chunk's system in registers, every part loaded anew as soon as its chunk is done with it
@@ -431,32 +431,40 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
         const uintx4* kt = rows_lds[n & 1][0];
         const uintx4* qt = rows_lds[n & 1][1];
         const ChunkSystem& next = sys[static_cast<size_t>(c0 + min(n + 1, chunks - 1)) * D.hv + h];
-        if (n + 1 < chunks) fetch(n + 1);
+        fetch(n + 1);
         // P = K S^T (chunk rows by value dims), and the outputs' S q, transposed (value dims by chunk rows)
         floatx4 pr[NC][2], ot[NC][2];
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int a = 0; a < 2; ++a) pr[c][a] = ot[c][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int KB = KS < 4 ? KS : 4;  // dims whose operands are read together
+        uintx4 kb[KB][2], qb[KB][2];
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            uintx4 ka[2], qa[2];
+            if (k % KB == 0) {
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                ka[a] = kt[key_at(chunk_row(u, a), KS * w + k)];
-                qa[a] = qt[query_at(16 * a + u, KS * w + k)];
+                for (int i = 0; i < KB; ++i)
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        kb[i][a] = kt[key_at(chunk_row(u, a), KS * w + k + i)];
+                        qb[i][a] = qt[query_at(16 * a + u, KS * w + k + i)];
+                    }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            const uintx4(&ka)[2] = kb[k % KB];
+            const uintx4(&qa)[2] = qb[k % KB];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = st[c][(8 * k + j) % E][(8 * k + j) / E];
-                Parts<3> sp;
+                Parts<2> sp;
                 sp.split(x);
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
 #pragma unroll
-                    for (int p = 2; p >= 0; --p) pr[c][a] = mfma(ka[a], sp.p[p], pr[c][a]);
+                    for (int p = 1; p >= 0; --p) pr[c][a] = mfma(ka[a], sp.p[p], pr[c][a]);
                     ot[c][a] = mfma(sp.p[1], qa[a], ot[c][a]);
                     ot[c][a] = mfma(sp.p[0], qa[a], ot[c][a]);
                 }
@@ -482,11 +490,9 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
                 un[c][a] = mfma(top[0][a], yp.p[0], x);
             }
         }
-        if (n + 1 < chunks) {
-            fetch_v(n + 1);
-            load_into(next);
-            load_t(next);
-        }
+        fetch_v(n + 1);
+        load_into(next);
+        load_t(next);
         // O^T = exp(G) S q + U^T M^T
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -507,7 +513,7 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
                         make_uint2(pack_bf16(ot[c][a][0], ot[c][a][1]), pack_bf16(ot[c][a][2], ot[c][a][3]));
             }
         }
-        if (n + 1 < chunks) load_m(next);
+        load_m(next);
         // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U)
         Parts<3> zp[NC];
 #pragma unroll
@@ -519,7 +525,7 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
 #pragma unroll
             for (int o = 0; o < E; ++o) st[c][o] *= whole;
         }
-        if (n + 1 < chunks) load_left(next);
+        load_left(next);
         uint32_t kv[8][E / 2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -546,8 +552,8 @@ __global__ __launch_bounds__(64 * NW) void k_delta_chunks(DeltaDev D, DeltaBatch
 #pragma unroll
                 for (int p = 2; p >= 0; --p) st[c][o] = mfma(a, zp[c].p[p], st[c][o]);
         }
-        if (n + 1 < chunks) stage((n + 1) & 1);
-        __syncthreads();
+        stage((n + 1) & 1);
+        lds_barrier();  // (the next chunk's loads stay in flight)
     }
     const int to = B.last ? B.last[s] : -1;
     if (to < 0 || to >= B.slots) return;

@@ -753,7 +753,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
             st.values16(v, vs, p, base, lane);
         }
         if (step + 1 < to) stage(buf ^ 1);
-        __syncthreads();
+        lds_barrier();  // (the pages' loads stay in flight)
     }
     bad = __syncthreads_or(bad);
     const bool whole = per >= it.steps;
