@@ -2210,8 +2210,8 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 int check_rows_operand(const char* name, const char* what, const void* p, int64_t stride, int64_t width) {
     if (!p) return fail(Q38_EINVAL, std::string(name) + ": null " + what);
     if (!aligned16(p)) return fail(Q38_EINVAL, std::string(name) + ": " + what + " must be 16-byte aligned");
-    if (stride < width || stride % 8 || stride > (int64_t{1} << 32))
-        return fail(Q38_EINVAL, std::string(name) + ": " + what + " stride must be a multiple of 8, at least the row");
+    if (stride < width || stride % 8 || stride >= (int64_t{1} << 24))
+        return fail(Q38_EINVAL, std::string(name) + ": " + what + " stride must be a multiple of 8, at least the row, below 2^24");
     return Q38_OK;
 }
 

@@ -321,13 +321,13 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
     }
 }
 
-// A wave holds 16 NC value columns of a head's state, transposed: S^T tile o (o < E = DK / 16) has
+// A wave holds 16 value columns of a head's state, transposed: S^T tile o (o < E = DK / 16) has
 // key dim E (4 w + r) + o in its result row 4 w + r and the value dim in its column. Lane (u, w) thus
 // holds key dims 4 E w .. 4 E (w + 1) - 1 of value dim u, eight of them in a row being an operand of
 // S k and S q with keys and queries read as stored, and the update's operand, K^T, is formed from 16-byte
 // runs of eight keys by byte permutes. No value moves between lanes, and waves share nothing but
 // the keys and queries in LDS.
-template <int DK, int NW, int NC>
+template <int DK, int NW>
 __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(DeltaDev D, DeltaBatchDev B,
                                                           const ChunkSystem* __restrict__ sys, int bound) {
     constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8, NT = 64 * NW, PC = kChunk * CH / NT;
@@ -335,41 +335,57 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
     const int lane = threadIdx.x & 63, u = lane & 15, w = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.y, s = blockIdx.z, hk = h / (D.hv / D.hk);
-    const int dv = (blockIdx.x * NW + wave) * 16 * NC;  // the wave's first value dim
+    const int dv = (blockIdx.x * NW + wave) * 16;  // the wave's first value dim
     const RowSpan span = row_span(B.off, s, B.rows);
     const int c0 = __builtin_amdgcn_readfirstlane(first_chunk(B, s));
     // (offsets that do not ascend could name more chunks than the workspace holds)
     const int chunks = min((span.end - span.begin + kChunk - 1) / kChunk, bound - c0);
     const size_t elems = static_cast<size_t>(D.hv) * D.dv * DK;
     const int from = B.origin ? B.origin[s] : -1;
-    floatx4 st[NC][E];
-    auto state_at = [&](int slot, int c, int r) {  // E consecutive key dims
-        return B.states + slot * elems + (static_cast<size_t>(h) * D.dv + dv + 16 * c + u) * DK + E * (4 * w + r);
+    floatx4 st[E];
+    auto state_at = [&](int slot, int r) {  // E consecutive key dims
+        return B.states + slot * elems + (static_cast<size_t>(h) * D.dv + dv + u) * DK + E * (4 * w + r);
     };
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int o = 0; o < E; o += 4) {
+            floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (from >= B.slots) x = x + __builtin_nanf("");
+            else if (from >= 0) x = *reinterpret_cast<const floatx4*>(state_at(from, r) + o);
 #pragma unroll
-            for (int o = 0; o < E; o += 4) {
-                floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (from >= B.slots) x = x + __builtin_nanf("");
-                else if (from >= 0) x = *reinterpret_cast<const floatx4*>(state_at(from, c, r) + o);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) st[c][o + e][r] = x[e];
-            }
-    // Loads of the next chunk are made always, of the last row again where there is none: its update is
-    // nothing (beta 0 in the system), and without branches a wait counts the loads that it needs alone.
+            for (int e = 0; e < 4; ++e) st[o + e][r] = x[e];
+        }
     // keys: swizzled for reads down chunk_row()'s rows; queries: for reads down consecutive rows
     auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
     auto query_at = [](int row, int ch) { return row * CH + (ch ^ (row & 7)); };
+    // The next chunk's loads are made always and their number is the same on every path, so that a wait
+    // counts only the loads that it needs: a whole chunk's by uniform addresses and a lane's offset,
+    // the others' rows clamped to the sequence's last (a repeated row's update is nothing: its beta in
+    // the system is 0).
+    const uint32_t ko = 2 * ((threadIdx.x / CH) * static_cast<uint32_t>(D.ks) + 8 * (threadIdx.x % CH));
+    const uint32_t qo = 2 * ((threadIdx.x / CH) * static_cast<uint32_t>(D.qs) + 8 * (threadIdx.x % CH));
+    const uint32_t vo = 2 * (8 * w * static_cast<uint32_t>(D.vs) + u);
+    const char* const kb0 = reinterpret_cast<const char*>(D.k + span.begin * D.ks + hk * DK);
+    const char* const qb0 = reinterpret_cast<const char*>(D.q + span.begin * D.qs + hk * DK);
+    const char* const vb0 = reinterpret_cast<const char*>(D.v + span.begin * D.vs + h * D.dv + dv);
     uintx4 kr[PC], qr[PC];
+    const int length = span.end - span.begin;
     auto fetch = [&](int chunk) {
+        if ((chunk + 1) * kChunk <= length) {
 #pragma unroll
-        for (int i = 0; i < PC; ++i) {
-            const int piece = threadIdx.x + i * NT, r = min(span.begin + chunk * kChunk + piece / CH, span.end - 1);
-            kr[i] = *reinterpret_cast<const uintx4*>(D.k + r * D.ks + hk * DK + 8 * (piece % CH));
-            qr[i] = *reinterpret_cast<const uintx4*>(D.q + r * D.qs + hk * DK + 8 * (piece % CH));
+            for (int i = 0; i < PC; ++i) {
+                const int64_t row = chunk * kChunk + i * (NT / CH);
+                kr[i] = *reinterpret_cast<const uintx4*>(kb0 + 2 * row * D.ks + ko);
+                qr[i] = *reinterpret_cast<const uintx4*>(qb0 + 2 * row * D.qs + qo);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PC; ++i) {
+                const int64_t row = min(chunk * kChunk + static_cast<int>(threadIdx.x) / CH + i * (NT / CH), length - 1);
+                kr[i] = *reinterpret_cast<const uintx4*>(kb0 + 2 * row * D.ks + 16 * (threadIdx.x % CH));
+                qr[i] = *reinterpret_cast<const uintx4*>(qb0 + 2 * row * D.qs + 16 * (threadIdx.x % CH));
+            }
         }
     };
     auto stage = [&](int buf) {
@@ -380,15 +396,22 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             rows_lds[buf][1][query_at(piece / CH, piece % CH)] = qr[i];
         }
     };
-    uint16_t vr[NC][8];
+    uint16_t vr[8];
     auto fetch_v = [&](int chunk) {
+        if ((chunk + 1) * kChunk <= length) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int r = min(span.begin + chunk * kChunk + 8 * w + j, span.end - 1);
+            for (int j = 0; j < 8; ++j)
+                vr[j] = *reinterpret_cast<const uint16_t*>(vb0 + 2 * static_cast<int64_t>(chunk * kChunk + j) * D.vs + vo);
+        } else {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) vr[c][j] = D.v[r * D.vs + h * D.dv + dv + 16 * c + u];
+            for (int j = 0; j < 8; ++j) {
+                const int64_t row = min(chunk * kChunk + 8 * w + j, length - 1);
+                vr[j] = *reinterpret_cast<const uint16_t*>(vb0 + 2 * row * D.vs + 2 * u);
+            }
         }
     };
+    char* const ob0 = reinterpret_cast<char*>(D.out + (static_cast<size_t>(span.begin) * D.hv + h) * D.dv + dv);
+    const uint32_t oo = 2 * (static_cast<uint32_t>(u) * D.hv * D.dv + 4 * w);
     // a chunk's system in registers, every part loaded anew as soon as its chunk is done with it
     uintx4 top[3][2], mop[2][2];
     floatx4 into[2], left[2];
@@ -432,100 +455,54 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
         const uintx4* qt = rows_lds[n & 1][1];
         const ChunkSystem& next = sys[static_cast<size_t>(c0 + min(n + 1, chunks - 1)) * D.hv + h];
         fetch(n + 1);
-        // P = K S^T (chunk rows by value dims), and the outputs' S q, transposed (value dims by chunk rows)
-        floatx4 pr[NC][2], ot[NC][2];
+        // P = K S^T (chunk rows by value dims)
+        floatx4 pr[2], ot[2];
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) pr[c][a] = ot[c][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int a = 0; a < 2; ++a) pr[a] = ot[a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
         constexpr int KB = KS < 4 ? KS : 4;  // dims whose operands are read together
-        uintx4 kb[KB][2], qb[KB][2];
+        Parts<2> sp[KS];
+        uintx4 qb[KS][2];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            if (k % KB == 0) {
+        for (int k0 = 0; k0 < KS; k0 += KB) {
+            uintx4 kb[KB][2];
 #pragma unroll
-                for (int i = 0; i < KB; ++i)
+            for (int k = 0; k < KB; ++k)
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        kb[i][a] = kt[key_at(chunk_row(u, a), KS * w + k + i)];
-                        qb[i][a] = qt[query_at(16 * a + u, KS * w + k + i)];
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            const uintx4(&ka)[2] = kb[k % KB];
-            const uintx4(&qa)[2] = qb[k % KB];
+                for (int a = 0; a < 2; ++a) kb[k][a] = kt[key_at(chunk_row(u, a), KS * w + k0 + k)];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            for (int k = 0; k < KB; ++k)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) qb[k0 + k][a] = qt[query_at(16 * a + u, KS * w + k0 + k)];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
                 float x[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = st[c][(8 * k + j) % E][(8 * k + j) / E];
-                Parts<2> sp;
-                sp.split(x);
+                for (int j = 0; j < 8; ++j) x[j] = st[(8 * (k0 + k) + j) % E][(8 * (k0 + k) + j) / E];
+                sp[k0 + k].split(x);
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
+                for (int p = 1; p >= 0; --p)
 #pragma unroll
-                    for (int p = 1; p >= 0; --p) pr[c][a] = mfma(ka[a], sp.p[p], pr[c][a]);
-                    ot[c][a] = mfma(sp.p[1], qa[a], ot[c][a]);
-                    ot[c][a] = mfma(sp.p[0], qa[a], ot[c][a]);
-                }
+                    for (int a = 0; a < 2; ++a) pr[a] = mfma(kb[k][a], sp[k0 + k].p[p], pr[a]);
             }
         }
-        // U = T diag(beta) (V - exp(G) P)
-        floatx4 un[NC][2];
+        __builtin_amdgcn_sched_barrier(0);
+        // the outputs' S q, transposed (value dims by chunk rows), beside Y = V - exp(G) P and its parts
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 1; p >= 0; --p)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) ot[a] = mfma(sp[k].p[p], qb[k][a], ot[a]);
+        Parts<3> yp;
+        {
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = bf2f(vr[c][j]) - into[j >> 2][j & 3] * pr[c][j >> 2][j & 3];
-            Parts<3> yp;
+            for (int j = 0; j < 8; ++j) y[j] = bf2f(vr[j]) - into[j >> 2][j & 3] * pr[j >> 2][j & 3];
             yp.split(y);
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-                x = mfma(top[2][a], yp.p[0], x);
-                x = mfma(top[1][a], yp.p[1], x);
-                x = mfma(top[0][a], yp.p[2], x);
-                x = mfma(top[1][a], yp.p[0], x);
-                x = mfma(top[0][a], yp.p[1], x);
-                un[c][a] = mfma(top[0][a], yp.p[0], x);
-            }
         }
-        fetch_v(n + 1);
-        load_into(next);
-        load_t(next);
-        // O^T = exp(G) S q + U^T M^T
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = un[c][j >> 2][j & 3];
-            Parts<2> up;
-            up.split(x);
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                ot[c][a] *= eg[a];
-                ot[c][a] = mfma(up.p[0], mop[1][a], ot[c][a]);
-                ot[c][a] = mfma(up.p[1], mop[0][a], ot[c][a]);
-                ot[c][a] = mfma(up.p[0], mop[0][a], ot[c][a]) * D.scale;
-                const int r = span.begin + n * kChunk + 16 * a + u;
-                if (r < span.end)
-                    *reinterpret_cast<uint2*>(D.out + (static_cast<size_t>(r) * D.hv + h) * D.dv + dv + 16 * c + 4 * w) =
-                        make_uint2(pack_bf16(ot[c][a][0], ot[c][a][1]), pack_bf16(ot[c][a][2], ot[c][a][3]));
-            }
-        }
-        load_m(next);
-        // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U)
-        Parts<3> zp[NC];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            float z[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = left[j >> 2][j & 3] * un[c][j >> 2][j & 3];
-            zp[c].split(z);
-#pragma unroll
-            for (int o = 0; o < E; ++o) st[c][o] *= whole;
-        }
-        load_left(next);
+        __builtin_amdgcn_sched_barrier(0);
+        // U = T diag(beta) Y, beside K^T's operands and the state's decay
         uint32_t kv[8][E / 2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -541,6 +518,32 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
                 }
             }
         }
+        floatx4 un[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            x = mfma(top[2][a], yp.p[0], x);
+            x = mfma(top[1][a], yp.p[1], x);
+            x = mfma(top[0][a], yp.p[2], x);
+            x = mfma(top[1][a], yp.p[0], x);
+            x = mfma(top[0][a], yp.p[1], x);
+            un[a] = mfma(top[0][a], yp.p[0], x);
+        }
+#pragma unroll
+        for (int o = 0; o < E; ++o) st[o] *= whole;
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_v(n + 1);
+        load_into(next);
+        load_t(next);
+        // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U), beside the outputs' parts of U
+        Parts<3> zp;
+        {
+            float z[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = left[j >> 2][j & 3] * un[j >> 2][j & 3];
+            zp.split(z);
+        }
+        load_left(next);
 #pragma unroll
         for (int o = 0; o < E; ++o) {
             uintx4 a;
@@ -548,23 +551,52 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             for (int j = 0; j < 4; ++j)
                 a[j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], o & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int p = 2; p >= 0; --p) st[c][o] = mfma(a, zp[c].p[p], st[c][o]);
+            for (int p = 2; p >= 0; --p) st[o] = mfma(a, zp.p[p], st[o]);
         }
+        Parts<2> up;
+        {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = un[j >> 2][j & 3];
+            up.split(x);
+        }
+        // O^T = exp(G) S q + U^T M^T
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            ot[a] *= eg[a];
+            ot[a] = mfma(up.p[0], mop[1][a], ot[a]);
+            ot[a] = mfma(up.p[1], mop[0][a], ot[a]);
+            ot[a] = mfma(up.p[0], mop[0][a], ot[a]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_m(next);
         stage((n + 1) & 1);
+        uint2 ov[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            ot[a] *= D.scale;
+            ov[a] = make_uint2(pack_bf16(ot[a][0], ot[a][1]), pack_bf16(ot[a][2], ot[a][3]));
+        }
+        char* const ob = ob0 + static_cast<int64_t>(n) * kChunk * D.hv * D.dv * 2;
+        const uint32_t tile = 32u * D.hv * D.dv;  // bytes of 16 rows
+        if ((n + 1) * kChunk <= length) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) *reinterpret_cast<uint2*>(ob + a * tile + oo) = ov[a];
+        } else {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+                if (n * kChunk + 16 * a + u < length) *reinterpret_cast<uint2*>(ob + a * tile + oo) = ov[a];
+        }
         lds_barrier();  // (the next chunk's loads stay in flight)
     }
     const int to = B.last ? B.last[s] : -1;
     if (to < 0 || to >= B.slots) return;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int o = 0; o < E; o += 4)
-                *reinterpret_cast<floatx4*>(state_at(to, c, r) + o) =
-                    (floatx4){st[c][o][r], st[c][o + 1][r], st[c][o + 2][r], st[c][o + 3][r]};
+        for (int o = 0; o < E; o += 4)
+            *reinterpret_cast<floatx4*>(state_at(to, r) + o) =
+                (floatx4){st[o][r], st[o + 1][r], st[o + 2][r], st[o + 3][r]};
 }
 
 // Sequences of up to so many rows go row by row.
@@ -577,7 +609,7 @@ hipError_t launch_chunks(const DeltaDev& D, const DeltaBatchDev& B, ChunkSystem*
     const int bound = chunk_bound(B);
     const hipError_t e = launch(k_delta_system<DK>, dim3(bound, D.hv), dim3(64), 0, st, D, B, sys);
     if (e != hipSuccess) return e;
-    return launch(k_delta_chunks<DK, 4, 1>, dim3(D.dv / 64, D.hv, B.seqs), dim3(256), 0, st, D, B,
+    return launch(k_delta_chunks<DK, 4>, dim3(D.dv / 64, D.hv, B.seqs), dim3(256), 0, st, D, B,
                   static_cast<const ChunkSystem*>(sys), bound);
 }
 

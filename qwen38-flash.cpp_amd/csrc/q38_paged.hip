@@ -135,12 +135,14 @@ struct HalfRows {
 // A sequence's pages. The 32 tokens from `base` lie in the pages of their two 16-token halves (one
 // page, for pages of 32 and more): the numbers are uniform over the wave.
 struct PageWalk {
-    const int32_t* table;  // the sequence's row
+    const int32_t* table;  // the sequence's row, read through the scalar cache: a vector load's wait
+                           // would also be one for all keys and values in flight
     int shift, pages, hkv, head, see;
     bool bad;
     // (a page out of range counts as page 0, a half behind the last seen token as that token's page)
     __device__ __forceinline__ int64_t half(int t) {
-        int page = table[min(t, see - 1) >> shift];
+        typedef const __attribute__((address_space(4))) int32_t scalar_t;
+        int page = ((scalar_t*)(reinterpret_cast<uintptr_t>(table)))[min(t, see - 1) >> shift];
         if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(pages)) {
             bad = true;
             page = 0;
@@ -399,49 +401,43 @@ __device__ __forceinline__ floatx4 add_special(const PagedCacheDev& C, const int
 constexpr int kSplitWaves = 4;                 // waves of a workgroup
 constexpr int kSplitTokens = 32 * kSplitWaves; // tokens of a step
 
+__device__ __forceinline__ int64_t uniform(int64_t v) {  // a value that every lane holds, in scalar registers
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
+    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
 // Where the share's first step lies: the sequence that holds step w * share of the list, and that
-// sequence's first step. Returns the list's length. All threads take part; seqs <= 256 are weighed once.
+// sequence's first step; returns the list's length. Every wave finds it by itself, 64 sequences a
+// round (a scan over the workgroup took two barriers and 2 us of the smallest calls); up to 64 sequences
+// are weighed once.
 __device__ __forceinline__ int64_t find_share(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t w, int64_t W,
                                               int* seq, int64_t* seq_start, int64_t* share) {
-    __shared__ int64_t sums[4], hit_start;
-    __shared__ int hit;
-    const int tid = threadIdx.x, lane = tid & 63;
-    int64_t total = 0, mine = 0;
-    for (int s0 = 0; s0 < B.seqs; s0 += 256) {
-        mine = s0 + tid < B.seqs ? attn_weight(S, B, shift, s0 + tid) : 0;
-        int64_t sum = mine;
-        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) sums[tid >> 6] = sum;
-        __syncthreads();
-        total += sums[0] + sums[1] + sums[2] + sums[3];
-        __syncthreads();
-    }
-    *share = (total + W - 1) / W;
+    const int lane = threadIdx.x & 63;
+    auto weight = [&](int s) { return s < B.seqs ? static_cast<int64_t>(attn_weight(S, B, shift, s)) : 0; };
+    int64_t mine = 0, sum = 0;
+    for (int s0 = 0; s0 < B.seqs; s0 += 64) sum += mine = weight(s0 + lane);
+    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+    sum = uniform(sum);
+    *share = (sum + W - 1) / W;
     const int64_t want = w * *share;
-    if (want >= total) return total;
     int64_t before = 0;
-    for (int s0 = 0; s0 < B.seqs; s0 += 256) {
-        if (B.seqs > 256) mine = s0 + tid < B.seqs ? attn_weight(S, B, shift, s0 + tid) : 0;
+    for (int s0 = 0; s0 < B.seqs && want < sum; s0 += 64) {
+        if (B.seqs > 64) mine = weight(s0 + lane);
         int64_t upto = mine;
         for (int d = 1; d < 64; d <<= 1) {
             const int64_t x = __shfl_up(upto, d);
             if (lane >= d) upto += x;
         }
-        if (lane == 63) sums[tid >> 6] = upto;
-        __syncthreads();
-        int64_t start = before + upto - mine;
-        for (int i = 0; i < (tid >> 6); ++i) start += sums[i];
-        before += sums[0] + sums[1] + sums[2] + sums[3];
-        if (want >= start && want < start + mine) {
-            hit = s0 + tid;
-            hit_start = start;
+        const uint64_t past = __ballot(before + upto > want);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            *seq = __builtin_amdgcn_readfirstlane(s0 + l);
+            *seq_start = before + uniform(__shfl(upto - mine, l));
+            break;
         }
-        __syncthreads();
-        if (before > want) break;
+        before += uniform(__shfl(upto, 63));
     }
-    *seq = hit;
-    *seq_start = hit_start;
-    return total;
+    return sum;
 }
 
 // A workgroup's share of a kv head's steps; wave i takes tokens 32 i .. 32 i + 31 of every step, the
@@ -788,14 +784,17 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
     }
 }
 
-// Joins the pieces of an item that several workgroups worked on, one wave per (row, query head):
-// TILES: those of k_paged_tile, W ranges per item; else those of k_paged_split, W shares.
+// Joins the pieces of an item that several workgroups worked on, a workgroup per (row, query head),
+// each of its waves every fourth piece, eight in flight. TILES: pieces of k_paged_tile, W ranges per
+// item; else those of k_paged_split, W shares.
 template <int D, bool TILES>
-__global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchDev B, AttnSplit S, int hq, int W,
+__global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchDev B, AttnSplit S, int W,
                                                     int items, const float* __restrict__ part,
                                                     uint16_t* __restrict__ out, int64_t os) {
+    constexpr int E = D / 64;
+    __shared__ float sums[4][D + 2];
     const int row = blockIdx.x, lane = threadIdx.x & 63, G = S.G, M = S.M;
-    const int h = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
     const int seq = row_sequence(B.off, B.seqs, row);
     if (seq < 0) return;
     // what lies in front of the sequence: steps (and the list's length), or tiles
@@ -815,7 +814,6 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchD
         total += __shfl_xor(total, d);
         start += __shfl_xor(start, d);
     }
-    if (h >= hq) return;
     AttnItem it;
     attn_sequence(B, C.shift, seq, &it);
     const int idx = (row - it.first) * G + h % G, head = h / G, at = idx % M;
@@ -844,31 +842,32 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchD
     }
     if (n == 1) return;
     auto piece = [&](int i) { return part + (first + i * step - (!TILES && i > 0)) * (M * (D + 2)); };
-    constexpr int E = D / 64;
-    float top = -INFINITY, sum = 0.0f, o[E] = {};
-    for (int p0 = 0; p0 < n; p0 += 64) {
-        const bool live = p0 + lane < n;
-        const float* mine = piece(live ? p0 + lane : n - 1);
-        const float mt = live ? mine[M * D + at] : -INFINITY, ms = live ? mine[M * D + M + at] : 0.0f;
-        const float now = fmaxf(top, wave_max(mt)), ref = now == -INFINITY ? 0.0f : now;
-        const float keep = __builtin_amdgcn_exp2f(top - ref), f = live ? __builtin_amdgcn_exp2f(mt - ref) : 0.0f;
-        top = now;
-        sum = sum * keep + wave_sum_xor(ms * f);
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, piece(i)[M * D + at]);
+    top = wave_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, o[E] = {};
+#pragma unroll 8
+    for (int i = wave; i < n; i += 4) {
+        const float* src = piece(i);
+        const float f = __builtin_amdgcn_exp2f(src[M * D + at] - ref);
+        sum = fmaf(src[M * D + M + at], f, sum);
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= keep;
-        const int left = min(64, n - p0);
-#pragma unroll 4
-        for (int i = 0; i < left; ++i) {
-            const float* src = piece(p0 + i) + at * D + lane * E;
-            const float fi = __shfl(f, i);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], fi, o[e]);
-        }
+        for (int e = 0; e < E; ++e) o[e] = fmaf(src[at * D + lane * E + e], f, o[e]);
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = o[e];
+    if (lane == 0) sums[wave][D] = sum;
+    __syncthreads();
+    if (wave) return;
+    sum = sums[0][D] + sums[1][D] + sums[2][D] + sums[3][D];
     const float inv = it.bad || attn_see(it, idx / G) > 0 ? 1.0f / sum : 0.0f;
     uint16_t* dst = out + row * os + h * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = f2bf(o[e] * inv);
+    for (int e = 0; e < E; ++e) {
+        const int d = lane * E + e;
+        dst[e] = f2bf((sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) * inv);
+    }
 }
 
 } // namespace
@@ -939,9 +938,9 @@ hipError_t launch_attention(const PagedCacheDev& C, const PagedBatchDev& B, cons
     }
     if (e != hipSuccess || !p.joined) return e;
     const AttnSplit S{hq / C.hkv, p.M, p.tiles ? TileGeo<D>::TB : kSplitTokens};
-    const dim3 grid(B.rows, (hq + 3) / 4);
-    return p.tiles ? launch(k_paged_join<D, true>, grid, dim3(256), 0, st, C, B, S, hq, p.W, p.items, part, out, os)
-                   : launch(k_paged_join<D, false>, grid, dim3(256), 0, st, C, B, S, hq, p.W, p.items, part, out, os);
+    const dim3 grid(B.rows, hq);
+    return p.tiles ? launch(k_paged_join<D, true>, grid, dim3(256), 0, st, C, B, S, p.W, p.items, part, out, os)
+                   : launch(k_paged_join<D, false>, grid, dim3(256), 0, st, C, B, S, p.W, p.items, part, out, os);
 }
 
 } // namespace
