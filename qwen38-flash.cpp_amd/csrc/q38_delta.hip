@@ -19,81 +19,117 @@ __device__ __forceinline__ float sum8(float v) {  // over 8 neighbouring lanes, 
     return v;
 }
 
-// Four waves take 32 value rows of one head of one sequence: 8 lanes per value row, lane `sub`
-// of them key dims 32 c + 4 sub .. + 3 (16-byte state accesses, 128 bytes together per row).
-template <int DK>
+// A value that is the same for the whole wave, through the scalar cache: its wait is not one for the
+// vector loads in flight.
+template <typename T>
+__device__ __forceinline__ T uniform_load(const T* p) {
+    typedef const __attribute__((address_space(4))) T scalar_t;
+    return *((scalar_t*)(reinterpret_cast<uintptr_t>(p)));
+}
+
+// A wave takes 8 R value rows of one head of one sequence: 8 lanes per value row, lane `sub` of them
+// key dims 32 c + 4 sub .. + 3 (16-byte state accesses, 128 bytes together per row). Bound by the
+// states' bytes for single tokens; the next row's operands are in flight during a row.
+template <int DK, int R>
 __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B) {
     constexpr int C = DK / 32;
-    const int s = blockIdx.z, h = blockIdx.y, sub = threadIdx.x & 7;
-    const int dv = blockIdx.x * 32 + (threadIdx.x >> 3);
+    const int s = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, sub = lane & 7;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int dv = (blockIdx.x * 4 + wave) * 8 * R + (lane >> 3);  // the lane's first value row, the next 8 on
     const int hk = h / (D.hv / D.hk);
-    const RowSpan span = row_span(B.off, s, B.rows);
-    const int from = B.origin ? B.origin[s] : -1;
+    const int first = uniform_load(B.off + s), behind = uniform_load(B.off + s + 1);
+    const int from = B.origin ? uniform_load(B.origin + s) : -1, last = B.last ? uniform_load(B.last + s) : -1;
+    const int begin = max(first, 0), end = min(behind, B.rows);
     const size_t elems = static_cast<size_t>(D.hv) * D.dv * DK;
     const size_t lane_at = (static_cast<size_t>(h) * D.dv + dv) * DK + 4 * sub;
-    float4 st[C];
+    float4 st[R][C];
+    const float fill = from >= B.slots ? __builtin_nanf("") : 0.0f;
+    if (from >= 0 && from < B.slots) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        st[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (from >= B.slots) st[c].x = st[c].y = st[c].z = st[c].w = __uint_as_float(0x7fc00000u);
-        else if (from >= 0) st[c] = *reinterpret_cast<const float4*>(B.states + from * elems + lane_at + 32 * c);
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                st[i][c] = *reinterpret_cast<const float4*>(B.states + from * elems + lane_at + i * 8 * DK + 32 * c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < C; ++c) st[i][c] = make_float4(fill, fill, fill, fill);
     }
     auto store = [&](int slot) {
         if (slot < 0 || slot >= B.slots) return;
 #pragma unroll
-        for (int c = 0; c < C; ++c) *reinterpret_cast<float4*>(B.states + slot * elems + lane_at + 32 * c) = st[c];
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                *reinterpret_cast<float4*>(B.states + slot * elems + lane_at + i * 8 * DK + 32 * c) = st[i][c];
     };
     struct RowIn {
         uint2 k[C], q[C];
-        float v, g, b;
-        int to;
+        uint16_t v[R];
+        float g, b;
     };
-    auto load = [&](int r) {
-        RowIn x;
+    auto load = [&](int r, RowIn& x) {
+        r = min(r, end - 1);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             x.k[c] = *reinterpret_cast<const uint2*>(D.k + r * D.ks + hk * DK + 32 * c + 4 * sub);
             x.q[c] = *reinterpret_cast<const uint2*>(D.q + r * D.qs + hk * DK + 32 * c + 4 * sub);
         }
-        x.v = bf2f(D.v[r * D.vs + h * D.dv + dv]);
-        x.g = D.g[static_cast<size_t>(r) * D.hv + h];
-        x.b = D.beta[static_cast<size_t>(r) * D.hv + h];
-        x.to = B.ckpt ? B.ckpt[r] : -1;
-        return x;
+#pragma unroll
+        for (int i = 0; i < R; ++i) x.v[i] = D.v[r * D.vs + h * D.dv + dv + 8 * i];
+        x.g = uniform_load(D.g + static_cast<size_t>(r) * D.hv + h);
+        x.b = uniform_load(D.beta + static_cast<size_t>(r) * D.hv + h);
     };
-    RowIn next;
-    if (span.begin < span.end) next = load(span.begin);
-    for (int r = span.begin; r < span.end; ++r) {
-        const RowIn x = next;
-        if (r + 1 < span.end) next = load(r + 1);
+    auto row = [&](int r, const RowIn& x) {
         const float decay = expf(x.g);
-        float hit = 0.0f;
+        float hit[R] = {}, o[R] = {};
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            st[c].x *= decay, st[c].y *= decay, st[c].z *= decay, st[c].w *= decay;
-            hit = fmaf(st[c].x, bflo(x.k[c].x), hit);
-            hit = fmaf(st[c].y, bfhi(x.k[c].x), hit);
-            hit = fmaf(st[c].z, bflo(x.k[c].y), hit);
-            hit = fmaf(st[c].w, bfhi(x.k[c].y), hit);
-        }
-        const float u = x.b * (x.v - sum8(hit));
-        float o = 0.0f;
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            st[c].x = fmaf(u, bflo(x.k[c].x), st[c].x);
-            st[c].y = fmaf(u, bfhi(x.k[c].x), st[c].y);
-            st[c].z = fmaf(u, bflo(x.k[c].y), st[c].z);
-            st[c].w = fmaf(u, bfhi(x.k[c].y), st[c].w);
-            o = fmaf(st[c].x, bflo(x.q[c].x), o);
-            o = fmaf(st[c].y, bfhi(x.q[c].x), o);
-            o = fmaf(st[c].z, bflo(x.q[c].y), o);
-            o = fmaf(st[c].w, bfhi(x.q[c].y), o);
+            for (int c = 0; c < C; ++c) {
+                float4& t = st[i][c];
+                t.x *= decay, t.y *= decay, t.z *= decay, t.w *= decay;
+                hit[i] = fmaf(t.x, bflo(x.k[c].x), hit[i]);
+                hit[i] = fmaf(t.y, bfhi(x.k[c].x), hit[i]);
+                hit[i] = fmaf(t.z, bflo(x.k[c].y), hit[i]);
+                hit[i] = fmaf(t.w, bfhi(x.k[c].y), hit[i]);
+            }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const float u = x.b * (bf2f(x.v[i]) - sum8(hit[i]));
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float4& t = st[i][c];
+                t.x = fmaf(u, bflo(x.k[c].x), t.x);
+                t.y = fmaf(u, bfhi(x.k[c].x), t.y);
+                t.z = fmaf(u, bflo(x.k[c].y), t.z);
+                t.w = fmaf(u, bfhi(x.k[c].y), t.w);
+                o[i] = fmaf(t.x, bflo(x.q[c].x), o[i]);
+                o[i] = fmaf(t.y, bfhi(x.q[c].x), o[i]);
+                o[i] = fmaf(t.z, bflo(x.q[c].y), o[i]);
+                o[i] = fmaf(t.w, bfhi(x.q[c].y), o[i]);
+            }
         }
-        o = sum8(o);
-        if (sub == 0) D.out[(static_cast<size_t>(r) * D.hv + h) * D.dv + dv] = f2bf(o * D.scale);
-        store(x.to);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            o[i] = sum8(o[i]);
+            if (sub == 0) D.out[(static_cast<size_t>(r) * D.hv + h) * D.dv + dv + 8 * i] = f2bf(o[i] * D.scale);
+        }
+        if (B.ckpt) store(uniform_load(B.ckpt + r));
+    };
+    if (begin < end) {
+        RowIn a, b;
+        load(begin, a);
+        for (int r = begin; r < end; r += 2) {
+            load(r + 1, b);
+            row(r, a);
+            if (r + 1 >= end) break;
+            load(r + 2, a);
+            row(r + 1, b);
+        }
     }
-    if (B.last) store(B.last[s]);
+    store(last);
 }
 
 // ---- the chunked form. Within a chunk of C rows, with G_i the sums of its log decays up to row i,
@@ -626,10 +662,11 @@ hipError_t launch_delta(const DeltaDev& D, const DeltaBatchDev& B, int max_rows,
                : D.dk == 128 ? launch_chunks<128>(D, B, sys, st)
                              : launch_chunks<256>(D, B, sys, st);
     }
-    const dim3 grid(D.dv / 32, D.hv, B.seqs);
-    return D.dk == 64    ? launch(k_delta_rows<64>, grid, dim3(256), 0, st, D, B)
-           : D.dk == 128 ? launch(k_delta_rows<128>, grid, dim3(256), 0, st, D, B)
-                         : launch(k_delta_rows<256>, grid, dim3(256), 0, st, D, B);
+    constexpr int R = 2;
+    const dim3 grid(D.dv / (32 * R), D.hv, B.seqs);
+    return D.dk == 64    ? launch(k_delta_rows<64, R>, grid, dim3(256), 0, st, D, B)
+           : D.dk == 128 ? launch(k_delta_rows<128, R>, grid, dim3(256), 0, st, D, B)
+                         : launch(k_delta_rows<256, R>, grid, dim3(256), 0, st, D, B);
 }
 
 } // namespace q38
