@@ -423,19 +423,33 @@ def _opt(t):
     return None if t is None else ptr(t)
 
 
+_dtypes = {}
+
+
+def _is(t, kind: str) -> bool:
+    """Whether a torch tensor's dtype is of a kind (torch is the caller's: it is not imported here before
+    a tensor of it comes in)."""
+    if not _dtypes:
+        import torch
+        _dtypes.update(int32={torch.int32}, float32={torch.float32}, int8={torch.int8},
+                       bf16={torch.bfloat16, torch.int16, torch.uint16})
+    return t.dtype in _dtypes[kind]
+
+
 def _int32(what: str, *tensors):
     for t in tensors:
-        if t is not None and (str(t.dtype) != "torch.int32" or not t.is_contiguous()):
+        if t is not None and not (_is(t, "int32") and t.is_contiguous()):
             raise ValueError(f"{what} must be contiguous int32 tensors")
 
 
-def _row_stride(t, heads: int, dim: int) -> int:
-    """Row stride in elements of a [rows, heads, dim] bf16 tensor whose rows are contiguous."""
-    rows_ok = t.dim() == 3 and tuple(t.shape[1:]) == (heads, dim) and t.stride(2) == 1 and (
-        heads == 1 or t.stride(1) == dim)
-    if not rows_ok or str(t.dtype) not in ("torch.bfloat16", "torch.int16", "torch.uint16"):
+def _row_stride(t, rows: int, heads: int, dim: int) -> int:
+    """Row stride in elements of a [rows or more, heads, dim] bf16 tensor whose rows are contiguous."""
+    stride, (n, h, d) = t.stride(), t.shape
+    if h != heads or d != dim or stride[2] != 1 or (stride[1] != dim and heads != 1) or not _is(t, "bf16"):
         raise ValueError(f"expected a bf16 tensor [rows, {heads}, {dim}] with contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+    if n < rows:
+        raise ValueError(f"an operand has {n} rows, the batch {rows}")
+    return stride[0] if n > 1 else heads * dim
 
 
 class PagedBatch:
@@ -448,7 +462,7 @@ class PagedBatch:
         n = tokens.numel()
         if row_offsets.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("row_offsets [n + 1], tokens [n] and page_table [n, pages] disagree")
-        self._keep = (row_offsets, tokens, page_table)
+        self._keep, self.rows = (row_offsets, tokens, page_table), rows
         self.desc = PagedBatchDesc(n, rows, max_rows, page_table.shape[1], ptr(row_offsets), ptr(tokens),
                                    ptr(page_table))
 
@@ -461,38 +475,34 @@ class PagedCache:
         q8 = key_scales is not None
         if keys.dim() != 4 or keys.shape != values.shape or not (keys.is_contiguous() and values.is_contiguous()):
             raise ValueError("keys and values must be contiguous [pages, kv_heads, page_tokens, head_dim] tensors")
-        for t in (keys, values):
-            if t.element_size() != (1 if q8 else 2):
-                raise ValueError("a Q8 cache holds int8 codes, a bf16 cache 16-bit values")
+        if not all(_is(t, "int8" if q8 else "bf16") for t in (keys, values)):
+            raise ValueError("a Q8 cache holds int8 codes, a bf16 cache bf16 values")
         if q8 != (value_scales is not None):
             raise ValueError("a Q8 cache has both scales, a bf16 cache none")
         for t in (key_scales, value_scales):
-            if q8 and (t.shape != keys.shape[:3] or str(t.dtype) != "torch.float32" or not t.is_contiguous()):
+            if q8 and (t.shape != keys.shape[:3] or not _is(t, "float32") or not t.is_contiguous()):
                 raise ValueError("scales must be contiguous float32 [pages, kv_heads, page_tokens] tensors")
         self._ctx, self._keep = ctx, (keys, values, key_scales, value_scales)
-        pages, heads, page, dim = keys.shape
+        pages, self._heads, page, self._dim = keys.shape
         self.desc = PagedCacheDesc(ptr(keys), ptr(values), _opt(key_scales), _opt(value_scales),
-                                   Q38_KV_Q8 if q8 else Q38_KV_BF16, pages, page, heads, dim)
+                                   Q38_KV_Q8 if q8 else Q38_KV_BF16, pages, page, self._heads, self._dim)
 
     def append(self, batch: PagedBatch, k, v, st=None):
         """k, v: [rows, kv_heads, head_dim] bf16, any row stride."""
-        d = self.desc
-        ks, vs = _row_stride(k, d.kv_heads, d.head_dim), _row_stride(v, d.kv_heads, d.head_dim)
-        if min(k.shape[0], v.shape[0]) < batch.desc.rows:
-            raise ValueError("k and v have fewer rows than the batch")
-        check(lib.q38_paged_append(self._ctx.h, C.byref(d), C.byref(batch.desc), ptr(k), ks, ptr(v), vs, st))
+        ks = _row_stride(k, batch.rows, self._heads, self._dim)
+        vs = _row_stride(v, batch.rows, self._heads, self._dim)
+        check(lib.q38_paged_append(self._ctx and self._ctx.h, self.desc, batch.desc, k.data_ptr(), ks, v.data_ptr(), vs,
+                                   st))
 
     def workspace_size(self, batch: PagedBatch, q_heads: int) -> int:
-        return lib.q38_paged_attention_workspace_size(C.byref(self.desc), C.byref(batch.desc), q_heads)
+        return lib.q38_paged_attention_workspace_size(self.desc, batch.desc, q_heads)
 
     def attend(self, batch: PagedBatch, q, out, scale: float, ws, st=None):
         """q, out: [rows, q_heads, head_dim] bf16, any row stride."""
-        d, heads = self.desc, q.shape[1]
-        qs, os_ = _row_stride(q, heads, d.head_dim), _row_stride(out, heads, d.head_dim)
-        if min(q.shape[0], out.shape[0]) < batch.desc.rows:
-            raise ValueError("q and out have fewer rows than the batch")
-        check(lib.q38_paged_attention(self._ctx.h, C.byref(d), C.byref(batch.desc), ptr(q), qs, heads, scale, ptr(out),
-                                      os_, _opt(ws), 0 if ws is None else ws.numel() * ws.element_size(), st))
+        heads = q.shape[1]
+        qs, os_ = _row_stride(q, batch.rows, heads, self._dim), _row_stride(out, batch.rows, heads, self._dim)
+        check(lib.q38_paged_attention(self._ctx and self._ctx.h, self.desc, batch.desc, q.data_ptr(), qs, heads, scale,
+                                      out.data_ptr(), os_, _opt(ws), 0 if ws is None else ws.nbytes, st))
 
 
 class DeltaBatch:
@@ -507,9 +517,10 @@ class DeltaBatch:
             raise ValueError("row_offsets [n + 1], origin [n] and final_slots [n] disagree")
         if checkpoints is not None and checkpoints.numel() < rows:
             raise ValueError("checkpoints has fewer entries than the batch rows")
-        if states is not None and (states.dim() != 4 or str(states.dtype) != "torch.float32" or not states.is_contiguous()):
+        if states is not None and (states.dim() != 4 or not _is(states, "float32") or not states.is_contiguous()):
             raise ValueError("states must be a contiguous float32 [slots, value_heads, value_dim, key_dim] tensor")
-        self._keep = (states, row_offsets, origin, final_slots, checkpoints)
+        self._keep, self.rows = (states, row_offsets, origin, final_slots, checkpoints), rows
+        self._state_shape = None if states is None else tuple(states.shape[1:])
         self.desc = DeltaBatchDesc(n, rows, max_rows, 0 if states is None else states.shape[0], ptr(row_offsets),
                                    _opt(origin), _opt(final_slots), _opt(checkpoints), _opt(states))
 
@@ -518,27 +529,24 @@ class DeltaRule:
     """The gated delta rule of one layer geometry (q38_delta_rule)."""
 
     def __init__(self, ctx: "Ctx", key_heads: int, value_heads: int, key_dim: int, value_dim: int, scale: float):
-        self._ctx = ctx
+        self._ctx, self._hk, self._hv, self._dk, self._dv = ctx, key_heads, value_heads, key_dim, value_dim
         self.desc = DeltaDesc(key_heads, value_heads, key_dim, value_dim, scale)
 
     def workspace_size(self, batch: DeltaBatch) -> int:
-        return lib.q38_delta_workspace_size(C.byref(self.desc), C.byref(batch.desc))
+        return lib.q38_delta_workspace_size(self.desc, batch.desc)
 
     def run(self, batch: DeltaBatch, q, k, v, log_decay, beta, out, ws, st=None):
         """q, k: [rows, key_heads, key_dim], v: [rows, value_heads, value_dim] bf16 at any row
         stride; log_decay, beta: contiguous [rows, value_heads] float32; out: contiguous, as v."""
-        d = self.desc
-        if batch._keep[0] is not None and tuple(batch._keep[0].shape[1:]) != (d.value_heads, d.value_dim, d.key_dim):
+        hk, hv, dk, dv, rows = self._hk, self._hv, self._dk, self._dv, batch.rows
+        if batch._state_shape not in (None, (hv, dv, dk)):
             raise ValueError("states do not have this rule's heads and dims")
-        strides = [_row_stride(t, h, n) for t, h, n in ((q, d.key_heads, d.key_dim), (k, d.key_heads, d.key_dim),
-                                                        (v, d.value_heads, d.value_dim))]
-        if _row_stride(out, d.value_heads, d.value_dim) != d.value_heads * d.value_dim:
+        qs, ks, vs = _row_stride(q, rows, hk, dk), _row_stride(k, rows, hk, dk), _row_stride(v, rows, hv, dv)
+        if _row_stride(out, rows, hv, dv) != hv * dv:
             raise ValueError("out must be contiguous")
         for t in (log_decay, beta):
-            if str(t.dtype) != "torch.float32" or not t.is_contiguous() or t.shape[1:] != (d.value_heads,):
+            if t.shape[1:] != (hv,) or t.shape[0] < rows or not _is(t, "float32") or not t.is_contiguous():
                 raise ValueError("log_decay and beta must be contiguous float32 [rows, value_heads] tensors")
-        if min(t.shape[0] for t in (q, k, v, log_decay, beta, out)) < batch.desc.rows:
-            raise ValueError("an operand has fewer rows than the batch")
-        check(lib.q38_delta_rule(self._ctx.h, C.byref(d), C.byref(batch.desc), ptr(q), strides[0], ptr(k), strides[1],
-                                 ptr(v), strides[2], ptr(log_decay), ptr(beta), ptr(out), _opt(ws),
-                                 0 if ws is None else ws.numel() * ws.element_size(), st))
+        check(lib.q38_delta_rule(self._ctx and self._ctx.h, self.desc, batch.desc, q.data_ptr(), qs, k.data_ptr(), ks,
+                                 v.data_ptr(), vs, log_decay.data_ptr(), beta.data_ptr(), out.data_ptr(), _opt(ws),
+                                 0 if ws is None else ws.nbytes, st))
