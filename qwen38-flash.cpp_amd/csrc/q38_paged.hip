@@ -13,6 +13,7 @@
 #include "q38_internal.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace q38 {
 
@@ -86,6 +87,14 @@ __device__ __forceinline__ floatx4 mfma(uintx4 a, uintx4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 constexpr float kNan = __builtin_nanf("");
+// The largest of the values of lanes u, 16 + u, 32 + u and 48 + u (a swap with itself leaves the lower
+// and the upper of two rows' values in both: their order does not matter here).
+__device__ __forceinline__ float quarters_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // ---- the register layout of the attention products.
 // A wave works transposed, on 32 tokens and 16 queries (a column each) at a time: S^T = K Q^T,
@@ -226,7 +235,11 @@ template <int D, bool Q8, int MT>
 struct AttnState {
     using Geo = AttnGeo<D, Q8>;
     floatx4 o[MT][Geo::E];
-    float top[MT], sum[MT];  // sum: of the lane's own tokens
+    // the sum of the probabilities. bf16 caches: of the rounded ones, by a product with ones (every
+    // result row is the sum over all tokens), so that a row whose weight lies on one token gives
+    // its value without their rounding; Q8: of the lane's own tokens (all[m][0]).
+    floatx4 all[MT];
+    float top[MT];
     int lim[MT];             // tokens that the query sees
 
     __device__ __forceinline__ void clear(const AttnItem& it, const AttnSplit& S, int m0, int lane) {
@@ -235,7 +248,7 @@ struct AttnState {
             const int idx = it.tile * S.M + m0 + 16 * m + (lane & 15);
             lim[m] = idx < it.rows * S.G ? attn_see(it, idx / S.G) : 0;
             top[m] = -INFINITY;
-            sum[m] = 0.0f;
+            all[m] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int o_ = 0; o_ < Geo::E; ++o_) o[m][o_] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -258,14 +271,13 @@ struct AttnState {
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) best = fmaxf(best, p[j]);
-        best = fmaxf(best, xor_lane_f<16>(best));
-        best = fmaxf(best, xor_lane_f<32>(best));
+        best = quarters_max(best);
         best = best == -INFINITY ? best : best * c;  // (c may be 0)
         if (__any(best > top[m])) {  // rare after the first tokens: the sums are brought to the new maximum
             const float now = fmaxf(best, top[m]);
             const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[m] - now);
             top[m] = now;
-            sum[m] *= keep;
+            all[m] *= keep;
 #pragma unroll
             for (int o_ = 0; o_ < Geo::E; ++o_) o[m][o_] *= keep;
         }
@@ -277,8 +289,19 @@ struct AttnState {
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[j] = first + j < lim[m] ? p[j] : 0.0f;
         }
+        if constexpr (Q8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[m] += p[j];
+            for (int j = 0; j < 8; ++j) all[m][0] += p[j];
+        }
+    }
+    // The sum over all tokens, the same in the four lanes of a query.
+    __device__ __forceinline__ float total(int m) const {
+        float v = all[m][0];
+        if constexpr (Q8) {
+            v += xor_lane_f<16>(v);
+            v += xor_lane_f<32>(v);
+        }
+        return v;
     }
 
     __device__ __forceinline__ void scores(const KeyTile<D, Q8>& k, const QueryTile<D, Q8, MT>& q, float c, int base,
@@ -310,7 +333,7 @@ struct AttnState {
 
     // O^T += V^T P^T; the probabilities, at most 1, are rounded to bf16 for it (with the value's
     // scale in a Q8 cache): half a step of each against the value it multiplies, as the output's
-    // own rounding; their sum is taken unrounded.
+    // own rounding.
     __device__ __forceinline__ void weights(const float (&p)[MT][8], const floatx4 (&vs)[2], int base, int lane,
                                             uintx4 (&b)[MT]) {
 #pragma unroll
@@ -328,6 +351,11 @@ struct AttnState {
     }
     template <bool CODES>  // the values as 8-bit codes, not as bf16
     __device__ __forceinline__ void products(const ValueTile<D, CODES>& t, const uintx4 (&b)[MT]) {
+        if constexpr (!Q8) {
+            constexpr uint32_t one = 0x3f803f80u;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) all[m] = mfma((uintx4){one, one, one, one}, b[m], all[m]);
+        }
 #pragma unroll
         for (int o_ = 0; o_ < Geo::E; ++o_) {
             uintx4 a;
@@ -498,9 +526,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         __syncthreads();  // (the previous piece's sums have been read)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            float sum = st.sum[m];
-            sum += xor_lane_f<16>(sum);
-            sum += xor_lane_f<32>(sum);
+            float sum = st.total(m);
             if (walk.bad) sum = kNan;
             const int row = 16 * m + (lane & 15);
             if (lane < 16) {
@@ -560,11 +586,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
 // queries per wave bring to the matrix cores' own time.
 template <int D>
 struct TileGeo {
-    static constexpr int WAVES = D == 256 ? 4 : 8;  // 256 dims: twice the registers, one wave per SIMD
+    static constexpr int WAVES = 4;
     static constexpr int M = 32 * WAVES;
-    static constexpr int TB = D == 256 ? 32 : 64;
-    static constexpr int CH = D / 8;                            // 16-byte chunks of a bf16 row
-    static constexpr int PIECES = TB * CH / (64 * WAVES);       // chunks per thread
+    static constexpr int TB = D == 64 ? 64 : 32;
+    static constexpr int CH = D / 8;                       // 16-byte chunks of a bf16 row
+    static constexpr int PIECES = TB * CH / (64 * WAVES);  // chunks per thread
     static constexpr size_t kLds = 2 * (2 * static_cast<size_t>(TB) * D * 2 + 2 * TB * 4);
 };
 // Place of a token's chunk in its tile: a wave's 16-byte reads of the keys go down 16 rows, 8 of
@@ -593,12 +619,13 @@ __device__ __forceinline__ bool find_tile(const AttnSplit& S, const PagedBatchDe
         const uint64_t past = __ballot(before + upto > want);
         if (past) {
             const int l = __builtin_ctzll(past);
-            attn_sequence(B, shift, s0 + l, it);
-            const int tiles = __shfl(n, l), start = before + __shfl(upto, l) - tiles;
+            attn_sequence(B, shift, __builtin_amdgcn_readfirstlane(s0 + l), it);
+            const int tiles = __builtin_amdgcn_readfirstlane(__shfl(n, l));
+            const int start = before + __builtin_amdgcn_readfirstlane(__shfl(upto, l)) - tiles;
             attn_tile(S, tiles - 1 - (want - start), it);
             return true;
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
     }
     return false;
 }
@@ -617,6 +644,12 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
     const int u = lane & 15, w = lane >> 4;
     AttnItem it;
     if (!find_tile(S, B, C.shift, blockIdx.x, &it)) return;
+    // (read by vector loads: told to be the same for all lanes, for scalar branches)
+    it.first = __builtin_amdgcn_readfirstlane(it.first);
+    it.rows = __builtin_amdgcn_readfirstlane(it.rows);
+    it.tokens = __builtin_amdgcn_readfirstlane(it.tokens);
+    it.bad = __builtin_amdgcn_readfirstlane(it.bad);
+    attn_tile(S, __builtin_amdgcn_readfirstlane(it.tile), &it);
     const int per = (it.steps + gridDim.z - 1) / gridDim.z, from = blockIdx.z * per, to = min(it.steps, from + per);
     if (from >= to) return;
     const int m0 = wave * 32, i0 = it.tile * TG::M + m0, rows = it.rows * G;
@@ -630,105 +663,56 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
     const int any = i0 < rows ? attn_see(it, min(i0 + 31, rows - 1) / G) : 0;
     const int stop = min(to * TB, it.see);
     const int32_t* table = B.table + static_cast<int64_t>(it.seq) * B.width;
-    bool bad = it.bad, special = false;
+    PageWalk walk{table, C.shift, C.pages, C.hkv, head, max(it.see, 1), it.bad};
+    bool special = false;
 
-    // staging: chunk (token, ch) of the tile from thread's piece; pages a tile ahead of the loads
-    int32_t page[PC];
-    uintx4 kr[PC], vr[PC];
+    // Staging. A wave's piece of a tile lies in 16 tokens of one page: uniform addresses and a lane's
+    // own offset. What lies behind the seen tokens is read with them and masked by its reader.
+    constexpr int EL = Q8 ? 1 : 2;
+    const int ch = threadIdx.x % CH, wt = wave * 64 / CH;  // the wave's first token of a piece
+    const uint32_t lane_off = ((lane / CH) * D + 8 * ch) * EL;
+    typedef typename std::conditional<Q8, uint2, uintx4>::type raw_t;
+    raw_t kr[PC], vr[PC];
     float sr[2] = {0.0f, 0.0f};
-    auto token_of = [&](int i) { return (static_cast<int>(threadIdx.x) + i * NT) / CH; };
-    const int ch = threadIdx.x % CH;
-    auto pages = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < PC; ++i) page[i] = t0 + token_of(i) < stop ? table[(t0 + token_of(i)) >> C.shift] : 0;
-    };
     auto fetch = [&](int t0) {
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int t = t0 + token_of(i);
-            kr[i] = vr[i] = (uintx4){0, 0, 0, 0};
-            if (t >= stop) continue;
-            const int64_t at = cache_row(page[i], C.pages, C.hkv, head, C.shift, t);
-            if (at < 0) {
-                bad = true;
-                continue;
-            }
-            if constexpr (Q8) {
-                const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(C.keys) + at * D + 8 * ch);
-                const uint2 y = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(C.values) + at * D + 8 * ch);
-                kr[i][0] = x.x, kr[i][1] = x.y;
-                vr[i][0] = y.x, vr[i][1] = y.y;
-            } else {
-                kr[i] = *reinterpret_cast<const uintx4*>(static_cast<const uint16_t*>(C.keys) + at * D + 8 * ch);
-                vr[i] = *reinterpret_cast<const uintx4*>(static_cast<const uint16_t*>(C.values) + at * D + 8 * ch);
-            }
+            const int64_t at = walk.half(t0 + i * (NT / CH) + wt) * (D * EL);
+            kr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.keys) + at + lane_off);
+            vr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.values) + at + lane_off);
         }
-        if constexpr (Q8) {
-            sr[0] = sr[1] = 0.0f;
-            const int t = t0 + threadIdx.x;
-            if (threadIdx.x < TB && t < stop) {
-                const int64_t at = cache_row(table[t >> C.shift], C.pages, C.hkv, head, C.shift, t);
-                if (at >= 0) sr[0] = C.ks[at], sr[1] = C.vs[at];
+        if constexpr (Q8)
+            if (wave < TB / 16) {  // 16 tokens' scales per wave
+                const int64_t at = walk.half(t0 + 16 * wave);
+                sr[0] = C.ks[at + u], sr[1] = C.vs[at + u];
             }
-        }
     };
-    auto widen = [](uintx4 x) {
-        return (uintx4){pack_bf16(code_f(x[0], 0), code_f(x[0], 1)), pack_bf16(code_f(x[0], 2), code_f(x[0], 3)),
-                        pack_bf16(code_f(x[1], 0), code_f(x[1], 1)), pack_bf16(code_f(x[1], 2), code_f(x[1], 3))};
+    auto widen = [](raw_t x) {
+        if constexpr (Q8)
+            return (uintx4){pack_bf16(code_f(x.x, 0), code_f(x.x, 1)), pack_bf16(code_f(x.x, 2), code_f(x.x, 3)),
+                            pack_bf16(code_f(x.y, 0), code_f(x.y, 1)), pack_bf16(code_f(x.y, 2), code_f(x.y, 3))};
+        else
+            return x;
     };
     auto stage = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int at = tile_at<D>(token_of(i), ch);
-            tiles[(2 * buf) * TB * CH + at] = Q8 ? widen(kr[i]) : kr[i];
-            tiles[(2 * buf + 1) * TB * CH + at] = Q8 ? widen(vr[i]) : vr[i];
+            const int at = tile_at<D>(i * (NT / CH) + wt + lane / CH, ch);
+            tiles[(2 * buf) * TB * CH + at] = widen(kr[i]);
+            tiles[(2 * buf + 1) * TB * CH + at] = widen(vr[i]);
         }
         if constexpr (Q8)
-            if (threadIdx.x < TB) {
-                scales[2 * buf * TB + threadIdx.x] = sr[0];
-                scales[(2 * buf + 1) * TB + threadIdx.x] = sr[1];
+            if (wave < TB / 16 && lane < 16) {
+                scales[2 * buf * TB + 16 * wave + u] = sr[0];
+                scales[(2 * buf + 1) * TB + 16 * wave + u] = sr[1];
             }
     };
-    pages(from * TB);
-    fetch(from * TB);
-    if (from + 1 < to) pages((from + 1) * TB);
-    stage(0);
-    __syncthreads();
-    for (int step = from; step < to; ++step) {
-        const int buf = (step - from) & 1;
-        if (step + 1 < to) {
-            fetch((step + 1) * TB);
-            if (step + 2 < to) pages((step + 2) * TB);
-        }
-        const uintx4* kt = tiles + (2 * buf) * TB * CH;
-        const uintx4* vt = kt + TB * CH;
-#pragma unroll 1
-        for (int sub = 0; sub < TB / 32; ++sub) {
-            const int base = step * TB + 32 * sub;
-            if (base >= any) break;
-            const bool masked = base + 32 > all;
-            floatx4 s[MT][2], ks[2], vs[2];
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) s[m][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-                const int t = 32 * sub + 8 * (u >> 2) + 4 * a + (u & 3);
-#pragma unroll
-                for (int i = 0; i < Geo::KS; ++i) {
-                    const uintx4 k = kt[tile_at<D>(t, 4 * i + w)];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) s[m][a] = mfma(k, qt.q[m][i], s[m][a]);
-                }
-                if constexpr (Q8) {
-                    const float* sc = scales + 2 * buf * TB + 32 * sub + 8 * w + 4 * a;
-                    ks[a] = *reinterpret_cast<const floatx4*>(sc);
-                    vs[a] = *reinterpret_cast<const floatx4*>(sc + TB);
-                }
-            }
-            float p[MT][8];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) st.soften(m, s[m], ks, c, base, masked, lane, p[m]);
-            ValueTile<D, false> v;
+    // 32 tokens of a staged tile
+    auto half = [&](int base, int sub, const uintx4* kt, const uintx4* vt, const float* sc) {
+        const bool masked = base + 32 > all;
+        auto key = [&](int a, int i) { return kt[tile_at<D>(32 * sub + 8 * (u >> 2) + 4 * a + (u & 3), 4 * i + w)]; };
+        ValueTile<D, false> v;
+        auto read_values = [&] {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int t = 32 * sub + 8 * w + j;
@@ -744,22 +728,70 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
                     }
                 }
             }
-            if constexpr (!Q8)
-                if (masked) special |= clean_values<D>(v, base, any, lane);
-            st.values16(v, vs, p, base, lane);
+        };
+        floatx4 s[MT][2], ks[2], vs[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) s[m][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (D < 256) {  // all reads in flight before the first product, the values' before the softmax
+            uintx4 k[2][Geo::KS];
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < Geo::KS; ++i) k[a][i] = key(a, i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < Geo::KS; ++i)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) s[m][a] = mfma(k[a][i], qt.q[m][i], s[m][a]);
+            read_values();
+        } else {  // (256 dims: no registers for them)
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < Geo::KS; ++i) {
+                    const uintx4 k = key(a, i);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) s[m][a] = mfma(k, qt.q[m][i], s[m][a]);
+                }
         }
-        if (step + 1 < to) stage(buf ^ 1);
-        lds_barrier();  // (the pages' loads stay in flight)
+        if constexpr (Q8)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                ks[a] = *reinterpret_cast<const floatx4*>(sc + 32 * sub + 8 * w + 4 * a);
+                vs[a] = *reinterpret_cast<const floatx4*>(sc + TB + 32 * sub + 8 * w + 4 * a);
+            }
+        float p[MT][8];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) st.soften(m, s[m], ks, c, base, masked, lane, p[m]);
+        if constexpr (D == 256) read_values();
+        if constexpr (!Q8)
+            if (masked) special |= clean_values<D>(v, base, any, lane);
+        st.values16(v, vs, p, base, lane);
+    };
+    fetch(from * TB);
+    stage(0);
+    __syncthreads();
+    for (int step = from; step < to; ++step) {
+        const int buf = (step - from) & 1;
+        fetch(min(step + 1, to - 1) * TB);
+        const uintx4* kt = tiles + (2 * buf) * TB * CH;
+#pragma unroll
+        for (int sub = 0; sub < TB / 32; ++sub)
+            if (step * TB + 32 * sub < any) half(step * TB + 32 * sub, sub, kt, kt + TB * CH, scales + 2 * buf * TB);
+        stage(buf ^ 1);
+        lds_barrier();
     }
-    bad = __syncthreads_or(bad);
+    const bool bad = __syncthreads_or(it.bad || (it.see > 0 && walk.bad));
     const bool whole = per >= it.steps;
     float* pd = nullptr;
     if (!whole) pd = part + ((static_cast<int64_t>(blockIdx.x) * C.hkv + head) * gridDim.z + blockIdx.z) * (TG::M * (D + 2));
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        float sum = st.sum[m];
-        sum += xor_lane_f<16>(sum);
-        sum += xor_lane_f<32>(sum);
+        float sum = st.total(m);
         if (bad) sum = kNan;
         const int idx = i0 + 16 * m + u;
         if (idx >= rows) continue;
@@ -904,7 +936,7 @@ AttnPlan attn_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows,
         p.W = std::max(1, 256 * (C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernel's occupancy
         p.joined = span > kSplitTokens;  // (no sequence of the table is longer than a step: nothing is split)
     } else {
-        p.M = C.d == 256 ? 128 : 256;
+        p.M = TileGeo<64>::M;
         p.items = static_cast<int>(std::min<int64_t>(B.rows * G / p.M + B.seqs, B.rows * G));
         // ranges of at least 256 tokens, until there are about two workgroups per CU
         const int64_t blocks = std::max<int64_t>(1, static_cast<int64_t>(p.items) * C.hkv);
