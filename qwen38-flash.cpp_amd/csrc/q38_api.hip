@@ -2266,8 +2266,8 @@ int q38_paged_append(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged
 }
 
 static int check_q_heads(const char* name, const PagedCacheDev& C, int32_t q_heads) {
-    if (q_heads < 1 || q_heads > 256 || q_heads % C.hkv)
-        return fail(Q38_EINVAL, std::string(name) + ": q_heads must be a multiple of kv_heads, at most 256");
+    if (q_heads < 1 || q_heads > 256 || q_heads % C.hkv || q_heads / C.hkv > 128)
+        return fail(Q38_EINVAL, std::string(name) + ": q_heads must be a multiple of kv_heads, at most 256 and 128 per kv head");
     return Q38_OK;
 }
 

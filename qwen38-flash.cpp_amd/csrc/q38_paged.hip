@@ -207,6 +207,12 @@ __device__ __forceinline__ void load_values(const PagedCacheDev& C, HalfRows at,
     }
 }
 
+// The sequence's row of query i of a tile (query i % G of the row's group), or -1 behind the tile's rows.
+__device__ __forceinline__ int tile_row(const AttnSplit& S, const AttnItem& it, int i) {
+    const int r = i / S.G, row = it.tile * S.rows() + r;
+    return r < S.rows() && row < it.rows ? row : -1;
+}
+
 // The queries of a tile as B operands: column lane % 16 of each group of 16.
 template <int D, bool Q8, int MT>
 struct QueryTile {
@@ -217,9 +223,9 @@ struct QueryTile {
         const int u = lane & 15, w = lane >> 4;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const int idx = it.tile * S.M + m0 + 16 * m + u;
-            const bool live = idx < it.rows * S.G;
-            const uint16_t* p = q0 + (it.first + (live ? idx / S.G : 0)) * qs + (head * S.G + (live ? idx % S.G : 0)) * D;
+            const int row = tile_row(S, it, m0 + 16 * m + u);
+            const bool live = row >= 0;
+            const uint16_t* p = q0 + (it.first + (live ? row : 0)) * qs + (head * S.G + (m0 + 16 * m + u) % S.G) * D;
 #pragma unroll
             for (int c = 0; c < AttnGeo<D, Q8>::KS; ++c) {
                 // (the keys' 16-byte loads hold 16 dims of an 8-bit row, 8 of a bf16 one)
@@ -245,8 +251,8 @@ struct AttnState {
     __device__ __forceinline__ void clear(const AttnItem& it, const AttnSplit& S, int m0, int lane) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const int idx = it.tile * S.M + m0 + 16 * m + (lane & 15);
-            lim[m] = idx < it.rows * S.G ? attn_see(it, idx / S.G) : 0;
+            const int row = tile_row(S, it, m0 + 16 * m + (lane & 15));
+            lim[m] = row >= 0 ? attn_see(it, row) : 0;
             top[m] = -INFINITY;
             all[m] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -273,8 +279,11 @@ struct AttnState {
         for (int j = 0; j < 8; ++j) best = fmaxf(best, p[j]);
         best = quarters_max(best);
         best = best == -INFINITY ? best : best * c;  // (c may be 0)
-        if (__any(best > top[m])) {  // rare after the first tokens: the sums are brought to the new maximum
-            const float now = fmaxf(best, top[m]);
+        // `top` is what exponents are taken from, and need not be the maximum itself: below 2^8 above it
+        // the probabilities and their sums are as exact. Rare after the first tokens, then: the sums
+        // brought to a new one.
+        if (__any(best > top[m] + 8.0f)) {
+            const float now = best > top[m] + 8.0f ? best : top[m];  // (a query's own need alone moves it)
             const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[m] - now);
             top[m] = now;
             all[m] *= keep;
@@ -305,7 +314,7 @@ struct AttnState {
     }
 
     __device__ __forceinline__ void scores(const KeyTile<D, Q8>& k, const QueryTile<D, Q8, MT>& q, float c, int base,
-                                           bool masked, int lane, float (&p)[MT][8]) {
+                                           bool masked, int lane, const floatx4 (&vs)[2], uintx4 (&b)[MT]) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             floatx4 s[2];
@@ -320,34 +329,31 @@ struct AttnState {
                     for (int i = 0; i < Geo::KS; ++i) {
                         // codes are integers of at most 8 bits: exact in bf16
                         const uint32_t x = k.k[a][i >> 1][2 * (i & 1)], y = k.k[a][i >> 1][2 * (i & 1) + 1];
-                        const uintx4 b = {pack_bf16(code_f(x, 0), code_f(x, 1)), pack_bf16(code_f(x, 2), code_f(x, 3)),
+                        const uintx4 kc = {pack_bf16(code_f(x, 0), code_f(x, 1)), pack_bf16(code_f(x, 2), code_f(x, 3)),
                                           pack_bf16(code_f(y, 0), code_f(y, 1)), pack_bf16(code_f(y, 2), code_f(y, 3))};
-                        s[a] = mfma(b, q.q[m][i], s[a]);
+                        s[a] = mfma(kc, q.q[m][i], s[a]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
-            soften(m, s, k.s, c, base, masked, lane, p[m]);
+            float p[8];
+            soften(m, s, k.s, c, base, masked, lane, p);
+            b[m] = weights(m, p, vs, base, lane);
         }
     }
 
     // O^T += V^T P^T; the probabilities, at most 1, are rounded to bf16 for it (with the value's
     // scale in a Q8 cache): half a step of each against the value it multiplies, as the output's
     // own rounding.
-    __device__ __forceinline__ void weights(const float (&p)[MT][8], const floatx4 (&vs)[2], int base, int lane,
-                                            uintx4 (&b)[MT]) {
+    __device__ __forceinline__ uintx4 weights(int m, const float (&p)[8], const floatx4 (&vs)[2], int base, int lane) {
+        float x[8];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = p[m][j];
-                // (an unseen token's scale may be anything)
-                if constexpr (Q8) x[j] = base + 8 * (lane >> 4) + j < lim[m] ? x[j] * vs[j >> 2][j & 3] : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[m][j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+        for (int j = 0; j < 8; ++j) {
+            x[j] = p[j];
+            // (an unseen token's scale may be anything)
+            if constexpr (Q8) x[j] = base + 8 * (lane >> 4) + j < lim[m] ? x[j] * vs[j >> 2][j & 3] : 0.0f;
         }
+        return (uintx4){pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
     }
     template <bool CODES>  // the values as 8-bit codes, not as bf16
     __device__ __forceinline__ void products(const ValueTile<D, CODES>& t, const uintx4 (&b)[MT]) {
@@ -373,36 +379,26 @@ struct AttnState {
             if (o_ & 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    __device__ __forceinline__ void values(const ValueTile<D, Q8>& t, const float (&p)[MT][8], int base, int lane) {
-        uintx4 b[MT];
-        weights(p, t.s, base, lane, b);
-        products<Q8>(t, b);
-    }
-    // the same for values widened to bf16 on their way, with their scales beside them
-    __device__ __forceinline__ void values16(const ValueTile<D, false>& t, const floatx4 (&vs)[2], const float (&p)[MT][8],
-                                             int base, int lane) {
-        uintx4 b[MT];
-        weights(p, vs, base, lane, b);
-        products<false>(t, b);
-    }
 };
 
 // bf16 values in steps that not every query of a tile sees whole. A product of a probability 0 and
 // an infinity or NaN is NaN, so tokens that nobody sees and elements that are not finite are
 // cleared; true where a seen one was not finite (never, in a healthy model): the outputs of the
 // queries that see it take it at the end (add_special).
+// All ones in each half of x that is an infinity or NaN (its exponent's carry into the sign's place).
 __device__ __forceinline__ uint32_t special_mask(uint32_t x) {
-    return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    const uint32_t m = ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    return m | (m - (m >> 15));
 }
 template <int D>
 __device__ __forceinline__ bool clean_values(ValueTile<D, false>& t, int base, int see, int lane) {
     uint32_t any = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const bool dead = base + 8 * (lane >> 4) + j >= see;
+        const uint32_t seen = static_cast<uint32_t>((base + 8 * (lane >> 4) + j - see) >> 31);
 #pragma unroll
         for (int i = 0; i < AttnGeo<D, false>::VD; ++i) {
-            const uint32_t x = dead ? 0u : t.v[j][i], m = special_mask(x);
+            const uint32_t x = t.v[j][i] & seen, m = special_mask(x);
             any |= m;
             t.v[j][i] = x & ~m;
         }
@@ -434,14 +430,13 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {  // a value that every l
     const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
     return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-// Where the share's first step lies: the sequence that holds step w * share of the list, and that
-// sequence's first step; returns the list's length. Every wave finds it by itself, 64 sequences a
-// round (a scan over the workgroup took two barriers and 2 us of the smallest calls); up to 64 sequences
-// are weighed once.
+// The list's length and a share's size, and the item that holds step w * share (if the list is that
+// long). Every wave finds it by itself, 64 sequences a round (a scan over the workgroup took two barriers
+// and 2 us of the smallest calls); up to 64 sequences are weighed once.
 __device__ __forceinline__ int64_t find_share(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t w, int64_t W,
-                                              int* seq, int64_t* seq_start, int64_t* share) {
+                                              AttnCursor* at, int64_t* share) {
     const int lane = threadIdx.x & 63;
-    auto weight = [&](int s) { return s < B.seqs ? static_cast<int64_t>(attn_weight(S, B, shift, s)) : 0; };
+    auto weight = [&](int s) { return s < B.seqs ? attn_weight(S, B, shift, s) : 0; };
     int64_t mine = 0, sum = 0;
     for (int s0 = 0; s0 < B.seqs; s0 += 64) sum += mine = weight(s0 + lane);
     for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
@@ -459,14 +454,57 @@ __device__ __forceinline__ int64_t find_share(const AttnSplit& S, const PagedBat
         const uint64_t past = __ballot(before + upto > want);
         if (past) {
             const int l = __builtin_ctzll(past);
-            *seq = __builtin_amdgcn_readfirstlane(s0 + l);
-            *seq_start = before + uniform(__shfl(upto - mine, l));
+            const AttnCursor c = attn_seek(S, B, shift, __builtin_amdgcn_readfirstlane(s0 + l),
+                                           before + uniform(__shfl(upto - mine, l)), want);
+            *at = AttnCursor{c.seq, __builtin_amdgcn_readfirstlane(c.tile), uniform(c.start)};
             break;
         }
         before += uniform(__shfl(upto, 63));
     }
     return sum;
 }
+// A wave's walk through its share. It lies in LDS between the pieces: nothing of it is needed while a
+// piece is worked on, and in registers it cost the inner loops theirs.
+struct ShareWalk {
+    AttnCursor at;
+    int64_t pos, end, share, start;  // start: the current piece's item
+    int first, rows, tokens, bad, tile, from, to;
+
+    // false where the share is empty
+    __device__ __forceinline__ bool open(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t w, int64_t W) {
+        AttnCursor c{0, 0, 0};
+        int64_t sh = 0;
+        const int64_t total = find_share(S, B, shift, w, W, &c, &sh);
+        if (w * sh >= total) return false;
+        if ((threadIdx.x & 63) == 0) at = c, share = sh, pos = w * sh, end = min(total, (w + 1) * sh);
+        return true;
+    }
+    // The next piece; the same for all lanes.
+    __device__ __forceinline__ bool next(const AttnSplit& S, const PagedBatchDev& B, int shift) {
+        AttnCursor c{__builtin_amdgcn_readfirstlane(at.seq), __builtin_amdgcn_readfirstlane(at.tile), uniform(at.start)};
+        int64_t p = uniform(pos);
+        AttnPiece pc;
+        if (!attn_next(S, B, shift, uniform(end), &c, &p, &pc)) return false;
+        if ((threadIdx.x & 63) == 0) {
+            at = c, pos = p, start = pc.start, seq_ = pc.it.seq;
+            first = pc.it.first, rows = pc.it.rows, tokens = pc.it.tokens, bad = pc.it.bad, tile = pc.it.tile;
+            from = pc.from, to = pc.to;
+        }
+        return true;
+    }
+    __device__ __forceinline__ AttnItem item(const AttnSplit& S) const {
+        AttnItem it;
+        it.seq = 0;
+        it.first = __builtin_amdgcn_readfirstlane(first);
+        it.rows = __builtin_amdgcn_readfirstlane(rows);
+        it.tokens = __builtin_amdgcn_readfirstlane(tokens);
+        it.bad = __builtin_amdgcn_readfirstlane(bad);
+        attn_tile(S, __builtin_amdgcn_readfirstlane(tile), &it);
+        return it;
+    }
+    __device__ __forceinline__ int seq() const { return __builtin_amdgcn_readfirstlane(seq_); }
+    int seq_;
+};
 
 // A workgroup's share of a kv head's steps; wave i takes tokens 32 i .. 32 i + 31 of every step, the
 // next step's keys and values in flight, and the waves' sums are joined through LDS at the end of
@@ -482,26 +520,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
     __shared__ int flags[kSplitWaves];
     const AttnSplit S{G, M, kSplitTokens};
     const int w = blockIdx.x, W = gridDim.x, head = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int seq = 0;
-    int64_t seq_start = 0, share = 0;
-    const int64_t total = find_share(S, B, C.shift, w, W, &seq, &seq_start, &share);
-    int64_t pos = w * share;
-    const int64_t end = min(total, pos + share);
-    AttnPiece pc;
-    while (attn_next(S, B, C.shift, end, &seq, &seq_start, &pos, &pc)) {
-        const AttnItem& it = pc.it;
-        PageWalk walk{B.table + static_cast<int64_t>(it.seq) * B.width, C.shift, C.pages, C.hkv, head, it.see, it.bad};
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ ShareWalk walks[kSplitWaves];
+    ShareWalk& sw = walks[wave];
+    if (!sw.open(S, B, C.shift, w, W)) return;
+    while (sw.next(S, B, C.shift)) {
+        // (opaque: what follows from the lane is formed anew per piece, not kept in registers for the next)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        AttnItem it = sw.item(S);
+        PageWalk walk{B.table + static_cast<int64_t>(sw.seq()) * B.width, C.shift, C.pages, C.hkv, head, it.see, it.bad};
         // tokens that every query of the tile sees: steps below need no mask
-        const int all = attn_see(it, it.tile * M / G);
+        const int all = attn_see(it, it.tile * S.rows());
         QueryTile<D, Q8, MT> qt;
         AttnState<D, Q8, MT> st;
         qt.load(q, qs, it, S, head, 0, c < 0.0f, lane);
         st.clear(it, S, 0, lane);
         KeyTile<D, Q8> kt;
         ValueTile<D, Q8> vt;
-        int base = pc.from * kSplitTokens + 32 * wave;
-        const int stop = min(pc.to * kSplitTokens, it.see);
+        int base = __builtin_amdgcn_readfirstlane(sw.from) * kSplitTokens + 32 * wave;
+        const int stop = min(__builtin_amdgcn_readfirstlane(sw.to) * kSplitTokens, it.see);
         HalfRows at{0, 0};
         bool special = false;
         if (base < stop) {
@@ -512,12 +550,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         }
         for (; base < stop; base += kSplitTokens) {
             const bool more = base + kSplitTokens < stop, masked = base + 32 > all;
-            float p[MT][8];
-            st.scores(kt, qt, fabsf(c), base, masked, lane, p);
+            uintx4 b[MT];
+            st.scores(kt, qt, fabsf(c), base, masked, lane, vt.s, b);
             if (more) load_keys<D, Q8>(C, at, lane, kt);
             if constexpr (!Q8)
                 if (masked) special |= clean_values<D>(vt, base, it.see, lane);
-            st.values(vt, p, base, lane);
+            st.template products<Q8>(vt, b);
             if (more) load_values<D, Q8>(C, at, lane, vt);
             if (base + 2 * kSplitTokens < stop) at = walk.rows(base + 2 * kSplitTokens);
         }
@@ -544,50 +582,52 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         if (lane == 0) flags[wave] = special;
         __syncthreads();
         special = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
-        const bool whole = pc.to - pc.from == it.steps;
+        asm volatile("" ::: "memory");  // (read anew: see ShareWalk)
+        it = sw.item(S);
+        const int from = sw.from;
+        const bool whole = sw.to - from == it.steps;
         float* pd = nullptr;
-        if (!whole) pd = part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(pc.start, share, w)) * (M * (D + 2));
+        if (!whole) pd = part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(sw.start, sw.share, w)) * (M * (D + 2));
         for (int e = threadIdx.x; e < M * D / 4; e += 256) {
-            const int row = e / (D / 4), d = e % (D / 4) * 4, idx = it.tile * M + row;
-            if (idx >= it.rows * G) continue;
-            float top = stats[row];
+            const int i = e / (D / 4), d = e % (D / 4) * 4, row = tile_row(S, it, i);
+            if (row < 0) continue;
+            float top = stats[i];
 #pragma unroll
-            for (int i = 1; i < kSplitWaves; ++i) top = fmaxf(top, stats[i * M + row]);
+            for (int n = 1; n < kSplitWaves; ++n) top = fmaxf(top, stats[n * M + i]);
             const float ref = top == -INFINITY ? 0.0f : top;
             float sum = 0.0f;
             floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < kSplitWaves; ++i) {
-                const float f = __builtin_amdgcn_exp2f(stats[i * M + row] - ref);
-                sum += stats[(kSplitWaves + i) * M + row] * f;
-                o += *reinterpret_cast<const floatx4*>(lds + (i * M + row) * LR + d) * f;
+            for (int n = 0; n < kSplitWaves; ++n) {
+                const float f = __builtin_amdgcn_exp2f(stats[n * M + i] - ref);
+                sum += stats[(kSplitWaves + n) * M + i] * f;
+                o += *reinterpret_cast<const floatx4*>(lds + (n * M + i) * LR + d) * f;
             }
             if constexpr (!Q8)
                 if (special)
-                    o = add_special<D>(C, walk.table, head, max(special_from(all), pc.from * kSplitTokens),
-                                       min(stop, attn_see(it, idx / G)), d, o);
+                    o = add_special<D>(C, walk.table, head, max(special_from(all), from * kSplitTokens),
+                                       min(stop, attn_see(it, row)), d, o);
             if (whole) {
-                const float inv = it.bad || attn_see(it, idx / G) > 0 ? 1.0f / sum : 0.0f;
+                const float inv = it.bad || attn_see(it, row) > 0 ? 1.0f / sum : 0.0f;
                 const uint2 x = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-                *reinterpret_cast<uint2*>(out + (it.first + idx / G) * os + (head * G + idx % G) * D + d) = x;
+                *reinterpret_cast<uint2*>(out + (it.first + row) * os + (head * G + i % G) * D + d) = x;
             } else {
-                *reinterpret_cast<floatx4*>(pd + row * D + d) = o;
-                if (d == 0) pd[M * D + row] = top, pd[M * D + M + row] = sum;
+                *reinterpret_cast<floatx4*>(pd + i * D + d) = o;
+                if (d == 0) pd[M * D + i] = top, pd[M * D + M + i] = sum;
             }
         }
     }
 }
 
-// ---- many queries per sequence. A workgroup takes M = 32 x waves queries of one item and one of
-// `splits` equal ranges of its tokens; keys and values go through LDS, TB tokens at a time and the
-// next ones in flight (an 8-bit cache is converted on the way: its codes are exact in bf16), and
+// ---- many queries per sequence. Tiles of M = 128 queries, 32 per wave, in equal shares as above;
+// keys and values go through LDS, TB tokens at a time and the next ones in flight (an 8-bit cache is converted on the way: its codes are exact in bf16), and
 // every wave multiplies them with its own 32 queries. Bound by the matrix cores, by the
 // exponentials beside them (8 per lane for 16 products of 128 dims) and by LDS reads, which 32
 // queries per wave bring to the matrix cores' own time.
 template <int D>
 struct TileGeo {
-    static constexpr int WAVES = 4;
-    static constexpr int M = 32 * WAVES;
+    // 16-query groups per wave, waves and so 128 queries; 256 dims take the registers of two groups
+    static constexpr int MT = D == 256 ? 1 : 2, WAVES = D == 256 ? 8 : 4, M = 16 * MT * WAVES;
     static constexpr int TB = D == 64 ? 64 : 32;
     static constexpr int CH = D / 8;                       // 16-byte chunks of a bf16 row
     static constexpr int PIECES = TB * CH / (64 * WAVES);  // chunks per thread
@@ -600,76 +640,51 @@ __device__ __forceinline__ int tile_at(int token, int chunk) {
     return token * (D / 8) + (chunk ^ ((token & 3) | ((token >> 1) & 4)));
 }
 
-// Which item a workgroup takes: the sequences' tiles in order, a sequence's last (longest) first.
-__device__ __forceinline__ bool find_tile(const AttnSplit& S, const PagedBatchDev& B, int shift, int want, AttnItem* it) {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int s0 = 0; s0 < B.seqs; s0 += 64) {
-        const int s = s0 + lane;
-        int n = 0;
-        if (s < B.seqs) {
-            const RowSpan span = row_span(B.off, s, B.rows);
-            n = attn_tiles(S, span.end - span.begin);
-        }
-        int upto = n;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(upto, d);
-            if (lane >= d) upto += x;
-        }
-        const uint64_t past = __ballot(before + upto > want);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            attn_sequence(B, shift, __builtin_amdgcn_readfirstlane(s0 + l), it);
-            const int tiles = __builtin_amdgcn_readfirstlane(__shfl(n, l));
-            const int start = before + __builtin_amdgcn_readfirstlane(__shfl(upto, l)) - tiles;
-            attn_tile(S, tiles - 1 - (want - start), it);
-            return true;
-        }
-        before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
-    }
-    return false;
-}
-
 template <int D, bool Q8>
-__global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_paged_tile(
-    PagedCacheDev C, PagedBatchDev B, int G, const uint16_t* __restrict__ q, int64_t qs, float c, uint16_t* __restrict__ out,
-    int64_t os, float* __restrict__ part) {
+__global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
+    PagedCacheDev C, PagedBatchDev B, int G, int shares, const uint16_t* __restrict__ q, int64_t qs, float c,
+    uint16_t* __restrict__ out, int64_t os, float* __restrict__ part) {
     using Geo = AttnGeo<D, false>;
     using TG = TileGeo<D>;
-    constexpr int TB = TG::TB, NT = 64 * TG::WAVES, CH = TG::CH, PC = TG::PIECES, MT = 2;
+    constexpr int TB = TG::TB, NT = 64 * TG::WAVES, CH = TG::CH, PC = TG::PIECES, MT = TG::MT;
     extern __shared__ uintx4 tiles[];  // [2][keys, values][TB][CH], then [2][key, value scales][TB]
     float* const scales = reinterpret_cast<float*>(tiles + 4 * TB * CH);
-    const AttnSplit S{G, TG::M, TB};
-    const int head = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const AttnSplit S{G, TG::M, kSplitTokens};
+    // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD takes neighbouring shares of
+    // one head, whose tiles read the same keys and values at about the same time.
+    const int per_xcd = gridDim.x / 8, n = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+    if (n >= shares * C.hkv) return;
+    const int head = n / shares, place = n % shares, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m0 = wave * 16 * MT;
+    const bool negate = c < 0.0f;
+    c = fabsf(c);
+    __shared__ ShareWalk walks[TG::WAVES];
+    ShareWalk& sw = walks[wave];
+    if (!sw.open(S, B, C.shift, place, shares)) return;
+    while (sw.next(S, B, C.shift)) {
+    // (opaque: what follows from the lane is formed anew per piece, not kept in registers for the next)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
     const int u = lane & 15, w = lane >> 4;
-    AttnItem it;
-    if (!find_tile(S, B, C.shift, blockIdx.x, &it)) return;
-    // (read by vector loads: told to be the same for all lanes, for scalar branches)
-    it.first = __builtin_amdgcn_readfirstlane(it.first);
-    it.rows = __builtin_amdgcn_readfirstlane(it.rows);
-    it.tokens = __builtin_amdgcn_readfirstlane(it.tokens);
-    it.bad = __builtin_amdgcn_readfirstlane(it.bad);
-    attn_tile(S, __builtin_amdgcn_readfirstlane(it.tile), &it);
-    const int per = (it.steps + gridDim.z - 1) / gridDim.z, from = blockIdx.z * per, to = min(it.steps, from + per);
-    if (from >= to) return;
-    const int m0 = wave * 32, i0 = it.tile * TG::M + m0, rows = it.rows * G;
+    AttnItem it = sw.item(S);
     QueryTile<D, false, MT> qt;
     AttnState<D, Q8, MT> st;
-    qt.load(q, qs, it, S, head, m0, c < 0.0f, lane);
+    qt.load(q, qs, it, S, head, m0, negate, lane);
     st.clear(it, S, m0, lane);
-    c = fabsf(c);
     // tokens that all, and any, of the wave's queries see
-    const int all = i0 < rows ? attn_see(it, i0 / G) : 0;
-    const int any = i0 < rows ? attn_see(it, min(i0 + 31, rows - 1) / G) : 0;
-    const int stop = min(to * TB, it.see);
-    const int32_t* table = B.table + static_cast<int64_t>(it.seq) * B.width;
-    PageWalk walk{table, C.shift, C.pages, C.hkv, head, max(it.see, 1), it.bad};
+    const int r0 = tile_row(S, it, m0), rows_left = min(it.rows, (it.tile + 1) * S.rows());
+    const int all = r0 >= 0 ? attn_see(it, r0) : 0;
+    const int any = r0 >= 0 ? attn_see(it, min(it.tile * S.rows() + (m0 + 16 * MT - 1) / G, rows_left - 1)) : 0;
+    const int from = __builtin_amdgcn_readfirstlane(sw.from) * (kSplitTokens / TB);
+    const int stop = min(__builtin_amdgcn_readfirstlane(sw.to) * kSplitTokens, it.see);
+    const int to = max(from + 1, (stop + TB - 1) / TB);
+    PageWalk walk{B.table + static_cast<int64_t>(sw.seq()) * B.width, C.shift, C.pages, C.hkv, head, max(it.see, 1), it.bad};
     bool special = false;
 
     // Staging. A wave's piece of a tile lies in 16 tokens of one page: uniform addresses and a lane's
     // own offset. What lies behind the seen tokens is read with them and masked by its reader.
     constexpr int EL = Q8 ? 1 : 2;
-    const int ch = threadIdx.x % CH, wt = wave * 64 / CH;  // the wave's first token of a piece
+    const int ch = lane % CH, wt = wave * 64 / CH;  // the wave's first token of a piece
     const uint32_t lane_off = ((lane / CH) * D + 8 * ch) * EL;
     typedef typename std::conditional<Q8, uint2, uintx4>::type raw_t;
     raw_t kr[PC], vr[PC];
@@ -764,13 +779,17 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
                 ks[a] = *reinterpret_cast<const floatx4*>(sc + 32 * sub + 8 * w + 4 * a);
                 vs[a] = *reinterpret_cast<const floatx4*>(sc + TB + 32 * sub + 8 * w + 4 * a);
             }
-        float p[MT][8];
+        uintx4 b[MT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) st.soften(m, s[m], ks, c, base, masked, lane, p[m]);
+        for (int m = 0; m < MT; ++m) {
+            float p[8];
+            st.soften(m, s[m], ks, c, base, masked, lane, p);
+            b[m] = st.weights(m, p, vs, base, lane);
+        }
         if constexpr (D == 256) read_values();
         if constexpr (!Q8)
             if (masked) special |= clean_values<D>(v, base, any, lane);
-        st.values16(v, vs, p, base, lane);
+        st.template products<false>(v, b);
     };
     fetch(from * TB);
     stage(0);
@@ -778,127 +797,120 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, D == 256 ? 1 : 2) void k_pa
     for (int step = from; step < to; ++step) {
         const int buf = (step - from) & 1;
         fetch(min(step + 1, to - 1) * TB);
+        // (waves whose queries see nothing of the tile's end multiply it all the same: a branch around
+        // the products made the compiler move every sum once per step)
         const uintx4* kt = tiles + (2 * buf) * TB * CH;
 #pragma unroll
         for (int sub = 0; sub < TB / 32; ++sub)
-            if (step * TB + 32 * sub < any) half(step * TB + 32 * sub, sub, kt, kt + TB * CH, scales + 2 * buf * TB);
+            half(step * TB + 32 * sub, sub, kt, kt + TB * CH, scales + 2 * buf * TB);
         stage(buf ^ 1);
         lds_barrier();
     }
     const bool bad = __syncthreads_or(it.bad || (it.see > 0 && walk.bad));
-    const bool whole = per >= it.steps;
+    asm volatile("" ::: "memory");  // (read anew: see ShareWalk)
+    it = sw.item(S);
+    const bool whole = sw.to - sw.from == it.steps;
     float* pd = nullptr;
-    if (!whole) pd = part + ((static_cast<int64_t>(blockIdx.x) * C.hkv + head) * gridDim.z + blockIdx.z) * (TG::M * (D + 2));
+    if (!whole)
+        pd = part + ((static_cast<int64_t>(head) * shares + place) * 2 + attn_slot(sw.start, sw.share, place)) * (TG::M * (D + 2));
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         float sum = st.total(m);
         if (bad) sum = kNan;
-        const int idx = i0 + 16 * m + u;
-        if (idx >= rows) continue;
+        const int i = m0 + 16 * m + u, row = tile_row(S, it, i);
+        if (row < 0) continue;
         const float inv = bad || st.lim[m] > 0 ? 1.0f / sum : 0.0f;
-        const int row = m0 + 16 * m + u;
-        uint16_t* dst = out + (it.first + idx / G) * os + (head * G + idx % G) * D;
+        uint16_t* dst = out + (it.first + row) * os + (head * G + i % G) * D;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int o = 0; o < Geo::E; o += 4) {
                 const int d = Geo::dim(4 * w + r, o);
-                floatx4 x = {st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
-                if constexpr (!Q8)
-                    if (special)
-                        x = add_special<D>(C, table, head, max(special_from(all), from * TB), min(stop, st.lim[m]), d, x);
+                const floatx4 x = {st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
                 if (whole)
                     *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
                 else
-                    *reinterpret_cast<floatx4*>(pd + row * D + d) = x;
+                    *reinterpret_cast<floatx4*>(pd + i * D + d) = x;
             }
-        if (!whole && w == 0) pd[TG::M * D + row] = st.top[m], pd[TG::M * D + TG::M + row] = sum;
+        if (!whole && w == 0) pd[TG::M * D + i] = st.top[m], pd[TG::M * D + TG::M + i] = sum;
+    }
+    if constexpr (!Q8)
+        if (special) {  // to what the lane has just written
+#pragma unroll 1
+            for (int n = 0; n < MT * Geo::E; ++n) {
+                const int i = m0 + 16 * (n / Geo::E) + u, row = tile_row(S, it, i);
+                if (row < 0) continue;
+                const int d = Geo::dim(4 * w + n % Geo::E / (Geo::E / 4), 0) + n % (Geo::E / 4) * 4 % Geo::EC +
+                              n % (Geo::E / 4) * 4 / Geo::EC * 16 * Geo::EC;
+                const int t0 = max(special_from(all), from * TB), lim = min(stop, attn_see(it, row));
+                if (whole) {
+                    uint2* p = reinterpret_cast<uint2*>(out + (it.first + row) * os + (head * G + i % G) * D + d);
+                    const floatx4 x = add_special<D>(C, walk.table, head, t0, lim, d,
+                                                     (floatx4){bflo(p->x), bfhi(p->x), bflo(p->y), bfhi(p->y)});
+                    *p = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+                } else {
+                    floatx4* p = reinterpret_cast<floatx4*>(pd + i * D + d);
+                    *p = add_special<D>(C, walk.table, head, t0, lim, d, *p);
+                }
+            }
+        }
     }
 }
 
-// Joins the pieces of an item that several workgroups worked on, a workgroup per (row, query head),
-// each of its waves every fourth piece, eight in flight. TILES: pieces of k_paged_tile, W ranges per
-// item; else those of k_paged_split, W shares.
-template <int D, bool TILES>
+// Joins the pieces of the items that the shares' ends cut: a workgroup per (cut, kv head, QB of the
+// tile's queries), a wave per query, PB pieces in flight; an item's first cut does the work.
+template <int D, int QB, int PB>
 __global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchDev B, AttnSplit S, int W,
-                                                    int items, const float* __restrict__ part,
-                                                    uint16_t* __restrict__ out, int64_t os) {
+                                                    const float* __restrict__ part, uint16_t* __restrict__ out, int64_t os) {
     constexpr int E = D / 64;
-    __shared__ float sums[4][D + 2];
-    const int row = blockIdx.x, lane = threadIdx.x & 63, G = S.G, M = S.M;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
-    const int seq = row_sequence(B.off, B.seqs, row);
-    if (seq < 0) return;
-    // what lies in front of the sequence: steps (and the list's length), or tiles
-    int64_t total = 0, start = 0;
-    for (int s = lane; s < (TILES ? seq : B.seqs); s += 64) {
-        int n;
-        if constexpr (TILES) {
-            const RowSpan span = row_span(B.off, s, B.rows);
-            n = attn_tiles(S, span.end - span.begin);
-        } else {
-            n = attn_weight(S, B, C.shift, s);
-        }
-        total += n;
-        if (s < seq) start += n;
-    }
-    for (int d = 32; d >= 1; d >>= 1) {
-        total += __shfl_xor(total, d);
-        start += __shfl_xor(start, d);
-    }
+    typedef float vec_t __attribute__((ext_vector_type(E)));
+    const int lane = threadIdx.x & 63, head = blockIdx.y, G = S.G, M = S.M;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    AttnCursor at{0, 0, 0};
+    int64_t share = 0;
+    const int64_t cut = blockIdx.x + 1, total = find_share(S, B, C.shift, cut, W, &at, &share);
+    if (cut * share >= total || at.start == cut * share || at.start / share + 1 != cut) return;
     AttnItem it;
-    attn_sequence(B, C.shift, seq, &it);
-    const int idx = (row - it.first) * G + h % G, head = h / G, at = idx % M;
-    int64_t first, step;  // the first piece, and from one to the next
-    int n;
-    if constexpr (TILES) {
-        attn_tile(S, idx / M, &it);
-        const int per = (it.steps + W - 1) / W;
-        n = (it.steps + per - 1) / per;
-        const int64_t item = start + attn_tiles(S, it.rows) - 1 - it.tile;
-        if (item >= items) return;  // (offsets that do not ascend: more tiles than rows)
-        first = (item * C.hkv + head) * W;
-        step = 1;
-    } else {
-        const int64_t share = (total + W - 1) / W;
-        for (int j = 0; j < idx / M; ++j) {
-            attn_tile(S, j, &it);
-            start += it.steps;
+    attn_sequence(B, C.shift, at.seq, &it);
+    attn_tile(S, at.tile, &it);
+    const int n = static_cast<int>((at.start + it.steps - 1) / share - at.start / share) + 1;
+    // (an item goes on behind its first share, whose second slot it takes; it began before the others)
+    const float* first = part + ((static_cast<int64_t>(head) * W + cut - 1) * 2 + 1) * (M * (D + 2));
+    auto piece = [&](int i) { return first + static_cast<int64_t>(2 * i - (i > 0)) * (M * (D + 2)); };
+#pragma unroll 2
+    for (int j = wave; j < QB; j += 4) {
+        const int i = blockIdx.z * QB + j, row = tile_row(S, it, i);
+        if (row < 0) continue;
+        float top = -INFINITY, sum = 0.0f;
+        vec_t o = {};
+        for (int p0 = 0; p0 < n; p0 += PB) {
+            float t[PB], l[PB], now = top;
+            vec_t x[PB];
+#pragma unroll
+            for (int p = 0; p < PB; ++p) {
+                const float* src = piece(min(p0 + p, n - 1));
+                t[p] = src[M * D + i];
+                l[p] = src[M * D + M + i];
+                x[p] = *reinterpret_cast<const vec_t*>(src + i * D + lane * E);
+                if (p0 + p >= n) t[p] = -INFINITY;
+                now = fmaxf(now, t[p]);
+            }
+            const float ref = now == -INFINITY ? 0.0f : now, keep = __builtin_amdgcn_exp2f(top - ref);
+            top = now;
+            sum *= keep;
+            o *= keep;
+#pragma unroll
+            for (int p = 0; p < PB; ++p) {
+                // (a repeated piece counts nothing, also where it holds a NaN)
+                const float f = p0 + p < n ? __builtin_amdgcn_exp2f(t[p] - ref) : 0.0f;
+                sum = p0 + p < n ? fmaf(l[p], f, sum) : sum;
+                o = p0 + p < n ? o + x[p] * f : o;
+            }
         }
-        attn_tile(S, idx / M, &it);
-        const int64_t w0 = start / share, w1 = (start + it.steps - 1) / share;
-        n = static_cast<int>(w1 - w0) + 1;
-        // (an item goes on behind its first share, whose second slot it takes; it began before the others)
-        first = (static_cast<int64_t>(head) * W + w0) * 2 + 1;
-        step = 2;
-    }
-    if (n == 1) return;
-    auto piece = [&](int i) { return part + (first + i * step - (!TILES && i > 0)) * (M * (D + 2)); };
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, piece(i)[M * D + at]);
-    top = wave_max(top);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o[E] = {};
-#pragma unroll 8
-    for (int i = wave; i < n; i += 4) {
-        const float* src = piece(i);
-        const float f = __builtin_amdgcn_exp2f(src[M * D + at] - ref);
-        sum = fmaf(src[M * D + M + at], f, sum);
+        const float inv = it.bad || attn_see(it, row) > 0 ? 1.0f / sum : 0.0f;
+        uint16_t* dst = out + (it.first + row) * os + (head * G + i % G) * D + lane * E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(src[at * D + lane * E + e], f, o[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = o[e];
-    if (lane == 0) sums[wave][D] = sum;
-    __syncthreads();
-    if (wave) return;
-    sum = sums[0][D] + sums[1][D] + sums[2][D] + sums[3][D];
-    const float inv = it.bad || attn_see(it, idx / G) > 0 ? 1.0f / sum : 0.0f;
-    uint16_t* dst = out + row * os + h * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        dst[e] = f2bf((sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) * inv);
+        for (int e = 0; e < E; ++e) dst[e] = f2bf(o[e] * inv);
     }
 }
 
@@ -917,32 +929,23 @@ hipError_t launch_paged_append(const PagedCacheDev& C, bool q8, const PagedBatch
 namespace {
 
 // Up to 32 queries per sequence and kv head the split kernel reads every token once; above, the tile
-// kernel does so once per 128 or 256 queries.
+// kernel does so once per 128.
 struct AttnPlan {
-    bool tiles;
-    int mt;         // split: 16-query groups
-    int W;          // split: workgroups per kv head; tiles: ranges per item
-    int items;      // tiles: items at most
-    bool joined;
-    int M;
+    bool tiles, joined;
+    int mt;  // split: 16-query groups
+    int M;   // queries per tile
+    int W;   // shares per kv head
 };
 AttnPlan attn_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
     AttnPlan p{};
-    const int64_t G = hq / C.hkv, queries = max_rows * G, span = static_cast<int64_t>(B.width) << C.shift;
+    const int G = hq / C.hkv;
+    const int64_t queries = static_cast<int64_t>(max_rows) * G;
     p.tiles = queries > 32;
-    if (!p.tiles) {
-        p.mt = queries <= 16 ? 1 : 2;
-        p.M = 16 * p.mt;
-        p.W = std::max(1, 256 * (C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernel's occupancy
-        p.joined = span > kSplitTokens;  // (no sequence of the table is longer than a step: nothing is split)
-    } else {
-        p.M = TileGeo<64>::M;
-        p.items = static_cast<int>(std::min<int64_t>(B.rows * G / p.M + B.seqs, B.rows * G));
-        // ranges of at least 256 tokens, until there are about two workgroups per CU
-        const int64_t blocks = std::max<int64_t>(1, static_cast<int64_t>(p.items) * C.hkv);
-        p.W = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / blocks, (span + 255) / 256)));
-        p.joined = p.W > 1;
-    }
+    p.mt = queries <= 16 ? 1 : 2;
+    p.M = p.tiles ? TileGeo<64>::M : 16 * p.mt;
+    p.W = std::max(1, 256 * (C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernels' occupancy
+    // (no sequence is longer than a step, or a share holds its head's whole list: nothing is cut inside an item)
+    p.joined = p.W > 1 && (static_cast<int64_t>(B.width) << C.shift) > kSplitTokens;
     return p;
 }
 
@@ -965,21 +968,21 @@ hipError_t launch_attention(const PagedCacheDev& C, const PagedBatchDev& B, cons
     } else {
         e = ensure_lds<k_paged_tile<D, Q8>>(TileGeo<D>::kLds);
         if (e == hipSuccess)
-            e = launch(k_paged_tile<D, Q8>, dim3(p.items, C.hkv, p.W), dim3(64 * TileGeo<D>::WAVES), TileGeo<D>::kLds, st, C, B,
-                       hq / C.hkv, q, qs, c, out, os, part);
+            e = launch(k_paged_tile<D, Q8>, dim3((p.W * C.hkv + 7) / 8 * 8), dim3(64 * TileGeo<D>::WAVES), TileGeo<D>::kLds,
+                       st, C, B, hq / C.hkv, p.W, q, qs, c, out, os, part);
     }
     if (e != hipSuccess || !p.joined) return e;
-    const AttnSplit S{hq / C.hkv, p.M, p.tiles ? TileGeo<D>::TB : kSplitTokens};
-    const dim3 grid(B.rows, hq);
-    return p.tiles ? launch(k_paged_join<D, true>, grid, dim3(256), 0, st, C, B, S, p.W, p.items, part, out, os)
-                   : launch(k_paged_join<D, false>, grid, dim3(256), 0, st, C, B, S, p.W, p.items, part, out, os);
+    const AttnSplit S{hq / C.hkv, p.M, kSplitTokens};
+    if (p.tiles)
+        return launch(k_paged_join<D, 32, 2>, dim3(p.W - 1, C.hkv, p.M / 32), dim3(256), 0, st, C, B, S, p.W, part, out, os);
+    return launch(k_paged_join<D, 4, 8>, dim3(p.W - 1, C.hkv, p.M / 4), dim3(256), 0, st, C, B, S, p.W, part, out, os);
 }
 
 } // namespace
 
 size_t paged_attention_ws(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
     const AttnPlan p = attn_plan(C, B, max_rows, hq);
-    const size_t pieces = static_cast<size_t>(C.hkv) * p.W * (p.tiles ? p.items : 2);
+    const size_t pieces = static_cast<size_t>(C.hkv) * p.W * 2;
     return p.joined ? pieces * p.M * (C.d + 2) * 4 : 0;
 }
 

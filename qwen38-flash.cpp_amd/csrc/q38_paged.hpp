@@ -63,24 +63,25 @@ __host__ __device__ inline int64_t cache_row(int32_t page, int pages, int hkv, i
 }
 
 // ---- how attention's work is split. A batch's work per kv head is a list of items, one per
-// (sequence, tile of M of its rows x group queries), each of so many steps of T tokens (at least
-// one: a tile that sees nothing still writes its zeros). The list of steps is cut into equal
-// shares, one per workgroup, whatever sequences they belong to, so that one long sequence or many
-// ragged ones load the chip evenly. An item inside one share is finished there; the pieces of the
-// others are joined by a second kernel.
-struct AttnItem {
-    int seq, tile;       // sequence, tile of its queries
-    int rows;            // the sequence's rows
-    int first;           // its first row in the tensors
-    int tokens;          // its tokens (0 where they are negative or behind the table)
-    int see;             // tokens that the tile's last row sees
-    int steps;           // max(1, ceil(see / T))
-    bool bad;            // tokens behind the table
-};
+// (sequence, tile of R of its rows), each of so many steps of T tokens (at least one: a tile that
+// sees nothing still writes its zeros). The list of steps is cut into equal shares, one per
+// workgroup, whatever sequences they belong to, so that one long sequence, many ragged ones or the
+// tiles of a prompt, each a little longer than the one before, load the chip evenly. An item inside
+// one share is finished there; the pieces of the others are joined by a second kernel.
 struct AttnSplit {
-    int G, M, T;  // queries per kv head and row; queries per tile; tokens per step
+    int G, M, T;  // queries per kv head and row; queries per tile (the tile's rows: M / G >= 1); tokens per step
+    __host__ __device__ int rows() const { return M / G; }
 };
-__host__ __device__ inline int attn_tiles(const AttnSplit& S, int rows) { return (rows * S.G + S.M - 1) / S.M; }
+struct AttnItem {
+    int seq, tile;
+    int rows;    // the sequence's rows
+    int first;   // its first row in the tensors
+    int tokens;  // its tokens (0 where they are negative or behind the table)
+    int see;     // tokens that the tile's last row sees
+    int steps;   // max(1, ceil(see / T))
+    bool bad;    // tokens behind the table
+};
+__host__ __device__ inline int attn_tiles(const AttnSplit& S, int rows) { return (rows + S.rows() - 1) / S.rows(); }
 __host__ __device__ inline void attn_sequence(const PagedBatchDev& B, int shift, int seq, AttnItem* it) {
     const RowSpan span = row_span(B.off, seq, B.rows);
     it->seq = seq;
@@ -96,48 +97,89 @@ __host__ __device__ inline int attn_see(const AttnItem& it, int r) {
     return n < 0 ? 0 : n;
 }
 __host__ __device__ inline void attn_tile(const AttnSplit& S, int tile, AttnItem* it) {
-    const int last = (tile + 1) * S.M - 1, end = it->rows * S.G - 1;
+    const int behind = (tile + 1) * S.rows();
     it->tile = tile;
-    it->see = attn_see(*it, (last < end ? last : end) / S.G);
+    it->see = attn_see(*it, (behind < it->rows ? behind : it->rows) - 1);
     it->steps = it->see > S.T ? (it->see + S.T - 1) / S.T : 1;
 }
-// Steps of all tiles of a sequence.
-__host__ __device__ inline int attn_weight(const AttnSplit& S, const PagedBatchDev& B, int shift, int seq) {
-    AttnItem it;
-    attn_sequence(B, shift, seq, &it);
-    int sum = 0;
-    for (int j = 0, n = attn_tiles(S, it.rows); j < n; ++j) {
-        attn_tile(S, j, &it);
-        sum += it.steps;
+// sum over i < n of floor((a i + b) / m), by Euclid's steps (the lattice points under a line)
+__host__ __device__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    int64_t sum = 0;
+    while (n) {
+        sum += static_cast<int64_t>(n - 1) * n / 2 * (a / m) + static_cast<int64_t>(n) * (b / m);
+        a %= m;
+        b %= m;
+        const uint32_t top = a * n + b;
+        if (top < m) break;
+        n = top / m;
+        b = top % m;
+        const uint32_t t = m;
+        m = a;
+        a = t;
     }
     return sum;
 }
-// A share's next piece: `it` and its steps [from, to), the item's first step at `start` of the
-// whole list. Call with *pos inside sequence seq, whose first step is at seq_start; moves *pos, and
-// *seq and *seq_start with it.
+// Steps of the sequence's tiles 0 .. n - 1 (n <= its tiles; all but its last tile have their R rows).
+__host__ __device__ inline int64_t attn_before(const AttnSplit& S, const AttnItem& it, int n) {
+    const int R = S.rows(), seen = it.tokens - it.rows;  // tokens in front of the first row
+    int64_t sum = 0;
+    if (n == attn_tiles(S, it.rows) && n > 0) {
+        AttnItem last = it;
+        attn_tile(S, --n, &last);
+        sum = last.steps;
+    }
+    const int blind = seen < 0 ? (-seen / R < n ? -seen / R : n) : 0;  // tiles that see nothing
+    return sum + blind + floor_sum(n - blind, S.T, R, seen + (blind + 1) * R + S.T - 1);
+}
+__host__ __device__ inline int64_t attn_weight(const AttnSplit& S, const PagedBatchDev& B, int shift, int seq) {
+    AttnItem it;
+    attn_sequence(B, shift, seq, &it);
+    return attn_before(S, it, attn_tiles(S, it.rows));
+}
+// A place in the list: an item and its first step.
+struct AttnCursor {
+    int seq, tile;
+    int64_t start;
+};
+// The item that holds step pos, inside sequence seq, whose first step is seq_start.
+__host__ __device__ inline AttnCursor attn_seek(const AttnSplit& S, const PagedBatchDev& B, int shift, int seq,
+                                                int64_t seq_start, int64_t pos) {
+    AttnItem it;
+    attn_sequence(B, shift, seq, &it);
+    int lo = 0, hi = attn_tiles(S, it.rows);
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (seq_start + attn_before(S, it, mid) <= pos) lo = mid;
+        else hi = mid;
+    }
+    return AttnCursor{seq, lo, seq_start + (lo ? attn_before(S, it, lo) : 0)};
+}
+// A share's next piece: an item's steps [from, to), the item's first step at `start` of the list. The
+// cursor stands at the item that holds step *pos and moves with it.
 struct AttnPiece {
     AttnItem it;
     int from, to;
     int64_t start;
 };
-__host__ __device__ inline bool attn_next(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t end, int* seq,
-                                          int64_t* seq_start, int64_t* pos, AttnPiece* out) {
-    while (*pos < end && *seq < B.seqs) {
-        attn_sequence(B, shift, *seq, &out->it);
-        int64_t at = *seq_start;
-        for (int j = 0, n = attn_tiles(S, out->it.rows); j < n; ++j) {
-            attn_tile(S, j, &out->it);
-            if (*pos < at + out->it.steps) {
-                out->start = at;
-                out->from = static_cast<int>(*pos - at);
-                out->to = static_cast<int>((end < at + out->it.steps ? end : at + out->it.steps) - at);
-                *pos = at + out->to;
-                return true;
+__host__ __device__ inline bool attn_next(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t end,
+                                          AttnCursor* at, int64_t* pos, AttnPiece* out) {
+    while (*pos < end && at->seq < B.seqs) {
+        attn_sequence(B, shift, at->seq, &out->it);
+        if (at->tile < attn_tiles(S, out->it.rows)) {
+            attn_tile(S, at->tile, &out->it);
+            const int64_t behind = at->start + out->it.steps;
+            out->start = at->start;
+            out->from = static_cast<int>(*pos - at->start);
+            out->to = static_cast<int>((end < behind ? end : behind) - at->start);
+            *pos = at->start + out->to;
+            if (*pos == behind) {
+                at->start = behind;
+                ++at->tile;
             }
-            at += out->it.steps;
+            return true;
         }
-        *seq_start = at;
-        ++*seq;
+        ++at->seq;
+        at->tile = 0;
     }
     return false;
 }

@@ -43,8 +43,18 @@ static void rows_and_pages() {
     CHECK(cache_row(3000000, 3000001, 64, 63, 10, 1023) == ((int64_t{3000000} * 64 + 63) << 10) + 1023);
 }
 
+static void sums(std::mt19937& rng) {
+    for (int n = 0; n < 3000; ++n) {
+        const uint32_t m = 1 + rng() % 300, a = rng() % 300, b = rng() % 5000, k = rng() % 200;
+        int64_t want = 0;
+        for (uint32_t i = 0; i < k; ++i) want += (a * i + b) / m;
+        CHECK(floor_sum(k, m, a, b) == want);
+    }
+    CHECK(floor_sum(1u << 19, 128, 1, (1u << 30)) > 0);
+}
+
 // Every step of every item is in exactly one share's piece, in order; pieces that are not whole
-// items have a slot of their own; and the joining side finds the same pieces.
+// items have a slot of their own; and the joining side finds the same pieces from the cuts.
 static void split(std::mt19937& rng, int seqs, int max_rows, int max_tokens, const AttnSplit& S, int W, bool wild) {
     auto pick = [&](int lo, int hi) { return static_cast<int>(rng() % static_cast<unsigned>(hi - lo + 1)) + lo; };
     const int shift = 4, width = max_tokens / 16 + 1;
@@ -59,23 +69,37 @@ static void split(std::mt19937& rng, int seqs, int max_rows, int max_tokens, con
     if (wild) off[static_cast<size_t>(pick(0, seqs))] = pick(-9, rows + 20);
     const PagedBatchDev B{off.data(), tokens.data(), nullptr, seqs, rows, width};
     std::vector<int64_t> start{0};
-    for (int i = 0; i < seqs; ++i) start.push_back(start.back() + attn_weight(S, B, shift, i));
+    for (int i = 0; i < seqs; ++i) {
+        AttnItem it;
+        attn_sequence(B, shift, i, &it);
+        int64_t sum = 0;
+        for (int j = 0; j < attn_tiles(S, it.rows); ++j) {
+            CHECK(attn_before(S, it, j) == sum);
+            attn_tile(S, j, &it);
+            sum += it.steps;
+        }
+        CHECK(attn_weight(S, B, shift, i) == sum);
+        start.push_back(start.back() + sum);
+    }
+    auto sequence_at = [&](int64_t pos) {
+        int seq = 0;
+        while (seq < seqs && start[static_cast<size_t>(seq) + 1] <= pos) ++seq;
+        return seq;
+    };
     const int64_t total = start.back(), share = (total + W - 1) / W;
     std::map<std::pair<int, int>, int> seen;  // item -> steps so far
     std::map<std::pair<int, int>, std::set<std::pair<int64_t, int>>> parts;
-    for (int64_t w = 0; w < W && share; ++w) {
+    for (int64_t w = 0; w < W && w * share < total; ++w) {
         const int64_t end = std::min(total, (w + 1) * share);
-        int64_t pos = w * share;
-        int seq = 0;
-        while (seq < seqs && start[static_cast<size_t>(seq) + 1] <= pos) ++seq;
-        int64_t seq_start = start[static_cast<size_t>(seq)];
+        int64_t pos = w * share, before = pos;
+        const int seq = sequence_at(pos);
+        AttnCursor at = attn_seek(S, B, shift, seq, start[static_cast<size_t>(seq)], pos);
         std::set<int> slots;
         AttnPiece p;
-        int64_t before = pos;
-        while (attn_next(S, B, shift, end, &seq, &seq_start, &pos, &p)) {
-            CHECK(p.from < p.to && p.to <= p.it.steps && pos - before == p.to - p.from);
+        while (attn_next(S, B, shift, end, &at, &pos, &p)) {
+            CHECK(p.from >= 0 && p.from < p.to && p.to <= p.it.steps && pos - before == p.to - p.from);
             before = pos;
-            CHECK(p.it.seq >= 0 && p.it.seq < seqs && p.it.rows > 0 && p.it.tile * S.M < p.it.rows * S.G);
+            CHECK(p.it.seq >= 0 && p.it.seq < seqs && p.it.rows > 0 && p.it.tile * S.rows() < p.it.rows);
             CHECK(p.it.first >= 0 && p.it.first + p.it.rows <= rows);
             CHECK(static_cast<int64_t>(p.it.see) <= static_cast<int64_t>(width) * 16);
             CHECK(static_cast<int64_t>(p.it.steps) * S.T >= p.it.see && (p.it.steps - 1) * S.T < std::max(1, p.it.see));
@@ -87,32 +111,39 @@ static void split(std::mt19937& rng, int seqs, int max_rows, int max_tokens, con
                 parts[{p.it.seq, p.it.tile}].insert({w, attn_slot(p.start, share, w)});
             }
         }
-        CHECK(pos >= end);
+        CHECK(pos == end);
     }
-    // the joining side, from an item's first step alone
     for (int i = 0; i < seqs; ++i) {
         AttnItem it;
         attn_sequence(B, shift, i, &it);
-        int64_t at = start[static_cast<size_t>(i)];
         for (int j = 0; j < attn_tiles(S, it.rows); ++j) {
             attn_tile(S, j, &it);
             CHECK((seen[{i, j}] == it.steps));
-            const int64_t w0 = at / share, w1 = (at + it.steps - 1) / share;
-            std::set<std::pair<int64_t, int>> want;
-            if (w0 != w1)
-                for (int64_t w = w0; w <= w1; ++w) want.insert({w, attn_slot(at, share, w)});
-            CHECK((want == parts[{i, j}]));
-            at += it.steps;
         }
     }
+    // the joining side: an item is joined once, at the first cut inside it
+    std::map<std::pair<int, int>, std::set<std::pair<int64_t, int>>> joined;
+    for (int64_t w = 1; w < W && w * share < total; ++w) {
+        const int seq = sequence_at(w * share);
+        const AttnCursor at = attn_seek(S, B, shift, seq, start[static_cast<size_t>(seq)], w * share);
+        if (at.start == w * share || at.start / share + 1 != w) continue;
+        AttnItem it;
+        attn_sequence(B, shift, at.seq, &it);
+        attn_tile(S, at.tile, &it);
+        auto& found = joined[{at.seq, at.tile}];
+        CHECK(found.empty());
+        for (int64_t v = at.start / share; v <= (at.start + it.steps - 1) / share; ++v) found.insert({v, v < w ? 1 : 0});
+    }
+    CHECK(joined == parts);
 }
 
 int main() {
     rows_and_pages();
     std::mt19937 rng(7);
+    sums(rng);
     for (int n = 0; n < 4000; ++n) {
-        const int G = 1 + static_cast<int>(rng() % 16);
-        const AttnSplit S{G, 16 << (rng() % 4), 32 << (rng() % 3)};
+        const int M = 16 << (rng() % 4), G = 1 + static_cast<int>(rng() % (M < 20 ? M : 20));
+        const AttnSplit S{G, M, 32 << (rng() % 3)};
         split(rng, 1 + static_cast<int>(rng() % 40), 1 + static_cast<int>(rng() % 50), 1 + static_cast<int>(rng() % 3000), S,
               1 + static_cast<int>(rng() % 300), n & 1);
     }
