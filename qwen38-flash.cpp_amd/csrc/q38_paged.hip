@@ -619,16 +619,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
     }
 }
 
-// ---- many queries per sequence. Tiles of M = 128 queries, 32 per wave, in equal shares as above;
+// ---- many queries per sequence. Tiles of 256 queries (128 of 256 dims) in equal shares as above;
 // keys and values go through LDS, TB tokens at a time and the next ones in flight (an 8-bit cache is converted on the way: its codes are exact in bf16), and
 // every wave multiplies them with its own 32 queries. Bound by the matrix cores, by the
 // exponentials beside them (8 per lane for 16 products of 128 dims) and by LDS reads, which 32
 // queries per wave bring to the matrix cores' own time.
 template <int D>
 struct TileGeo {
-    // 16-query groups per wave, waves and so 128 queries; 256 dims take the registers of two groups
-    static constexpr int MT = D == 256 ? 1 : 2, WAVES = D == 256 ? 8 : 4, M = 16 * MT * WAVES;
-    static constexpr int TB = D == 64 ? 64 : 32;
+    // One workgroup of two waves per SIMD fills a CU: two workgroups of one each share it unevenly (the
+    // older one's waves go first) and leave it half empty at the end, 588 us against 510 for a prompt
+    // batch. 16-query groups per wave: 256 dims take the registers of two.
+    static constexpr int MT = D == 256 ? 1 : 2, WAVES = 8, M = 16 * MT * WAVES;
+    static constexpr int TB = D == 256 ? 32 : 64;
     static constexpr int CH = D / 8;                       // 16-byte chunks of a bf16 row
     static constexpr int PIECES = TB * CH / (64 * WAVES);  // chunks per thread
     static constexpr size_t kLds = 2 * (2 * static_cast<size_t>(TB) * D * 2 + 2 * TB * 4);
@@ -671,9 +673,9 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     AttnState<D, Q8, MT> st;
     qt.load(q, qs, it, S, head, m0, negate, lane);
     st.clear(it, S, m0, lane);
-    // tokens that all, and any, of the wave's queries see
+    // tokens that all, and any, of the wave's queries see (a wave without queries has nothing to mask)
     const int r0 = tile_row(S, it, m0), rows_left = min(it.rows, (it.tile + 1) * S.rows());
-    const int all = r0 >= 0 ? attn_see(it, r0) : 0;
+    const int all = r0 >= 0 ? attn_see(it, r0) : 1 << 30;
     const int any = r0 >= 0 ? attn_see(it, min(it.tile * S.rows() + (m0 + 16 * MT - 1) / G, rows_left - 1)) : 0;
     const int from = __builtin_amdgcn_readfirstlane(sw.from) * (kSplitTokens / TB);
     const int stop = min(__builtin_amdgcn_readfirstlane(sw.to) * kSplitTokens, it.see);
@@ -929,7 +931,7 @@ hipError_t launch_paged_append(const PagedCacheDev& C, bool q8, const PagedBatch
 namespace {
 
 // Up to 32 queries per sequence and kv head the split kernel reads every token once; above, the tile
-// kernel does so once per 128.
+// kernel does so once per 128 or 256.
 struct AttnPlan {
     bool tiles, joined;
     int mt;  // split: 16-query groups
@@ -942,8 +944,8 @@ AttnPlan attn_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows,
     const int64_t queries = static_cast<int64_t>(max_rows) * G;
     p.tiles = queries > 32;
     p.mt = queries <= 16 ? 1 : 2;
-    p.M = p.tiles ? TileGeo<64>::M : 16 * p.mt;
-    p.W = std::max(1, 256 * (C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernels' occupancy
+    p.M = !p.tiles ? 16 * p.mt : C.d == 256 ? TileGeo<256>::M : TileGeo<128>::M;
+    p.W = std::max(1, 256 * (p.tiles || C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernels' occupancy
     // (no sequence is longer than a step, or a share holds its head's whole list: nothing is cut inside an item)
     p.joined = p.W > 1 && (static_cast<int64_t>(B.width) << C.shift) > kSplitTokens;
     return p;
