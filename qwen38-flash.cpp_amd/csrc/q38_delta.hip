@@ -217,6 +217,26 @@ __device__ __forceinline__ bool find_chunk(const DeltaBatchDev& B, int want, int
     }
     return false;
 }
+// The sequence that the slot-th group of workgroups takes. A walk is one chain per head, so the longest
+// sequences begin first; where all groups are on the chip at once, two workgroups per CU, those of the
+// second half join the first half's in the opposite order, the shortest beside the longest (eight ragged
+// prompts in their own order: 377 us, so: 285). Up to 64 sequences; more fill the chip in any order.
+__device__ __forceinline__ int nth_sequence(const DeltaBatchDev& B, int slot, int groups_per_round) {
+    if (B.seqs > 64 || B.seqs == 1) return slot;
+    const int lane = threadIdx.x & 63;
+    int length = -1;
+    if (lane < B.seqs) {
+        const RowSpan span = row_span(B.off, lane, B.rows);
+        length = span.end - span.begin;
+    }
+    int rank = 0;
+    for (int s = 0; s < B.seqs; ++s) {
+        const int other = __builtin_amdgcn_readlane(length, s);
+        rank += other > length || (other == length && s < lane);
+    }
+    if (B.seqs <= 2 * groups_per_round && slot >= groups_per_round) slot = B.seqs - 1 - (slot - groups_per_round);
+    return __builtin_ctzll(__ballot(lane < B.seqs && rank == slot));
+}
 // The sequence's first chunk in the list.
 __device__ __forceinline__ int first_chunk(const DeltaBatchDev& B, int seq) {
     int n = 0;
@@ -370,7 +390,8 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
     __shared__ uintx4 rows_lds[2][2][kChunk * CH];  // [buffer][keys, queries]
     const int lane = threadIdx.x & 63, u = lane & 15, w = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.y, s = blockIdx.z, hk = h / (D.hv / D.hk);
+    const int h = blockIdx.y, hk = h / (D.hv / D.hk);
+    const int s = nth_sequence(B, blockIdx.z, max(1, static_cast<int>(256 / (gridDim.x * gridDim.y))));
     const int dv = (blockIdx.x * NW + wave) * 16;  // the wave's first value dim
     const RowSpan span = row_span(B.off, s, B.rows);
     const int c0 = __builtin_amdgcn_readfirstlane(first_chunk(B, s));
@@ -497,7 +518,6 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
         for (int a = 0; a < 2; ++a) pr[a] = ot[a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
         constexpr int KB = KS < 4 ? KS : 4;  // dims whose operands are read together
         Parts<2> sp[KS];
-        uintx4 qb[KS][2];
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += KB) {
             uintx4 kb[KB][2];
@@ -505,10 +525,6 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             for (int k = 0; k < KB; ++k)
 #pragma unroll
                 for (int a = 0; a < 2; ++a) kb[k][a] = kt[key_at(chunk_row(u, a), KS * w + k0 + k)];
-#pragma unroll
-            for (int k = 0; k < KB; ++k)
-#pragma unroll
-                for (int a = 0; a < 2; ++a) qb[k0 + k][a] = qt[query_at(16 * a + u, KS * w + k0 + k)];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
@@ -524,6 +540,11 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
         }
         __builtin_amdgcn_sched_barrier(0);
         // the outputs' S q, transposed (value dims by chunk rows), beside Y = V - exp(G) P and its parts
+        uintx4 qb[KS][2];
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) qb[k][a] = qt[query_at(16 * a + u, KS * w + k)];
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -538,6 +559,8 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             yp.split(y);
         }
         __builtin_amdgcn_sched_barrier(0);
+        fetch_v(n + 1);
+        load_into(next);
         // U = T diag(beta) Y, beside K^T's operands and the state's decay
         uint32_t kv[8][E / 2];
 #pragma unroll
@@ -554,22 +577,17 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
                 }
             }
         }
-        floatx4 un[2];
+        // (chains of products that add to one result wait for each other: two or more take turns)
+        floatx4 un[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-            x = mfma(top[2][a], yp.p[0], x);
-            x = mfma(top[1][a], yp.p[1], x);
-            x = mfma(top[0][a], yp.p[2], x);
-            x = mfma(top[1][a], yp.p[0], x);
-            x = mfma(top[0][a], yp.p[1], x);
-            un[a] = mfma(top[0][a], yp.p[0], x);
-        }
+        for (int order = 2; order >= 0; --order)
+#pragma unroll
+            for (int i = 0; i <= order; ++i)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) un[a] = mfma(top[order - i][a], yp.p[i], un[a]);
 #pragma unroll
         for (int o = 0; o < E; ++o) st[o] *= whole;
         __builtin_amdgcn_sched_barrier(0);
-        fetch_v(n + 1);
-        load_into(next);
         load_t(next);
         // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U), beside the outputs' parts of U
         Parts<3> zp;
@@ -581,13 +599,17 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
         }
         load_left(next);
 #pragma unroll
-        for (int o = 0; o < E; ++o) {
-            uintx4 a;
+        for (int o = 0; o < E; o += 2) {
+            uintx4 a[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                a[j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], o & 1 ? 0x07060302u : 0x05040100u);
+            for (int j = 0; j < 4; ++j) {
+                a[0][j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], 0x05040100u);
+                a[1][j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], 0x07060302u);
+            }
 #pragma unroll
-            for (int p = 2; p >= 0; --p) st[o] = mfma(a, zp.p[p], st[o]);
+            for (int p = 2; p >= 0; --p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) st[o + i] = mfma(a[i], zp.p[p], st[o + i]);
         }
         Parts<2> up;
         {
@@ -598,12 +620,11 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
         }
         // O^T = exp(G) S q + U^T M^T
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            ot[a] *= eg[a];
-            ot[a] = mfma(up.p[0], mop[1][a], ot[a]);
-            ot[a] = mfma(up.p[1], mop[0][a], ot[a]);
-            ot[a] = mfma(up.p[0], mop[0][a], ot[a]);
-        }
+        for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[0], mop[1][a], ot[a] * eg[a]);
+#pragma unroll
+        for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[p], mop[0][a], ot[a]);
         __builtin_amdgcn_sched_barrier(0);
         load_m(next);
         stage((n + 1) & 1);

@@ -505,6 +505,15 @@ struct ShareWalk {
     __device__ __forceinline__ int seq() const { return __builtin_amdgcn_readfirstlane(seq_); }
     int seq_;
 };
+// What a share leaves for the join: the item that goes on behind it, if it began in it, and the
+// number of its pieces (0: none).
+struct alignas(32) CutItem {
+    int pieces, first, rows, tokens, tile, bad;
+};
+__device__ __forceinline__ void note_cut(CutItem* cut, const ShareWalk& sw, const AttnItem& it) {
+    *cut = CutItem{static_cast<int>((sw.start + it.steps - 1) / sw.share - sw.start / sw.share) + 1, it.first, it.rows,
+                   it.tokens, it.tile, it.bad};
+}
 
 // A workgroup's share of a kv head's steps; wave i takes tokens 32 i .. 32 i + 31 of every step, the
 // next step's keys and values in flight, and the waves' sums are joined through LDS at the end of
@@ -513,7 +522,8 @@ template <int D, bool Q8, int MT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCacheDev C, PagedBatchDev B, int G,
                                                                            const uint16_t* __restrict__ q, int64_t qs,
                                                                            float c, uint16_t* __restrict__ out, int64_t os,
-                                                                           float* __restrict__ part) {
+                                                                           float* __restrict__ part,
+                                                                           CutItem* __restrict__ cuts) {
     using Geo = AttnGeo<D, Q8>;
     constexpr int M = 16 * MT, LR = D + 4;  // (rows of the waves' sums padded: 16 bytes move the banks)
     extern __shared__ float lds[];          // [waves][M][LR], then [waves][M] maxima and sums
@@ -523,6 +533,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __shared__ ShareWalk walks[kSplitWaves];
     ShareWalk& sw = walks[wave];
+    CutItem* const cut = cuts + head * W + w;
+    if (threadIdx.x == 0) cut->pieces = 0;
     if (!sw.open(S, B, C.shift, w, W)) return;
     while (sw.next(S, B, C.shift)) {
         // (opaque: what follows from the lane is formed anew per piece, not kept in registers for the next)
@@ -587,7 +599,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         const int from = sw.from;
         const bool whole = sw.to - from == it.steps;
         float* pd = nullptr;
-        if (!whole) pd = part + ((static_cast<int64_t>(head) * W + w) * 2 + attn_slot(sw.start, sw.share, w)) * (M * (D + 2));
+        if (!whole) {
+            const int slot = attn_slot(sw.start, sw.share, w);
+            pd = part + ((static_cast<int64_t>(head) * W + w) * 2 + slot) * (M * (D + 2));
+            if (slot && threadIdx.x == 0) note_cut(cut, sw, it);
+        }
         for (int e = threadIdx.x; e < M * D / 4; e += 256) {
             const int i = e / (D / 4), d = e % (D / 4) * 4, row = tile_row(S, it, i);
             if (row < 0) continue;
@@ -645,7 +661,7 @@ __device__ __forceinline__ int tile_at(int token, int chunk) {
 template <int D, bool Q8>
 __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     PagedCacheDev C, PagedBatchDev B, int G, int shares, const uint16_t* __restrict__ q, int64_t qs, float c,
-    uint16_t* __restrict__ out, int64_t os, float* __restrict__ part) {
+    uint16_t* __restrict__ out, int64_t os, float* __restrict__ part, CutItem* __restrict__ cuts) {
     using Geo = AttnGeo<D, false>;
     using TG = TileGeo<D>;
     constexpr int TB = TG::TB, NT = 64 * TG::WAVES, CH = TG::CH, PC = TG::PIECES, MT = TG::MT;
@@ -662,6 +678,8 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     c = fabsf(c);
     __shared__ ShareWalk walks[TG::WAVES];
     ShareWalk& sw = walks[wave];
+    CutItem* const cut = cuts + n;
+    if (threadIdx.x == 0) cut->pieces = 0;
     if (!sw.open(S, B, C.shift, place, shares)) return;
     while (sw.next(S, B, C.shift)) {
     // (opaque: what follows from the lane is formed anew per piece, not kept in registers for the next)
@@ -813,8 +831,11 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     it = sw.item(S);
     const bool whole = sw.to - sw.from == it.steps;
     float* pd = nullptr;
-    if (!whole)
-        pd = part + ((static_cast<int64_t>(head) * shares + place) * 2 + attn_slot(sw.start, sw.share, place)) * (TG::M * (D + 2));
+    if (!whole) {
+        const int slot = attn_slot(sw.start, sw.share, place);
+        pd = part + (static_cast<int64_t>(n) * 2 + slot) * (TG::M * (D + 2));
+        if (slot && threadIdx.x == 0) note_cut(cut, sw, it);
+    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         float sum = st.total(m);
@@ -859,25 +880,27 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     }
 }
 
-// Joins the pieces of the items that the shares' ends cut: a workgroup per (cut, kv head, QB of the
-// tile's queries), a wave per query, PB pieces in flight; an item's first cut does the work.
+// Joins the pieces of the items that the shares' ends cut: a workgroup per (share that an item goes on
+// from, kv head, QB of the tile's queries), a wave per query, PB pieces in flight.
 template <int D, int QB, int PB>
-__global__ __launch_bounds__(256) void k_paged_join(PagedCacheDev C, PagedBatchDev B, AttnSplit S, int W,
-                                                    const float* __restrict__ part, uint16_t* __restrict__ out, int64_t os) {
+__global__ __launch_bounds__(256) void k_paged_join(AttnSplit S, int W, const float* __restrict__ part,
+                                                    const CutItem* __restrict__ cuts, uint16_t* __restrict__ out,
+                                                    int64_t os) {
     constexpr int E = D / 64;
     typedef float vec_t __attribute__((ext_vector_type(E)));
     const int lane = threadIdx.x & 63, head = blockIdx.y, G = S.G, M = S.M;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    AttnCursor at{0, 0, 0};
-    int64_t share = 0;
-    const int64_t cut = blockIdx.x + 1, total = find_share(S, B, C.shift, cut, W, &at, &share);
-    if (cut * share >= total || at.start == cut * share || at.start / share + 1 != cut) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), place = head * W + blockIdx.x;
+    const CutItem cut = cuts[place];
+    const int n = __builtin_amdgcn_readfirstlane(cut.pieces);
+    if (n == 0) return;
     AttnItem it;
-    attn_sequence(B, C.shift, at.seq, &it);
-    attn_tile(S, at.tile, &it);
-    const int n = static_cast<int>((at.start + it.steps - 1) / share - at.start / share) + 1;
-    // (an item goes on behind its first share, whose second slot it takes; it began before the others)
-    const float* first = part + ((static_cast<int64_t>(head) * W + cut - 1) * 2 + 1) * (M * (D + 2));
+    it.first = __builtin_amdgcn_readfirstlane(cut.first);
+    it.rows = __builtin_amdgcn_readfirstlane(cut.rows);
+    it.tokens = __builtin_amdgcn_readfirstlane(cut.tokens);
+    it.tile = __builtin_amdgcn_readfirstlane(cut.tile);
+    it.bad = __builtin_amdgcn_readfirstlane(cut.bad);
+    // (it is the second slot of its first share and the first of the others)
+    const float* first = part + (static_cast<int64_t>(place) * 2 + 1) * (M * (D + 2));
     auto piece = [&](int i) { return first + static_cast<int64_t>(2 * i - (i > 0)) * (M * (D + 2)); };
 #pragma unroll 2
     for (int j = wave; j < QB; j += 4) {
@@ -953,45 +976,49 @@ AttnPlan attn_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows,
 
 template <int D, bool Q8, int MT>
 hipError_t launch_split(const PagedCacheDev& C, const PagedBatchDev& B, const AttnPlan& p, const uint16_t* q, int64_t qs,
-                        int hq, float c, uint16_t* out, int64_t os, float* part, hipStream_t st) {
+                        int hq, float c, uint16_t* out, int64_t os, float* part, CutItem* cuts, hipStream_t st) {
     constexpr size_t lds = (static_cast<size_t>(kSplitWaves) * 16 * MT * (D + 4) + 2 * kSplitWaves * 16 * MT) * 4;
     const hipError_t e = ensure_lds<k_paged_split<D, Q8, MT>>(lds);
     if (e != hipSuccess) return e;
-    return launch(k_paged_split<D, Q8, MT>, dim3(p.W, C.hkv), dim3(256), lds, st, C, B, hq / C.hkv, q, qs, c, out, os, part);
+    return launch(k_paged_split<D, Q8, MT>, dim3(p.W, C.hkv), dim3(256), lds, st, C, B, hq / C.hkv, q, qs, c, out, os, part,
+                  cuts);
 }
 template <int D, bool Q8>
 hipError_t launch_attention(const PagedCacheDev& C, const PagedBatchDev& B, const AttnPlan& p, const uint16_t* q, int64_t qs,
-                            int hq, float scale, uint16_t* out, int64_t os, float* part, hipStream_t st) {
+                            int hq, float scale, uint16_t* out, int64_t os, void* ws, hipStream_t st) {
     const float c = scale * 1.44269504088896341f;  // exponents of 2
+    CutItem* const cuts = static_cast<CutItem*>(ws);
+    float* const part = reinterpret_cast<float*>(cuts + static_cast<size_t>(C.hkv) * p.W);
     hipError_t e;
     if (!p.tiles) {
-        e = p.mt == 1 ? launch_split<D, Q8, 1>(C, B, p, q, qs, hq, c, out, os, part, st)
-                      : launch_split<D, Q8, 2>(C, B, p, q, qs, hq, c, out, os, part, st);
+        e = p.mt == 1 ? launch_split<D, Q8, 1>(C, B, p, q, qs, hq, c, out, os, part, cuts, st)
+                      : launch_split<D, Q8, 2>(C, B, p, q, qs, hq, c, out, os, part, cuts, st);
     } else {
         e = ensure_lds<k_paged_tile<D, Q8>>(TileGeo<D>::kLds);
         if (e == hipSuccess)
             e = launch(k_paged_tile<D, Q8>, dim3((p.W * C.hkv + 7) / 8 * 8), dim3(64 * TileGeo<D>::WAVES), TileGeo<D>::kLds,
-                       st, C, B, hq / C.hkv, p.W, q, qs, c, out, os, part);
+                       st, C, B, hq / C.hkv, p.W, q, qs, c, out, os, part, cuts);
     }
     if (e != hipSuccess || !p.joined) return e;
     const AttnSplit S{hq / C.hkv, p.M, kSplitTokens};
     if (p.tiles)
-        return launch(k_paged_join<D, 32, 2>, dim3(p.W - 1, C.hkv, p.M / 32), dim3(256), 0, st, C, B, S, p.W, part, out, os);
-    return launch(k_paged_join<D, 4, 8>, dim3(p.W - 1, C.hkv, p.M / 4), dim3(256), 0, st, C, B, S, p.W, part, out, os);
+        return launch(k_paged_join<D, 32, 2>, dim3(p.W - 1, C.hkv, p.M / 32), dim3(256), 0, st, S, p.W, part, cuts,
+                      out, os);
+    return launch(k_paged_join<D, 4, 16>, dim3(p.W - 1, C.hkv, p.M / 4), dim3(256), 0, st, S, p.W, part, cuts, out, os);
 }
 
 } // namespace
 
 size_t paged_attention_ws(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows, int hq) {
     const AttnPlan p = attn_plan(C, B, max_rows, hq);
-    const size_t pieces = static_cast<size_t>(C.hkv) * p.W * 2;
-    return p.joined ? pieces * p.M * (C.d + 2) * 4 : 0;
+    const size_t shares = static_cast<size_t>(C.hkv) * p.W;
+    return shares * sizeof(CutItem) + (p.joined ? shares * 2 * p.M * (C.d + 2) * 4 : 0);
 }
 
 hipError_t launch_paged_attention(const PagedCacheDev& C, bool q8, const PagedBatchDev& B, int max_rows, const uint16_t* q,
                                   int64_t qs, int hq, float scale, uint16_t* out, int64_t os, void* ws, hipStream_t st) {
     const AttnPlan p = attn_plan(C, B, max_rows, hq);
-    auto go = [&](auto kern) { return kern(C, B, p, q, qs, hq, scale, out, os, static_cast<float*>(ws), st); };
+    auto go = [&](auto kern) { return kern(C, B, p, q, qs, hq, scale, out, os, ws, st); };
     if (q8)
         return C.d == 64    ? go(launch_attention<64, true>)
                : C.d == 128 ? go(launch_attention<128, true>)
