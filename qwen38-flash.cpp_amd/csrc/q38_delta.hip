@@ -377,28 +377,146 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
     }
 }
 
-// A wave holds 16 value columns of a head's state, transposed: S^T tile o (o < E = DK / 16) has
-// key dim E (4 w + r) + o in its result row 4 w + r and the value dim in its column. Lane (u, w) thus
-// holds key dims 4 E w .. 4 E (w + 1) - 1 of value dim u, eight of them in a row being an operand of
-// S k and S q with keys and queries read as stored, and the update's operand, K^T, is formed from 16-byte
-// runs of eight keys by byte permutes. No value moves between lanes, and waves share nothing but
-// the keys and queries in LDS.
-template <int DK, int NW>
-__global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(DeltaDev D, DeltaBatchDev B,
-                                                          const ChunkSystem* __restrict__ sys, int bound) {
-    constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8, NT = 64 * NW, PC = kChunk * CH / NT;
-    __shared__ uintx4 rows_lds[2][2][kChunk * CH];  // [buffer][keys, queries]
+// The walk. A state wave holds 16 value columns of a head's state, transposed: S^T tile o (o < E =
+// DK / 16) has key dim E (4 w + r) + o in its result row 4 w + r and the value dim in its column. Lane
+// (u, w) thus holds key dims 4 E w .. 4 E (w + 1) - 1 of value dim u, eight of them in a row being an
+// operand of S k and S q with keys and queries read as stored, and the update's operand, K^T, is formed
+// from 16-byte runs of eight keys by byte permutes: no value moves between lanes. A sequence is one chain
+// of chunks per head, and a wave issues an instruction every four cycles at best, so what the chain does
+// not need is left to a second wave on another SIMD: an output wave per state wave takes the operands
+// of S and U through LDS a chunk later, and loads and stages the keys (one wave doing all: 240 us for
+// a prompt of 4,001 rows, 1.9 us a chunk).
+template <int DK>
+struct WalkGeo {
+    static constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8;
+    static constexpr int NW = 2;                              // state waves of a workgroup, and output waves
+    static constexpr int PC = kChunk * CH / (64 * NW);        // 16-byte pieces of the keys per output thread
+    static constexpr int kKeys = kChunk * CH, kParts = NW * KS * 2 * 64, kUpd = NW * 2 * 64;
+    static constexpr size_t kLds = 2 * 16 * static_cast<size_t>(kKeys + kParts + kUpd);
+};
+
+template <int DK>
+__global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(DeltaDev D, DeltaBatchDev B,
+                                                                           const ChunkSystem* __restrict__ sys, int bound) {
+    using Geo = WalkGeo<DK>;
+    constexpr int E = Geo::E, KS = Geo::KS, CH = Geo::CH, NW = Geo::NW, PC = Geo::PC, KB = KS < 4 ? KS : 4;
+    extern __shared__ uintx4 walk_lds[];  // [2] of: keys, the state's parts, U
+    uintx4* const keys_lds = walk_lds;
+    uintx4* const parts_lds = walk_lds + 2 * Geo::kKeys;
+    floatx4* const upd_lds = reinterpret_cast<floatx4*>(walk_lds + 2 * (Geo::kKeys + Geo::kParts));
     const int lane = threadIdx.x & 63, u = lane & 15, w = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.y, hk = h / (D.hv / D.hk);
-    const int s = nth_sequence(B, blockIdx.z, max(1, static_cast<int>(256 / (gridDim.x * gridDim.y))));
-    const int dv = (blockIdx.x * NW + wave) * 16;  // the wave's first value dim
+    const int pair = wave % NW;
+    const bool outputs = wave >= NW;
+    // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: those of one head, which read the
+    // same chunk systems, keys and queries, are one XCD's (apart from each other they were bound by what
+    // their L2s fetched, 371 us for eight ragged prompts).
+    const int groups = D.dv / (16 * NW), turn = blockIdx.x / 8, chain = turn / groups * 8 + blockIdx.x % 8;
+    if (chain >= D.hv * B.seqs) return;
+    const int h = chain % D.hv, hk = h / (D.hv / D.hk);
+    const int s = nth_sequence(B, chain / D.hv, max(1, 256 / (groups * D.hv)));
+    const int dv = (turn % groups * NW + pair) * 16;  // the wave's first value dim
     const RowSpan span = row_span(B.off, s, B.rows);
+    const int length = __builtin_amdgcn_readfirstlane(span.end - span.begin), begin = __builtin_amdgcn_readfirstlane(span.begin);
     const int c0 = __builtin_amdgcn_readfirstlane(first_chunk(B, s));
     // (offsets that do not ascend could name more chunks than the workspace holds)
-    const int chunks = min((span.end - span.begin + kChunk - 1) / kChunk, bound - c0);
+    const int chunks = max(0, min((length + kChunk - 1) / kChunk, bound - c0));
+    const ChunkSystem* const sys0 = sys + static_cast<size_t>(c0) * D.hv + h;
+    auto system = [&](int n) -> const ChunkSystem& { return sys0[static_cast<size_t>(min(n, chunks - 1)) * D.hv]; };
+    // keys: swizzled for reads down chunk_row()'s rows
+    auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
+    // Loads of a next chunk are made always, of the last one's again behind it, and their number is the same
+    // on every path, so that a wait counts only the loads that it needs. Rows behind the sequence: its last
+    // row again, whose update is nothing (its beta in the system is 0).
+
+    if (outputs) {
+        const char* const kb = reinterpret_cast<const char*>(D.k + begin * D.ks + hk * DK);
+        const char* const qb = reinterpret_cast<const char*>(D.q + begin * D.qs + hk * DK);
+        char* const ob = reinterpret_cast<char*>(D.out + (static_cast<size_t>(begin) * D.hv + h) * D.dv + dv);
+        const int tid = pair * 64 + lane;
+        uintx4 kr[PC], qr[KS][2], mop[2][2];
+        float eg[2];
+        auto fetch_keys = [&](int chunk) {
+#pragma unroll
+            for (int i = 0; i < PC; ++i) {
+                const int64_t row = min(chunk * kChunk + tid / CH + i * (64 * NW / CH), length - 1);
+                kr[i] = *reinterpret_cast<const uintx4*>(kb + 2 * row * D.ks + 16 * (tid % CH));
+            }
+        };
+        auto stage_keys = [&](int buf) {
+#pragma unroll
+            for (int i = 0; i < PC; ++i) keys_lds[buf * Geo::kKeys + key_at(tid / CH + i * (64 * NW / CH), tid % CH)] = kr[i];
+        };
+        auto fetch_queries = [&](int chunk) {  // operands: row 16 a + u, dims 4 E w + 8 k ..
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const int64_t row = min(chunk * kChunk + 16 * a + u, length - 1);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    qr[k][a] = *reinterpret_cast<const uintx4*>(qb + 2 * row * D.qs + 16 * (KS * w + k));
+            }
+        };
+        auto fetch_scores = [&](const ChunkSystem& cs) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p) mop[p][a] = cs.m[p][a][lane];
+                eg[a] = cs.into[16 * a + u];
+            }
+        };
+        if (chunks > 0) {
+            fetch_keys(0);
+            fetch_queries(0);
+            fetch_scores(system(0));
+            stage_keys(0);
+        }
+        lds_barrier();
+        for (int n = 0; n <= chunks && chunks > 0; ++n) {  // the keys of chunk n + 1, the outputs of chunk n - 1
+            fetch_keys(min(n + 1, chunks - 1));
+            if (n > 0) {
+                const uintx4* parts = parts_lds + ((n - 1) & 1) * Geo::kParts + pair * KS * 2 * 64 + lane;
+                const floatx4* upd = upd_lds + ((n - 1) & 1) * Geo::kUpd + pair * 2 * 64 + lane;
+                // O^T = exp(G) S q + U^T M^T, transposed: value dims by chunk rows
+                floatx4 ot[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int p = 1; p >= 0; --p)
+#pragma unroll
+                        for (int a = 0; a < 2; ++a) ot[a] = mfma(parts[(k * 2 + p) * 64], qr[k][a], ot[a]);
+                const floatx4 un[2] = {upd[0], upd[64]};
+                Parts<2> up;
+                {
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = un[j >> 2][j & 3];
+                    up.split(x);
+                }
+#pragma unroll
+                for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[0], mop[1][a], ot[a] * eg[a]);
+#pragma unroll
+                for (int p = 1; p >= 0; --p)
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[p], mop[0][a], ot[a]);
+                fetch_queries(n);
+                fetch_scores(system(n));
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    ot[a] *= D.scale;
+                    const int row = (n - 1) * kChunk + 16 * a + u;
+                    if (row < length)
+                        *reinterpret_cast<uint2*>(ob + 2 * (static_cast<int64_t>(row) * D.hv * D.dv + 4 * w)) =
+                            make_uint2(pack_bf16(ot[a][0], ot[a][1]), pack_bf16(ot[a][2], ot[a][3]));
+                }
+            }
+            stage_keys((n + 1) & 1);
+            lds_barrier();  // (the next chunk's loads stay in flight)
+        }
+        return;
+    }
+
     const size_t elems = static_cast<size_t>(D.hv) * D.dv * DK;
-    const int from = B.origin ? B.origin[s] : -1;
+    const int from = B.origin ? uniform_load(B.origin + s) : -1;
     floatx4 st[E];
     auto state_at = [&](int slot, int r) {  // E consecutive key dims
         return B.states + slot * elems + (static_cast<size_t>(h) * D.dv + dv + u) * DK + E * (4 * w + r);
@@ -413,79 +531,31 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
 #pragma unroll
             for (int e = 0; e < 4; ++e) st[o + e][r] = x[e];
         }
-    // keys: swizzled for reads down chunk_row()'s rows; queries: for reads down consecutive rows
-    auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
-    auto query_at = [](int row, int ch) { return row * CH + (ch ^ (row & 7)); };
-    // The next chunk's loads are made always and their number is the same on every path, so that a wait
-    // counts only the loads that it needs: a whole chunk's by uniform addresses and a lane's offset,
-    // the others' rows clamped to the sequence's last (a repeated row's update is nothing: its beta in
-    // the system is 0).
-    const uint32_t ko = 2 * ((threadIdx.x / CH) * static_cast<uint32_t>(D.ks) + 8 * (threadIdx.x % CH));
-    const uint32_t qo = 2 * ((threadIdx.x / CH) * static_cast<uint32_t>(D.qs) + 8 * (threadIdx.x % CH));
+    const char* const vb = reinterpret_cast<const char*>(D.v + begin * D.vs + h * D.dv + dv);
     const uint32_t vo = 2 * (8 * w * static_cast<uint32_t>(D.vs) + u);
-    const char* const kb0 = reinterpret_cast<const char*>(D.k + span.begin * D.ks + hk * DK);
-    const char* const qb0 = reinterpret_cast<const char*>(D.q + span.begin * D.qs + hk * DK);
-    const char* const vb0 = reinterpret_cast<const char*>(D.v + span.begin * D.vs + h * D.dv + dv);
-    uintx4 kr[PC], qr[PC];
-    const int length = span.end - span.begin;
-    auto fetch = [&](int chunk) {
-        if ((chunk + 1) * kChunk <= length) {
-#pragma unroll
-            for (int i = 0; i < PC; ++i) {
-                const int64_t row = chunk * kChunk + i * (NT / CH);
-                kr[i] = *reinterpret_cast<const uintx4*>(kb0 + 2 * row * D.ks + ko);
-                qr[i] = *reinterpret_cast<const uintx4*>(qb0 + 2 * row * D.qs + qo);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PC; ++i) {
-                const int64_t row = min(chunk * kChunk + static_cast<int>(threadIdx.x) / CH + i * (NT / CH), length - 1);
-                kr[i] = *reinterpret_cast<const uintx4*>(kb0 + 2 * row * D.ks + 16 * (threadIdx.x % CH));
-                qr[i] = *reinterpret_cast<const uintx4*>(qb0 + 2 * row * D.qs + 16 * (threadIdx.x % CH));
-            }
-        }
-    };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < PC; ++i) {
-            const int piece = threadIdx.x + i * NT;
-            rows_lds[buf][0][key_at(piece / CH, piece % CH)] = kr[i];
-            rows_lds[buf][1][query_at(piece / CH, piece % CH)] = qr[i];
-        }
-    };
     uint16_t vr[8];
     auto fetch_v = [&](int chunk) {
         if ((chunk + 1) * kChunk <= length) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                vr[j] = *reinterpret_cast<const uint16_t*>(vb0 + 2 * static_cast<int64_t>(chunk * kChunk + j) * D.vs + vo);
+                vr[j] = *reinterpret_cast<const uint16_t*>(vb + 2 * static_cast<int64_t>(chunk * kChunk + j) * D.vs + vo);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int64_t row = min(chunk * kChunk + 8 * w + j, length - 1);
-                vr[j] = *reinterpret_cast<const uint16_t*>(vb0 + 2 * row * D.vs + 2 * u);
+                vr[j] = *reinterpret_cast<const uint16_t*>(vb + 2 * row * D.vs + 2 * u);
             }
         }
     };
-    char* const ob0 = reinterpret_cast<char*>(D.out + (static_cast<size_t>(span.begin) * D.hv + h) * D.dv + dv);
-    const uint32_t oo = 2 * (static_cast<uint32_t>(u) * D.hv * D.dv + 4 * w);
     // a chunk's system in registers, every part loaded anew as soon as its chunk is done with it
-    uintx4 top[3][2], mop[2][2];
+    uintx4 top[3][2];
     floatx4 into[2], left[2];
-    float eg[2], whole = 1.0f;
+    float whole = 1.0f;
     auto load_t = [&](const ChunkSystem& cs) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int p = 0; p < 3; ++p) top[p][a] = cs.t[p][a][lane];
-    };
-    auto load_m = [&](const ChunkSystem& cs) {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-#pragma unroll
-            for (int p = 0; p < 2; ++p) mop[p][a] = cs.m[p][a][lane];
-            eg[a] = cs.into[16 * a + u];
-        }
     };
     auto load_into = [&](const ChunkSystem& cs) {
 #pragma unroll
@@ -497,27 +567,19 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
         whole = cs.into[kChunk - 1];
     };
     if (chunks > 0) {
-        const ChunkSystem& cs = sys[static_cast<size_t>(c0) * D.hv + h];
-        fetch(0);
         fetch_v(0);
-        load_into(cs);
-        load_t(cs);
-        load_m(cs);
-        load_left(cs);
-        stage(0);
+        load_into(system(0));
+        load_t(system(0));
+        load_left(system(0));
     }
-    __syncthreads();
+    lds_barrier();
     for (int n = 0; n < chunks; ++n) {
-        const uintx4* kt = rows_lds[n & 1][0];
-        const uintx4* qt = rows_lds[n & 1][1];
-        const ChunkSystem& next = sys[static_cast<size_t>(c0 + min(n + 1, chunks - 1)) * D.hv + h];
-        fetch(n + 1);
+        const uintx4* kt = keys_lds + (n & 1) * Geo::kKeys;
+        uintx4* parts = parts_lds + (n & 1) * Geo::kParts + pair * KS * 2 * 64 + lane;
+        floatx4* upd = upd_lds + (n & 1) * Geo::kUpd + pair * 2 * 64 + lane;
+        const ChunkSystem& next = system(n + 1);
         // P = K S^T (chunk rows by value dims)
-        floatx4 pr[2], ot[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a) pr[a] = ot[a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-        constexpr int KB = KS < 4 ? KS : 4;  // dims whose operands are read together
-        Parts<2> sp[KS];
+        floatx4 pr[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += KB) {
             uintx4 kb[KB][2];
@@ -525,43 +587,24 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             for (int k = 0; k < KB; ++k)
 #pragma unroll
                 for (int a = 0; a < 2; ++a) kb[k][a] = kt[key_at(chunk_row(u, a), KS * w + k0 + k)];
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);  // (all reads in flight before the first product)
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = st[(8 * (k0 + k) + j) % E][(8 * (k0 + k) + j) / E];
-                sp[k0 + k].split(x);
+                Parts<2> sp;
+                sp.split(x);
 #pragma unroll
-                for (int p = 1; p >= 0; --p)
+                for (int p = 1; p >= 0; --p) {
+                    parts[((k0 + k) * 2 + p) * 64] = sp.p[p];
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) pr[a] = mfma(kb[k][a], sp[k0 + k].p[p], pr[a]);
+                    for (int a = 0; a < 2; ++a) pr[a] = mfma(kb[k][a], sp.p[p], pr[a]);
+                }
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        // the outputs' S q, transposed (value dims by chunk rows), beside Y = V - exp(G) P and its parts
-        uintx4 qb[KS][2];
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) qb[k][a] = qt[query_at(16 * a + u, KS * w + k)];
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int p = 1; p >= 0; --p)
-#pragma unroll
-                for (int a = 0; a < 2; ++a) ot[a] = mfma(sp[k].p[p], qb[k][a], ot[a]);
-        Parts<3> yp;
-        {
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = bf2f(vr[j]) - into[j >> 2][j & 3] * pr[j >> 2][j & 3];
-            yp.split(y);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        fetch_v(n + 1);
-        load_into(next);
-        // U = T diag(beta) Y, beside K^T's operands and the state's decay
+        // K^T's rows and the state's decay, beside the products' end
         uint32_t kv[8][E / 2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -577,7 +620,19 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
                 }
             }
         }
-        // (chains of products that add to one result wait for each other: two or more take turns)
+#pragma unroll
+        for (int o = 0; o < E; ++o) st[o] *= whole;
+        // U = T diag(beta) Y, Y = V - exp(G) P (chains of products that add to one result wait for each
+        // other: two or more take turns)
+        Parts<3> yp;
+        {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = bf2f(vr[j]) - into[j >> 2][j & 3] * pr[j >> 2][j & 3];
+            yp.split(y);
+        }
+        fetch_v(n + 1);
+        load_into(next);
         floatx4 un[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int order = 2; order >= 0; --order)
@@ -585,11 +640,8 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             for (int i = 0; i <= order; ++i)
 #pragma unroll
                 for (int a = 0; a < 2; ++a) un[a] = mfma(top[order - i][a], yp.p[i], un[a]);
-#pragma unroll
-        for (int o = 0; o < E; ++o) st[o] *= whole;
-        __builtin_amdgcn_sched_barrier(0);
         load_t(next);
-        // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U), beside the outputs' parts of U
+        // S^T = exp(G_C) S^T + K^T (exp(G_C - G) U)
         Parts<3> zp;
         {
             float z[8];
@@ -597,6 +649,8 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
             for (int j = 0; j < 8; ++j) z[j] = left[j >> 2][j & 3] * un[j >> 2][j & 3];
             zp.split(z);
         }
+        upd[0] = un[0];
+        upd[64] = un[1];
         load_left(next);
 #pragma unroll
         for (int o = 0; o < E; o += 2) {
@@ -611,42 +665,10 @@ __global__ __launch_bounds__(64 * NW, DK == 256 ? 1 : 2) void k_delta_chunks(Del
 #pragma unroll
                 for (int i = 0; i < 2; ++i) st[o + i] = mfma(a[i], zp.p[p], st[o + i]);
         }
-        Parts<2> up;
-        {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = un[j >> 2][j & 3];
-            up.split(x);
-        }
-        // O^T = exp(G) S q + U^T M^T
-#pragma unroll
-        for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[0], mop[1][a], ot[a] * eg[a]);
-#pragma unroll
-        for (int p = 1; p >= 0; --p)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[p], mop[0][a], ot[a]);
-        __builtin_amdgcn_sched_barrier(0);
-        load_m(next);
-        stage((n + 1) & 1);
-        uint2 ov[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            ot[a] *= D.scale;
-            ov[a] = make_uint2(pack_bf16(ot[a][0], ot[a][1]), pack_bf16(ot[a][2], ot[a][3]));
-        }
-        char* const ob = ob0 + static_cast<int64_t>(n) * kChunk * D.hv * D.dv * 2;
-        const uint32_t tile = 32u * D.hv * D.dv;  // bytes of 16 rows
-        if ((n + 1) * kChunk <= length) {
-#pragma unroll
-            for (int a = 0; a < 2; ++a) *reinterpret_cast<uint2*>(ob + a * tile + oo) = ov[a];
-        } else {
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-                if (n * kChunk + 16 * a + u < length) *reinterpret_cast<uint2*>(ob + a * tile + oo) = ov[a];
-        }
         lds_barrier();  // (the next chunk's loads stay in flight)
     }
-    const int to = B.last ? B.last[s] : -1;
+    if (chunks > 0) lds_barrier();  // the output waves' last chunk
+    const int to = B.last ? uniform_load(B.last + s) : -1;
     if (to < 0 || to >= B.slots) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -666,7 +688,9 @@ hipError_t launch_chunks(const DeltaDev& D, const DeltaBatchDev& B, ChunkSystem*
     const int bound = chunk_bound(B);
     const hipError_t e = launch(k_delta_system<DK>, dim3(bound, D.hv), dim3(64), 0, st, D, B, sys);
     if (e != hipSuccess) return e;
-    return launch(k_delta_chunks<DK, 4>, dim3(D.dv / 64, D.hv, B.seqs), dim3(256), 0, st, D, B,
+    using Geo = WalkGeo<DK>;
+    if (const hipError_t l = ensure_lds<k_delta_chunks<DK>>(Geo::kLds); l != hipSuccess) return l;
+    return launch(k_delta_chunks<DK>, dim3(D.dv / (16 * Geo::NW) * ((D.hv * B.seqs + 7) / 8 * 8)), dim3(128 * Geo::NW), Geo::kLds, st, D, B,
                   static_cast<const ChunkSystem*>(sys), bound);
 }
 
