@@ -248,27 +248,33 @@ __device__ __forceinline__ int first_chunk(const DeltaBatchDev& B, int seq) {
     return n;
 }
 
-// One wave per (chunk, value head).
-template <int DK>
+// One wave per chunk and value head, or two value heads of one key head (N = 2): their products are the
+// same, and the substitution of one head's diagonal blocks fills half a wave. Bound by the latency of its
+// dependent steps (a head per wave: 86 us for 16,384 chunk heads, 1.9 TB/s of systems written).
+template <int DK, int N>
 __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B, ChunkSystem* __restrict__ sys) {
     constexpr int KS = DK / 32, LD = kChunk + 4;
-    __shared__ __align__(16) float As[kChunk][LD], Ts[kChunk][LD], Ws[16][20];
-    __shared__ double Gs[kChunk];
-    __shared__ float Bs[kChunk];
-    const int h = blockIdx.y, lane = threadIdx.x, u = lane & 15, w = lane >> 4, hk = h / (D.hv / D.hk);
+    __shared__ __align__(16) float As[N][kChunk][LD], Ts[N][kChunk][LD];
+    __shared__ double Gs[N][kChunk];
+    __shared__ float Bs[N][kChunk];
+    const int h0 = blockIdx.y * N, lane = threadIdx.x, u = lane & 15, w = lane >> 4, hk = h0 / (D.hv / D.hk);
     int r0 = 0, n = 0;
     if (!find_chunk(B, blockIdx.x, &r0, &n)) return;
-    // the decay sums, in double: differences of far sums must keep a weak decay's digits
-    const bool mine = lane < n;
-    const float g = mine ? D.g[static_cast<size_t>(r0 + lane) * D.hv + h] : 0.0f;
-    double G = g < kFloor ? kFloor : g;
-    for (int d = 1; d < kChunk; d <<= 1) {
-        const double x = __shfl_up(G, d);
-        if (lane >= d) G += x;
-    }
-    if (lane < kChunk) {
-        Gs[lane] = G;
-        Bs[lane] = mine ? D.beta[static_cast<size_t>(r0 + lane) * D.hv + h] : 0.0f;
+    // the decay sums, in double: differences of far sums must keep a weak decay's digits (lanes 32 e .. of head e)
+    {
+        const int e = N == 2 ? lane >> 5 : 0, i = lane & 31;
+        const bool mine = i < n;
+        const size_t at = static_cast<size_t>(r0 + i) * D.hv + h0 + e;
+        const float g = mine ? D.g[at] : 0.0f;
+        double G = g < kFloor ? kFloor : g;
+        for (int d = 1; d < kChunk; d <<= 1) {
+            const double x = __shfl_up(G, d, 32);
+            if (i >= d) G += x;
+        }
+        if (N == 2 || lane < kChunk) {
+            Gs[e][i] = G;
+            Bs[e][i] = mine ? D.beta[at] : 0.0f;
+        }
     }
     // operands: row 16 t + u, dims 32 s + 8 w ..; rows behind the sequence are zeros
     uintx4 kop[2][KS], qop[2][KS];
@@ -285,31 +291,31 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
         }
     }
     __syncthreads();
-    floatx4 qk[2][2];
+    floatx4 qk[N][2][2];
 #pragma unroll
     for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
         for (int tj = 0; tj <= ti; ++tj) {
-            floatx4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
-            qk[ti][tj] = kk;
+            floatx4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qq = kk;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 kk = mfma(kop[ti][s], kop[tj][s], kk);
-                qk[ti][tj] = mfma(qop[ti][s], kop[tj][s], qk[ti][tj]);
+                qq = mfma(qop[ti][s], kop[tj][s], qq);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * ti + 4 * w + r, j = 16 * tj + u;
-                const float d = j <= i ? expf(static_cast<float>(Gs[i] - Gs[j])) : 0.0f;
-                As[i][j] = j < i ? Bs[i] * kk[r] * d : 0.0f;
-                qk[ti][tj][r] *= d;
-                if (j > i) qk[ti][tj][r] = 0.0f;
-            }
+            for (int e = 0; e < N; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * ti + 4 * w + r, j = 16 * tj + u;
+                    const float d = j <= i ? expf(static_cast<float>(Gs[e][i] - Gs[e][j])) : 0.0f;
+                    As[e][i][j] = j < i ? Bs[e][i] * kk[r] * d : 0.0f;
+                    qk[e][ti][tj][r] = j <= i ? qq[r] * d : 0.0f;
+                }
         }
     __syncthreads();
     // the two diagonal blocks' inverses, a column per lane, by substitution
     {
-        const int b = 16 * (w & 1);
+        const int b = 16 * (w & 1), e = N == 2 ? w >> 1 : 0;
         float t[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -317,63 +323,78 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
                 if (j >= i) break;
-                const floatx4 a = *reinterpret_cast<const floatx4*>(&As[b + i][b + j]);
+                const floatx4 a = *reinterpret_cast<const floatx4*>(&As[e][b + i][b + j]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (j + e < i) x = fmaf(a[e], t[j + e], x);
+                for (int c = 0; c < 4; ++c)
+                    if (j + c < i) x = fmaf(a[c], t[j + c], x);
             }
             t[i] = i == u ? 1.0f : -x;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            Ts[b + i][b + u] = t[i];
-            Ts[i][16 + u] = 0.0f;
+            Ts[e][b + i][b + u] = t[i];
+            Ts[e][i][16 + u] = 0.0f;
         }
     }
     __syncthreads();
-    // the block below them: -T22 (A21 T11), float products
-    floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    // the block below them: -T22 (A21 T11), float products (A21 T11 in place of A11, which is done with)
+    floatx4 x[N];
 #pragma unroll
-    for (int k = 0; k < 16; k += 4) x = __builtin_amdgcn_mfma_f32_16x16x4f32(As[16 + u][k + w], Ts[k + w][u], x, 0, 0, 0);
+    for (int e = 0; e < N; ++e) {
+        x[e] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) Ws[4 * w + r][u] = x[r];
-    __syncthreads();
-    x = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < 16; k += 4)
+            x[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(As[e][16 + u][k + w], Ts[e][k + w][u], x[e], 0, 0, 0);
 #pragma unroll
-    for (int k = 0; k < 16; k += 4) x = __builtin_amdgcn_mfma_f32_16x16x4f32(Ts[16 + u][16 + k + w], Ws[k + w][u], x, 0, 0, 0);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) Ts[16 + 4 * w + r][u] = -x[r];
-    // (As has been read) the scores
-#pragma unroll
-    for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-        for (int tj = 0; tj < 2; ++tj)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) As[16 * ti + 4 * w + r][16 * tj + u] = tj <= ti ? qk[ti][tj][r] : 0.0f;
-    __syncthreads();
-    ChunkSystem& out = sys[static_cast<size_t>(blockIdx.x) * D.hv + h];
-    float beta[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) beta[j] = Bs[8 * w + j];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-        float row[8];
-        Parts<3> t;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) row[j] = Ts[chunk_row(u, a)][8 * w + j] * beta[j];
-        t.split(row);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) out.t[p][a][lane] = t.p[p];
-        Parts<2> m;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) row[j] = As[16 * a + u][8 * w + j];
-        m.split(row);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) out.m[p][a][lane] = m.p[p];
+        for (int r = 0; r < 4; ++r) As[e][4 * w + r][u] = x[e][r];
     }
-    if (lane < kChunk) {
-        out.into[lane] = expf(static_cast<float>(Gs[lane]));
-        out.left[lane] = expf(static_cast<float>(Gs[kChunk - 1] - Gs[lane]));
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        x[e] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+            x[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Ts[e][16 + u][16 + k + w], As[e][k + w][u], x[e], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) Ts[e][16 + 4 * w + r][u] = -x[e][r];
+    }
+    __syncthreads();
+    // the scores, where A was
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+            for (int tj = 0; tj < 2; ++tj)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) As[e][16 * ti + 4 * w + r][16 * tj + u] = tj <= ti ? qk[e][ti][tj][r] : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        ChunkSystem& out = sys[static_cast<size_t>(blockIdx.x) * D.hv + h0 + e];
+        float beta[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) beta[j] = Bs[e][8 * w + j];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            float row[8];
+            Parts<3> t;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) row[j] = Ts[e][chunk_row(u, a)][8 * w + j] * beta[j];
+            t.split(row);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) out.t[p][a][lane] = t.p[p];
+            Parts<2> m;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) row[j] = As[e][16 * a + u][8 * w + j];
+            m.split(row);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) out.m[p][a][lane] = m.p[p];
+        }
+        if (lane < kChunk) {
+            out.into[lane] = expf(static_cast<float>(Gs[e][lane]));
+            out.left[lane] = expf(static_cast<float>(Gs[e][kChunk - 1] - Gs[e][lane]));
+        }
     }
 }
 
@@ -686,7 +707,8 @@ int chunk_bound(const DeltaBatchDev& B) { return B.rows / kChunk + (B.seqs < B.r
 template <int DK>
 hipError_t launch_chunks(const DeltaDev& D, const DeltaBatchDev& B, ChunkSystem* sys, hipStream_t st) {
     const int bound = chunk_bound(B);
-    const hipError_t e = launch(k_delta_system<DK>, dim3(bound, D.hv), dim3(64), 0, st, D, B, sys);
+    const hipError_t e = D.hv / D.hk % 2 ? launch(k_delta_system<DK, 1>, dim3(bound, D.hv), dim3(64), 0, st, D, B, sys)
+                                         : launch(k_delta_system<DK, 2>, dim3(bound, D.hv / 2), dim3(64), 0, st, D, B, sys);
     if (e != hipSuccess) return e;
     using Geo = WalkGeo<DK>;
     if (const hipError_t l = ensure_lds<k_delta_chunks<DK>>(Geo::kLds); l != hipSuccess) return l;
