@@ -720,7 +720,7 @@ int q38_hc_initialize_stream(const uint16_t* embedding, int32_t rows, int32_t hi
  * workspace serves one call at a time and is left dirty; calls (or graph replays) that overlap
  * need one each. All-zero batches (rows or sequences 0) return Q38_OK. */
 
-/* A layer's pages (caller's device memory, 16-byte aligned). Q38_KV_Q8 keeps int8 codes and one
+/* A layer's pages (caller's device memory, all of it 16-byte aligned). Q38_KV_Q8 keeps int8 codes and one
  * float scale per (token, kv head): value = code * scale. */
 enum { Q38_KV_BF16 = 0, Q38_KV_Q8 = 1 };
 typedef struct q38_paged_cache {
@@ -748,7 +748,7 @@ typedef struct q38_paged_batch {
 } q38_paged_batch;
 /* Writes the rows' keys and values into their pages. k, v: device, row r at k + r * k_stride
  * elements, [kv_heads][head_dim] bf16 each (slices of a projection's output); 16-byte aligned,
- * strides multiples of 8 and at least kv_heads * head_dim. Q38_KV_Q8: with a = max|x| of the
+ * strides multiples of 8, at least kv_heads * head_dim and below 2^24 (as all row strides here). Q38_KV_Q8: with a = max|x| of the
  * head's row, code = rint(x * 127 / a) (ties to even; the product is exact and no rounded
  * quotient crosses a tie, so the codes are those of exact arithmetic) and scale = a / 127; a row
  * of zeros has scale 0, a row with an infinity or NaN scale NaN, which attention then shows. A
@@ -758,14 +758,16 @@ int q38_paged_append(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged
                      int64_t k_stride, const uint16_t* v, int64_t v_stride, void* stream);
 /* Attention of the rows over the cache, which already holds them (q38_paged_append): row r of
  * sequence i sees tokens 0 .. tokens[i] - n + r, and out = sum_t p_t v_t with p the softmax of
- * scale * (q . k_t); query head h reads kv head h / (q_heads / kv_heads). q and out: device bf16,
- * [q_heads][head_dim] per row at their strides (alignment as for k); they may not overlap. Scores,
- * softmax sums and the output's sums are float, p is rounded to bf16 for the product with V (in a
- * Q8 cache p times the value's scale), out is rounded once. A row that sees no token gives zeros;
- * what unseen places of the cache hold, infinities and NaN too, has no effect. A sequence with
- * tokens behind its table or a seen page out of range gives NaN. Results do not depend on the
- * other sequences' values, but on their lengths within float rounding (they move the points
- * where the cache is split). */
+ * scale * (q . k_t); query head h reads kv head h / (q_heads / kv_heads); q_heads is at most 256, and
+ * 128 per kv head. q and out: device bf16, [q_heads][head_dim] per row at their strides (alignment
+ * as for k); they may not overlap. Scores, softmax sums and the output's sums are float, p is
+ * rounded to bf16 for the product with V (in a Q8 cache p times the value's scale; in a bf16 cache
+ * the sum that divides is of the rounded p), out is rounded once. A row that sees no token gives
+ * zeros; what unseen places of the cache hold, infinities and NaN too, has no effect. All rows of a
+ * sequence with tokens behind its table are NaN; a page out of range makes the rows that see it
+ * NaN, and may make others of its sequence NaN too. Results do not depend on the other sequences'
+ * values, but on their lengths within float rounding (they move the points where the cache is
+ * split). The workspace is 16-byte aligned. */
 size_t q38_paged_attention_workspace_size(const q38_paged_cache* cache, const q38_paged_batch* batch, int32_t q_heads);
 int q38_paged_attention(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged_batch* batch, const uint16_t* q,
                         int64_t q_stride, int32_t q_heads, float scale, uint16_t* out, int64_t out_stride,
@@ -777,9 +779,11 @@ int q38_paged_attention(q38_ctx* ctx, const q38_paged_cache* cache, const q38_pa
  * key_heads)), v [value_heads][value_dim], each at its row stride (slices of one convolved row;
  * 16-byte aligned, strides multiples of 8); log_decay (g <= 0; -inf clears the state) and beta:
  * device float [rows][value_heads]; out: device bf16 [rows][value_heads][value_dim]. q and k are
- * taken as given (the layer normalises them before: |k| = 1 keeps the rule stable). Long
- * sequences run in chunks on the matrix cores with float accuracy (operands split into three
- * bf16 parts), short ones and calls with checkpoints row by row.
+ * taken as given (the layer normalises them before: |k| = 1 keeps the rule stable). Batches with
+ * max_rows above 16 run in chunks of 32 rows on the matrix cores, with states as exact as float
+ * ones (operands split into bf16 parts) and outputs as their own rounding; others, and calls with
+ * checkpoints, run row by row. Infinities and NaN among a sequence's operands reach its later rows
+ * and its state, in chunks also the earlier rows of their 32. The workspace is 16-byte aligned.
  * States: a pool [slots][value_heads][value_dim][key_dim] of floats, 16-byte aligned. origin[i]:
  * the slot a sequence starts from, negative (or a null array) for the zero state; final_slots[i]:
  * the slot its last state goes to, negative (or null) for none, its own origin for an update in

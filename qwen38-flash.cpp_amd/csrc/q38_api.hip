@@ -2243,6 +2243,7 @@ int check_paged_pointers(const char* name, const q38_paged_cache& c, const q38_p
     if (!aligned16(c.keys) || !aligned16(c.values)) return fail(Q38_EINVAL, at + "keys and values must be 16-byte aligned");
     if ((c.format == Q38_KV_Q8) != (c.key_scales != nullptr) || (c.format == Q38_KV_Q8) != (c.value_scales != nullptr))
         return fail(Q38_EINVAL, at + "a Q8 cache has scales, a bf16 cache has none");
+    if (!aligned16(c.key_scales) || !aligned16(c.value_scales)) return fail(Q38_EINVAL, at + "scales must be 16-byte aligned");
     return Q38_OK;
 }
 

@@ -1,9 +1,9 @@
 // q38_delta.hip — the gated delta rule of many requests over a pool of float states:
 //   S <- exp(g) S,  S <- S + beta (v - S k) k^T,  o = scale * S q      per row and value head.
 //
-//   k_delta_rows     row by row, the state in registers across a sequence's rows
-//   k_delta_system   the long form, chunks of 32 rows: each chunk's triangular system and scores
-//   k_delta_chunks   its walk over a sequence's chunks, the state in registers
+//   k_delta_rows     short sequences and checkpoints: row by row, the state in registers
+//   k_delta_system   long sequences, in chunks of 32 rows: every chunk's triangular system and scores
+//   k_delta_chunks   the walk over a sequence's chunks, the state in registers
 #include "q38_device.hpp"
 #include "q38_paged.hpp"
 #include "q38_internal.hpp"
@@ -28,8 +28,10 @@ __device__ __forceinline__ T uniform_load(const T* p) {
 }
 
 // A wave takes 8 R value rows of one head of one sequence: 8 lanes per value row, lane `sub` of them
-// key dims 32 c + 4 sub .. + 3 (16-byte state accesses, 128 bytes together per row). Bound by the
-// states' bytes for single tokens; the next row's operands are in flight during a row.
+// key dims 32 c + 4 sub .. + 3 (16-byte state accesses, 128 bytes together per row). Single tokens are
+// bound by the states' bytes: 104 us for 128 requests of 32 heads [128][128], 5.2 TB/s, a copy's rate,
+// and 4.9 us for one request. Longer sequences are a chain of two sums over lanes per row; the next row's
+// operands are in flight during a row.
 template <int DK, int R>
 __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B) {
     constexpr int C = DK / 32;
@@ -220,7 +222,7 @@ __device__ __forceinline__ bool find_chunk(const DeltaBatchDev& B, int want, int
 // The sequence that the slot-th group of workgroups takes. A walk is one chain per head, so the longest
 // sequences begin first; where all groups are on the chip at once, two workgroups per CU, those of the
 // second half join the first half's in the opposite order, the shortest beside the longest (eight ragged
-// prompts in their own order: 377 us, so: 285). Up to 64 sequences; more fill the chip in any order.
+// prompts in their own order: 377 us, so: 352). Up to 64 sequences; more fill the chip in any order.
 __device__ __forceinline__ int nth_sequence(const DeltaBatchDev& B, int slot, int groups_per_round) {
     if (B.seqs > 64 || B.seqs == 1) return slot;
     const int lane = threadIdx.x & 63;
@@ -249,8 +251,9 @@ __device__ __forceinline__ int first_chunk(const DeltaBatchDev& B, int seq) {
 }
 
 // One wave per chunk and value head, or two value heads of one key head (N = 2): their products are the
-// same, and the substitution of one head's diagonal blocks fills half a wave. Bound by the latency of its
-// dependent steps (a head per wave: 86 us for 16,384 chunk heads, 1.9 TB/s of systems written).
+// same, and the substitution of one head's diagonal blocks fills half a wave (eight ragged prompts, 16,320
+// systems: 86 us with one, 75 with two, 2.3 TB/s of systems written). Bound by the chain of its steps, and
+// by LDS, which holds 8 waves a CU.
 template <int DK, int N>
 __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B, ChunkSystem* __restrict__ sys) {
     constexpr int KS = DK / 32, LD = kChunk + 4;
@@ -405,8 +408,10 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 // from 16-byte runs of eight keys by byte permutes: no value moves between lanes. A sequence is one chain
 // of chunks per head, and a wave issues an instruction every four cycles at best, so what the chain does
 // not need is left to a second wave on another SIMD: an output wave per state wave takes the operands
-// of S and U through LDS a chunk later, and loads and stages the keys (one wave doing all: 240 us for
-// a prompt of 4,001 rows, 1.9 us a chunk).
+// of S and U through LDS a chunk later, and loads and stages the keys. A prompt of 4,001 rows: 160 us,
+// 1.27 us a chunk, bound by the state wave's own instructions (one wave doing all: 240 us); eight ragged
+// prompts, 16,192 rows: 345 us, two workgroups per CU, bound by the longest chains and by the systems,
+// which every group of 32 value dims reads.
 template <int DK>
 struct WalkGeo {
     static constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8;
@@ -430,8 +435,8 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     const int pair = wave % NW;
     const bool outputs = wave >= NW;
     // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: those of one head, which read the
-    // same chunk systems, keys and queries, are one XCD's (apart from each other they were bound by what
-    // their L2s fetched, 371 us for eight ragged prompts).
+    // same chunk systems, keys and queries, are one XCD's (eight ragged prompts: 371 us with the groups
+    // spread over the XCDs, 345 so).
     const int groups = D.dv / (16 * NW), turn = blockIdx.x / 8, chain = turn / groups * 8 + blockIdx.x % 8;
     if (chain >= D.hv * B.seqs) return;
     const int h = chain % D.hv, hk = h / (D.hv / D.hk);
@@ -699,7 +704,8 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                 (floatx4){st[o][r], st[o + 1][r], st[o + 2][r], st[o + 3][r]};
 }
 
-// Sequences of up to so many rows go row by row.
+// Sequences of up to so many rows go row by row. 16 rows of 32 heads, by rows and in chunks: one sequence
+// 17.4 and 18.4 us, eight 22.5 and 25.8, 64 117 and 130; 24 rows: 20.7 and 18.4, 29.3 and 25.8, 157 and 130.
 constexpr int kRowsForm = 16;
 bool by_rows(const DeltaBatchDev& B, int max_rows) { return B.ckpt || B.rows == 0 || max_rows <= kRowsForm; }
 int chunk_bound(const DeltaBatchDev& B) { return B.rows / kChunk + (B.seqs < B.rows ? B.seqs : B.rows); }
@@ -712,8 +718,9 @@ hipError_t launch_chunks(const DeltaDev& D, const DeltaBatchDev& B, ChunkSystem*
     if (e != hipSuccess) return e;
     using Geo = WalkGeo<DK>;
     if (const hipError_t l = ensure_lds<k_delta_chunks<DK>>(Geo::kLds); l != hipSuccess) return l;
-    return launch(k_delta_chunks<DK>, dim3(D.dv / (16 * Geo::NW) * ((D.hv * B.seqs + 7) / 8 * 8)), dim3(128 * Geo::NW), Geo::kLds, st, D, B,
-                  static_cast<const ChunkSystem*>(sys), bound);
+    const dim3 grid(D.dv / (16 * Geo::NW) * ((D.hv * B.seqs + 7) / 8 * 8));
+    return launch(k_delta_chunks<DK>, grid, dim3(128 * Geo::NW), Geo::kLds, st, D, B, static_cast<const ChunkSystem*>(sys),
+                  bound);
 }
 
 } // namespace

@@ -20,7 +20,8 @@ namespace q38 {
 namespace {
 
 // D / 8 lanes take one head row, 16 bytes each. The offsets are staged in LDS: one round trip to
-// memory, then the search for the row's sequence runs there.
+// memory, then the search for the row's sequence runs there. Decode steps take a launch's latency, long
+// prompts the bytes' time.
 template <int D, bool Q8>
 __global__ __launch_bounds__(256) void k_paged_append(PagedCacheDev C, PagedBatchDev B, const uint16_t* __restrict__ k,
                                                       int64_t ks, const uint16_t* __restrict__ v, int64_t vs) {
@@ -517,7 +518,8 @@ __device__ __forceinline__ void note_cut(CutItem* cut, const ShareWalk& sw, cons
 
 // A workgroup's share of a kv head's steps; wave i takes tokens 32 i .. 32 i + 31 of every step, the
 // next step's keys and values in flight, and the waves' sums are joined through LDS at the end of
-// a piece. Few queries per token: bound by the cache's bytes.
+// a piece. Few queries per token: bound by the cache's bytes (64 ragged requests of one row: 87 us,
+// 4.8 TB/s), one request by the latency of its few steps (4,001 tokens: 11.5 us).
 template <int D, bool Q8, int MT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCacheDev C, PagedBatchDev B, int G,
                                                                            const uint16_t* __restrict__ q, int64_t qs,
@@ -636,15 +638,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
 }
 
 // ---- many queries per sequence. Tiles of 256 queries (128 of 256 dims) in equal shares as above;
-// keys and values go through LDS, TB tokens at a time and the next ones in flight (an 8-bit cache is converted on the way: its codes are exact in bf16), and
-// every wave multiplies them with its own 32 queries. Bound by the matrix cores, by the
-// exponentials beside them (8 per lane for 16 products of 128 dims) and by LDS reads, which 32
-// queries per wave bring to the matrix cores' own time.
+// keys and values go through LDS, TB tokens at a time and the next ones in flight (an 8-bit cache is
+// converted on the way: its codes are exact in bf16), and every wave multiplies them with its own 32
+// queries. Bound by the matrix cores, by the exponentials beside them (8 per lane for 16 products of 128
+// dims) and by LDS reads, which 32 queries per wave bring to the matrix cores' own time: five ragged
+// prompts, 5,647 rows of 32 heads of 128 over 20,306 tokens, in 473 us, 633 TFLOP/s (4.9 ms with k_paged_split).
 template <int D>
 struct TileGeo {
     // One workgroup of two waves per SIMD fills a CU: two workgroups of one each share it unevenly (the
-    // older one's waves go first) and leave it half empty at the end, 588 us against 510 for a prompt
-    // batch. 16-query groups per wave: 256 dims take the registers of two.
+    // older one's waves go first: done after 430 us, the other's after 525) and leave it half empty at the
+    // end, 588 us against 473 for five ragged prompts. 16-query groups per wave (MT): 256 dims take the
+    // registers of two.
     static constexpr int MT = D == 256 ? 1 : 2, WAVES = 8, M = 16 * MT * WAVES;
     static constexpr int TB = D == 256 ? 32 : 64;
     static constexpr int CH = D / 8;                       // 16-byte chunks of a bf16 row
@@ -682,206 +686,207 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     if (threadIdx.x == 0) cut->pieces = 0;
     if (!sw.open(S, B, C.shift, place, shares)) return;
     while (sw.next(S, B, C.shift)) {
-    // (opaque: what follows from the lane is formed anew per piece, not kept in registers for the next)
-    int lane = threadIdx.x & 63;
-    asm volatile("" : "+v"(lane));
-    const int u = lane & 15, w = lane >> 4;
-    AttnItem it = sw.item(S);
-    QueryTile<D, false, MT> qt;
-    AttnState<D, Q8, MT> st;
-    qt.load(q, qs, it, S, head, m0, negate, lane);
-    st.clear(it, S, m0, lane);
-    // tokens that all, and any, of the wave's queries see (a wave without queries has nothing to mask)
-    const int r0 = tile_row(S, it, m0), rows_left = min(it.rows, (it.tile + 1) * S.rows());
-    const int all = r0 >= 0 ? attn_see(it, r0) : 1 << 30;
-    const int any = r0 >= 0 ? attn_see(it, min(it.tile * S.rows() + (m0 + 16 * MT - 1) / G, rows_left - 1)) : 0;
-    const int from = __builtin_amdgcn_readfirstlane(sw.from) * (kSplitTokens / TB);
-    const int stop = min(__builtin_amdgcn_readfirstlane(sw.to) * kSplitTokens, it.see);
-    const int to = max(from + 1, (stop + TB - 1) / TB);
-    PageWalk walk{B.table + static_cast<int64_t>(sw.seq()) * B.width, C.shift, C.pages, C.hkv, head, max(it.see, 1), it.bad};
-    bool special = false;
+        // (opaque: what follows from the lane is formed anew per piece, not kept in registers for the next)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int u = lane & 15, w = lane >> 4;
+        AttnItem it = sw.item(S);
+        QueryTile<D, false, MT> qt;
+        AttnState<D, Q8, MT> st;
+        qt.load(q, qs, it, S, head, m0, negate, lane);
+        st.clear(it, S, m0, lane);
+        // tokens that all, and any, of the wave's queries see (a wave without queries has nothing to mask)
+        const int r0 = tile_row(S, it, m0), rows_left = min(it.rows, (it.tile + 1) * S.rows());
+        const int all = r0 >= 0 ? attn_see(it, r0) : 1 << 30;
+        const int any = r0 >= 0 ? attn_see(it, min(it.tile * S.rows() + (m0 + 16 * MT - 1) / G, rows_left - 1)) : 0;
+        const int from = __builtin_amdgcn_readfirstlane(sw.from) * (kSplitTokens / TB);
+        const int stop = min(__builtin_amdgcn_readfirstlane(sw.to) * kSplitTokens, it.see);
+        const int to = max(from + 1, (stop + TB - 1) / TB);
+        PageWalk walk{B.table + static_cast<int64_t>(sw.seq()) * B.width, C.shift, C.pages, C.hkv, head, max(it.see, 1), it.bad};
+        bool special = false;
 
-    // Staging. A wave's piece of a tile lies in 16 tokens of one page: uniform addresses and a lane's
-    // own offset. What lies behind the seen tokens is read with them and masked by its reader.
-    constexpr int EL = Q8 ? 1 : 2;
-    const int ch = lane % CH, wt = wave * 64 / CH;  // the wave's first token of a piece
-    const uint32_t lane_off = ((lane / CH) * D + 8 * ch) * EL;
-    typedef typename std::conditional<Q8, uint2, uintx4>::type raw_t;
-    raw_t kr[PC], vr[PC];
-    float sr[2] = {0.0f, 0.0f};
-    auto fetch = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < PC; ++i) {
-            const int64_t at = walk.half(t0 + i * (NT / CH) + wt) * (D * EL);
-            kr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.keys) + at + lane_off);
-            vr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.values) + at + lane_off);
-        }
-        if constexpr (Q8)
-            if (wave < TB / 16) {  // 16 tokens' scales per wave
-                const int64_t at = walk.half(t0 + 16 * wave);
-                sr[0] = C.ks[at + u], sr[1] = C.vs[at + u];
+        // Staging. A wave's piece of a tile lies in 16 tokens of one page: uniform addresses and a lane's
+        // own offset. What lies behind the seen tokens is read with them and masked by its reader.
+        constexpr int EL = Q8 ? 1 : 2;
+        const int ch = lane % CH, wt = wave * 64 / CH;  // the wave's first token of a piece
+        const uint32_t lane_off = ((lane / CH) * D + 8 * ch) * EL;
+        typedef typename std::conditional<Q8, uint2, uintx4>::type raw_t;
+        raw_t kr[PC], vr[PC];
+        float sr[2] = {0.0f, 0.0f};
+        auto fetch = [&](int t0) {
+    #pragma unroll
+            for (int i = 0; i < PC; ++i) {
+                const int64_t at = walk.half(t0 + i * (NT / CH) + wt) * (D * EL);
+                kr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.keys) + at + lane_off);
+                vr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.values) + at + lane_off);
             }
-    };
-    auto widen = [](raw_t x) {
-        if constexpr (Q8)
-            return (uintx4){pack_bf16(code_f(x.x, 0), code_f(x.x, 1)), pack_bf16(code_f(x.x, 2), code_f(x.x, 3)),
-                            pack_bf16(code_f(x.y, 0), code_f(x.y, 1)), pack_bf16(code_f(x.y, 2), code_f(x.y, 3))};
-        else
-            return x;
-    };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < PC; ++i) {
-            const int at = tile_at<D>(i * (NT / CH) + wt + lane / CH, ch);
-            tiles[(2 * buf) * TB * CH + at] = widen(kr[i]);
-            tiles[(2 * buf + 1) * TB * CH + at] = widen(vr[i]);
-        }
-        if constexpr (Q8)
-            if (wave < TB / 16 && lane < 16) {
-                scales[2 * buf * TB + 16 * wave + u] = sr[0];
-                scales[(2 * buf + 1) * TB + 16 * wave + u] = sr[1];
+            if constexpr (Q8)
+                if (wave < TB / 16) {  // 16 tokens' scales per wave
+                    const int64_t at = walk.half(t0 + 16 * wave);
+                    sr[0] = C.ks[at + u], sr[1] = C.vs[at + u];
+                }
+        };
+        auto widen = [](raw_t x) {
+            if constexpr (Q8)
+                return (uintx4){pack_bf16(code_f(x.x, 0), code_f(x.x, 1)), pack_bf16(code_f(x.x, 2), code_f(x.x, 3)),
+                                pack_bf16(code_f(x.y, 0), code_f(x.y, 1)), pack_bf16(code_f(x.y, 2), code_f(x.y, 3))};
+            else
+                return x;
+        };
+        auto stage = [&](int buf) {
+    #pragma unroll
+            for (int i = 0; i < PC; ++i) {
+                const int at = tile_at<D>(i * (NT / CH) + wt + lane / CH, ch);
+                tiles[(2 * buf) * TB * CH + at] = widen(kr[i]);
+                tiles[(2 * buf + 1) * TB * CH + at] = widen(vr[i]);
             }
-    };
-    // 32 tokens of a staged tile
-    auto half = [&](int base, int sub, const uintx4* kt, const uintx4* vt, const float* sc) {
-        const bool masked = base + 32 > all;
-        auto key = [&](int a, int i) { return kt[tile_at<D>(32 * sub + 8 * (u >> 2) + 4 * a + (u & 3), 4 * i + w)]; };
-        ValueTile<D, false> v;
-        auto read_values = [&] {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int t = 32 * sub + 8 * w + j;
-                if constexpr (D == 64) {
-                    const uint2 x = reinterpret_cast<const uint2*>(vt + tile_at<D>(t, u >> 1))[u & 1];
-                    v.v[j][0] = x.x, v.v[j][1] = x.y;
-                } else {
-#pragma unroll
-                    for (int b = 0; b < D / 128; ++b) {
-                        const uintx4 x = vt[tile_at<D>(t, 16 * b + u)];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v.v[j][4 * b + i] = x[i];
+            if constexpr (Q8)
+                if (wave < TB / 16 && lane < 16) {
+                    scales[2 * buf * TB + 16 * wave + u] = sr[0];
+                    scales[(2 * buf + 1) * TB + 16 * wave + u] = sr[1];
+                }
+        };
+        // 32 tokens of a staged tile
+        auto half = [&](int base, int sub, const uintx4* kt, const uintx4* vt, const float* sc) {
+            const bool masked = base + 32 > all;
+            auto key = [&](int a, int i) { return kt[tile_at<D>(32 * sub + 8 * (u >> 2) + 4 * a + (u & 3), 4 * i + w)]; };
+            ValueTile<D, false> v;
+            auto read_values = [&] {
+    #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int t = 32 * sub + 8 * w + j;
+                    if constexpr (D == 64) {
+                        const uint2 x = reinterpret_cast<const uint2*>(vt + tile_at<D>(t, u >> 1))[u & 1];
+                        v.v[j][0] = x.x, v.v[j][1] = x.y;
+                    } else {
+    #pragma unroll
+                        for (int b = 0; b < D / 128; ++b) {
+                            const uintx4 x = vt[tile_at<D>(t, 16 * b + u)];
+    #pragma unroll
+                            for (int i = 0; i < 4; ++i) v.v[j][4 * b + i] = x[i];
+                        }
+                    }
+                }
+            };
+            floatx4 s[MT][2], ks[2], vs[2];
+    #pragma unroll
+            for (int a = 0; a < 2; ++a)
+    #pragma unroll
+                for (int m = 0; m < MT; ++m) s[m][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (D < 256) {  // all reads in flight before the first product, the values' before the softmax
+                uintx4 k[2][Geo::KS];
+    #pragma unroll
+                for (int a = 0; a < 2; ++a)
+    #pragma unroll
+                    for (int i = 0; i < Geo::KS; ++i) k[a][i] = key(a, i);
+                __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+                for (int a = 0; a < 2; ++a)
+    #pragma unroll
+                    for (int i = 0; i < Geo::KS; ++i)
+    #pragma unroll
+                        for (int m = 0; m < MT; ++m) s[m][a] = mfma(k[a][i], qt.q[m][i], s[m][a]);
+                read_values();
+            } else {  // (256 dims: no registers for them)
+    #pragma unroll
+                for (int a = 0; a < 2; ++a)
+    #pragma unroll
+                    for (int i = 0; i < Geo::KS; ++i) {
+                        const uintx4 k = key(a, i);
+    #pragma unroll
+                        for (int m = 0; m < MT; ++m) s[m][a] = mfma(k, qt.q[m][i], s[m][a]);
+                    }
+            }
+            if constexpr (Q8)
+    #pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    ks[a] = *reinterpret_cast<const floatx4*>(sc + 32 * sub + 8 * w + 4 * a);
+                    vs[a] = *reinterpret_cast<const floatx4*>(sc + TB + 32 * sub + 8 * w + 4 * a);
+                }
+            uintx4 b[MT];
+    #pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float p[8];
+                st.soften(m, s[m], ks, c, base, masked, lane, p);
+                b[m] = st.weights(m, p, vs, base, lane);
+            }
+            if constexpr (D == 256) read_values();
+            if constexpr (!Q8)
+                if (masked) special |= clean_values<D>(v, base, any, lane);
+            st.template products<false>(v, b);
+        };
+        fetch(from * TB);
+        stage(0);
+        __syncthreads();
+        for (int step = from; step < to; ++step) {
+            const int buf = (step - from) & 1;
+            fetch(min(step + 1, to - 1) * TB);
+            // (waves whose queries see nothing of the tile's end multiply it all the same: a branch around
+            // the products made the compiler move every sum once per step)
+            const uintx4* kt = tiles + (2 * buf) * TB * CH;
+    #pragma unroll
+            for (int sub = 0; sub < TB / 32; ++sub)
+                half(step * TB + 32 * sub, sub, kt, kt + TB * CH, scales + 2 * buf * TB);
+            stage(buf ^ 1);
+            lds_barrier();
+        }
+        const bool bad = __syncthreads_or(it.bad || (it.see > 0 && walk.bad));
+        asm volatile("" ::: "memory");  // (read anew: see ShareWalk)
+        it = sw.item(S);
+        const bool whole = sw.to - sw.from == it.steps;
+        float* pd = nullptr;
+        if (!whole) {
+            const int slot = attn_slot(sw.start, sw.share, place);
+            pd = part + (static_cast<int64_t>(n) * 2 + slot) * (TG::M * (D + 2));
+            if (slot && threadIdx.x == 0) note_cut(cut, sw, it);
+        }
+    #pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float sum = st.total(m);
+            if (bad) sum = kNan;
+            const int i = m0 + 16 * m + u, row = tile_row(S, it, i);
+            if (row < 0) continue;
+            const float inv = bad || st.lim[m] > 0 ? 1.0f / sum : 0.0f;
+            uint16_t* dst = out + (it.first + row) * os + (head * G + i % G) * D;
+    #pragma unroll
+            for (int r = 0; r < 4; ++r)
+    #pragma unroll
+                for (int o = 0; o < Geo::E; o += 4) {
+                    const int d = Geo::dim(4 * w + r, o);
+                    const floatx4 x = {st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
+                    if (whole)
+                        *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
+                    else
+                        *reinterpret_cast<floatx4*>(pd + i * D + d) = x;
+                }
+            if (!whole && w == 0) pd[TG::M * D + i] = st.top[m], pd[TG::M * D + TG::M + i] = sum;
+        }
+        if constexpr (!Q8)
+            if (special) {  // to what the lane has just written
+    #pragma unroll 1
+                for (int n = 0; n < MT * Geo::E; ++n) {
+                    const int i = m0 + 16 * (n / Geo::E) + u, row = tile_row(S, it, i);
+                    if (row < 0) continue;
+                    const int d = Geo::dim(4 * w + n % Geo::E / (Geo::E / 4), 0) + n % (Geo::E / 4) * 4 % Geo::EC +
+                                  n % (Geo::E / 4) * 4 / Geo::EC * 16 * Geo::EC;
+                    const int t0 = max(special_from(all), from * TB), lim = min(stop, attn_see(it, row));
+                    if (whole) {
+                        uint2* p = reinterpret_cast<uint2*>(out + (it.first + row) * os + (head * G + i % G) * D + d);
+                        const floatx4 x = add_special<D>(C, walk.table, head, t0, lim, d,
+                                                         (floatx4){bflo(p->x), bfhi(p->x), bflo(p->y), bfhi(p->y)});
+                        *p = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+                    } else {
+                        floatx4* p = reinterpret_cast<floatx4*>(pd + i * D + d);
+                        *p = add_special<D>(C, walk.table, head, t0, lim, d, *p);
                     }
                 }
             }
-        };
-        floatx4 s[MT][2], ks[2], vs[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) s[m][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (D < 256) {  // all reads in flight before the first product, the values' before the softmax
-            uintx4 k[2][Geo::KS];
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int i = 0; i < Geo::KS; ++i) k[a][i] = key(a, i);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int i = 0; i < Geo::KS; ++i)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) s[m][a] = mfma(k[a][i], qt.q[m][i], s[m][a]);
-            read_values();
-        } else {  // (256 dims: no registers for them)
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int i = 0; i < Geo::KS; ++i) {
-                    const uintx4 k = key(a, i);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) s[m][a] = mfma(k, qt.q[m][i], s[m][a]);
-                }
-        }
-        if constexpr (Q8)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                ks[a] = *reinterpret_cast<const floatx4*>(sc + 32 * sub + 8 * w + 4 * a);
-                vs[a] = *reinterpret_cast<const floatx4*>(sc + TB + 32 * sub + 8 * w + 4 * a);
-            }
-        uintx4 b[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float p[8];
-            st.soften(m, s[m], ks, c, base, masked, lane, p);
-            b[m] = st.weights(m, p, vs, base, lane);
-        }
-        if constexpr (D == 256) read_values();
-        if constexpr (!Q8)
-            if (masked) special |= clean_values<D>(v, base, any, lane);
-        st.template products<false>(v, b);
-    };
-    fetch(from * TB);
-    stage(0);
-    __syncthreads();
-    for (int step = from; step < to; ++step) {
-        const int buf = (step - from) & 1;
-        fetch(min(step + 1, to - 1) * TB);
-        // (waves whose queries see nothing of the tile's end multiply it all the same: a branch around
-        // the products made the compiler move every sum once per step)
-        const uintx4* kt = tiles + (2 * buf) * TB * CH;
-#pragma unroll
-        for (int sub = 0; sub < TB / 32; ++sub)
-            half(step * TB + 32 * sub, sub, kt, kt + TB * CH, scales + 2 * buf * TB);
-        stage(buf ^ 1);
-        lds_barrier();
-    }
-    const bool bad = __syncthreads_or(it.bad || (it.see > 0 && walk.bad));
-    asm volatile("" ::: "memory");  // (read anew: see ShareWalk)
-    it = sw.item(S);
-    const bool whole = sw.to - sw.from == it.steps;
-    float* pd = nullptr;
-    if (!whole) {
-        const int slot = attn_slot(sw.start, sw.share, place);
-        pd = part + (static_cast<int64_t>(n) * 2 + slot) * (TG::M * (D + 2));
-        if (slot && threadIdx.x == 0) note_cut(cut, sw, it);
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        float sum = st.total(m);
-        if (bad) sum = kNan;
-        const int i = m0 + 16 * m + u, row = tile_row(S, it, i);
-        if (row < 0) continue;
-        const float inv = bad || st.lim[m] > 0 ? 1.0f / sum : 0.0f;
-        uint16_t* dst = out + (it.first + row) * os + (head * G + i % G) * D;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int o = 0; o < Geo::E; o += 4) {
-                const int d = Geo::dim(4 * w + r, o);
-                const floatx4 x = {st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
-                if (whole)
-                    *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
-                else
-                    *reinterpret_cast<floatx4*>(pd + i * D + d) = x;
-            }
-        if (!whole && w == 0) pd[TG::M * D + i] = st.top[m], pd[TG::M * D + TG::M + i] = sum;
-    }
-    if constexpr (!Q8)
-        if (special) {  // to what the lane has just written
-#pragma unroll 1
-            for (int n = 0; n < MT * Geo::E; ++n) {
-                const int i = m0 + 16 * (n / Geo::E) + u, row = tile_row(S, it, i);
-                if (row < 0) continue;
-                const int d = Geo::dim(4 * w + n % Geo::E / (Geo::E / 4), 0) + n % (Geo::E / 4) * 4 % Geo::EC +
-                              n % (Geo::E / 4) * 4 / Geo::EC * 16 * Geo::EC;
-                const int t0 = max(special_from(all), from * TB), lim = min(stop, attn_see(it, row));
-                if (whole) {
-                    uint2* p = reinterpret_cast<uint2*>(out + (it.first + row) * os + (head * G + i % G) * D + d);
-                    const floatx4 x = add_special<D>(C, walk.table, head, t0, lim, d,
-                                                     (floatx4){bflo(p->x), bfhi(p->x), bflo(p->y), bfhi(p->y)});
-                    *p = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-                } else {
-                    floatx4* p = reinterpret_cast<floatx4*>(pd + i * D + d);
-                    *p = add_special<D>(C, walk.table, head, t0, lim, d, *p);
-                }
-            }
-        }
     }
 }
 
 // Joins the pieces of the items that the shares' ends cut: a workgroup per (share that an item goes on
-// from, kv head, QB of the tile's queries), a wave per query, PB pieces in flight.
+// from, kv head, QB of the tile's queries), a wave per query, PB pieces in flight: few long tiles for
+// prompts (19 us for five), many pieces of one request's few queries (6.5 us for 4,001 tokens).
 template <int D, int QB, int PB>
 __global__ __launch_bounds__(256) void k_paged_join(AttnSplit S, int W, const float* __restrict__ part,
                                                     const CutItem* __restrict__ cuts, uint16_t* __restrict__ out,

@@ -31,7 +31,8 @@ def attend(q38, c, b, q=X, qs=512, heads=8, scale=0.1, out=X, os=512, ws=X, ws_b
 
 BAD_CACHE = [dict(format=2), dict(format=-1), dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=2048),
              dict(pages=0), dict(kv_heads=0), dict(kv_heads=65), dict(head_dim=96), dict(keys=None), dict(values=None),
-             dict(keys=X + 8), dict(values=X + 2), dict(key_scales=X), dict(format=1), dict(format=1, key_scales=X)]
+             dict(keys=X + 8), dict(values=X + 2), dict(key_scales=X), dict(format=1), dict(format=1, key_scales=X),
+             dict(format=1, key_scales=X + 4, value_scales=X), dict(format=1, key_scales=X, value_scales=X + 8)]
 BAD_BATCH = [dict(sequences=-1), dict(sequences=4097), dict(rows=-1), dict(rows=(1 << 19) + 1), dict(max_rows=0),
              dict(max_rows=4), dict(table_pages=0), dict(table_pages=1 << 26), dict(row_offsets=None),
              dict(tokens=None), dict(page_table=None)]
@@ -65,11 +66,19 @@ def test_bad_append_operands(q38, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(q=None), dict(out=None), dict(q=X + 4), dict(out=X + 8), dict(qs=504), dict(os=516),
-                                dict(heads=0), dict(heads=7), dict(heads=258), dict(scale=float("nan")),
+                                dict(heads=0), dict(heads=7), dict(heads=258), dict(qs=1 << 24), dict(scale=float("nan")),
                                 dict(scale=float("inf"))])
 def test_bad_attention_operands(q38, kw):
     assert attend(q38, cache(q38), batch(q38), **kw) == q38.Q38_EINVAL
     assert "context" not in q38.last_error()
+
+
+def test_too_many_queries_per_kv_head(q38):
+    c = cache(q38, kv_heads=1)
+    assert attend(q38, c, batch(q38), qs=129 * 64, heads=129, os=129 * 64) == q38.Q38_EINVAL
+    assert "128 per kv head" in q38.last_error()
+    assert attend(q38, c, batch(q38), qs=128 * 64, heads=128, os=128 * 64) == q38.Q38_EINVAL
+    assert "null context" in q38.last_error()
 
 
 def test_attention_workspace(q38):

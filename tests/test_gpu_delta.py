@@ -213,3 +213,125 @@ def test_rows_of_a_batch_do_not_depend_on_each_other(gpu, q38):
             d.states, d.slots, d.origin, d.last = c.states, c.slots, c.origin[i:i + 1], c.last[i:i + 1]
             o, s = run(q38, gpu, d)
             assert torch.equal(o, out[a:a + n]) and torch.equal(s[int(c.last[i])], states[int(c.last[i])])
+
+
+@pytest.mark.parametrize("dk", [64, 128, 256])
+@pytest.mark.parametrize("dv", [64, 128, 256])
+@pytest.mark.parametrize("hk,hv", [(1, 1), (1, 2), (2, 6)])
+def test_head_sizes_of_the_long_form(gpu, q38, dk, dv, hk, hv):
+    c = DeltaCase([45, 20, 1], hk, hv, dk, dv, seed=dk + dv + hv)
+    check(c, *run(q38, gpu, c))
+
+
+@pytest.mark.parametrize("seqs,rows", [(65, 20), (64, 33), (130, 3), (200, 17)])
+def test_many_sequences(gpu, q38, seqs, rows):
+    """More sequences than a wave has lanes, some of no rows."""
+    lens = [i * 7 % (rows + 1) if i % 5 else rows for i in range(seqs)]
+    c = DeltaCase(lens, 1, 2, 64, 64, seed=seqs)
+    check(c, *run(q38, gpu, c))
+
+
+def test_most_sequences(gpu, q38):
+    """4096 sequences: as many alone in small batches, bit for bit."""
+    for max_rows in (2, 20):
+        lens = [i % 3 for i in range(4096)]
+        lens[1000] = max_rows
+        c = DeltaCase(lens, 1, 1, 64, 64, seed=13, spare=0)
+        out, states = run(q38, gpu, c)
+        for a in (0, 960, 4060):
+            d = DeltaCase(lens[a:a + 41], 1, 1, 64, 64, spare=c.slots - 82)
+            r0, r1 = int(c.off[a]), int(c.off[a + 41] if a + 41 < 4097 else c.off[-1])
+            d.qkv, d.g_log, d.beta = c.qkv[r0:r1], c.g_log[r0:r1], c.beta[r0:r1]
+            d.rows = r1 - r0
+            d.states, d.origin, d.last = c.states, c.origin[a:a + 41], c.last[a:a + 41]
+            d.off = c.off[a:a + 1 + len(d.last)] - r0
+            o, s = run(q38, gpu, d, max_rows=min(max_rows, d.rows))
+            assert torch.equal(o, out[r0:r1])
+            at = d.last.long()
+            assert torch.equal(s[at], states[at])
+
+
+def test_no_rows_copies_states(gpu, q38):
+    c = DeltaCase([0, 0, 0], 2, 4, 64, 128, seed=14)
+    c.origin[1] = -1
+    rule = q38.DeltaRule(gpu, 2, 4, 64, 128, c.scale)
+    pool = c.states.cuda()
+    batch = q38.DeltaBatch(pool, c.off.cuda(), c.origin.cuda(), c.last.cuda(), 0, 0)
+    e = lambda *s, dt=BF16: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
+    rule.run(batch, e(0, 2, 64), e(0, 2, 64), e(0, 4, 128), e(0, 4, dt=torch.float32), e(0, 4, dt=torch.float32),
+             e(0, 4, 128), None, G.stream())
+    torch.cuda.synchronize()
+    want = c.states.clone()
+    want[c.last.long()] = want[c.origin.long()]
+    want[int(c.last[1])] = 0
+    assert torch.equal(pool.cpu().nan_to_num(123.0), want.nan_to_num(123.0))
+
+
+@pytest.mark.parametrize("rows", [[2, 1], [40, 3]])
+def test_slots_beyond_32_bits(gpu, q38, rows):
+    """A pool of more than 2^31 floats whose last slots are the batch's."""
+    c = DeltaCase(rows, 8, 32, 128, 128, seed=15)
+    want_out, want = run(q38, gpu, c)
+    slots = (1 << 31) // (32 * 128 * 128) + 16
+    shift = slots - c.slots
+    pool = torch.empty(slots, 32, 128, 128, device="cuda")
+    pool[shift:] = c.states.cuda()
+    rule = q38.DeltaRule(gpu, 8, 32, 128, 128, c.scale)
+    batch = q38.DeltaBatch(pool, c.off.cuda(), c.origin.cuda() + shift, c.last.cuda() + shift, c.rows, c.max_rows)
+    out = torch.zeros(c.rows, 32, 128, dtype=BF16, device="cuda")
+    rule.run(batch, *c.operands("cuda"), out, G.workspace(max(16, rule.workspace_size(batch))), G.stream())
+    torch.cuda.synchronize()
+    assert torch.equal(out.cpu(), want_out)
+    at = c.last.long()
+    assert torch.equal(pool[shift:].cpu()[at], want[at])
+
+
+@pytest.mark.parametrize("rows", [[2], [40]])
+def test_row_offsets_beyond_32_bits(gpu, q38, rows):
+    """Operands of more than 2^31 elements whose last rows are the batch's."""
+    stride = 1 << 20
+    c = DeltaCase(rows, 2, 4, 64, 64, seed=16)
+    want_out, want = run(q38, gpu, c)
+    before = (1 << 31) // stride + 5
+    wide = torch.zeros(before + c.rows, stride, dtype=BF16, device="cuda")
+    qkv = [t.cuda() for t in c.operands("cpu")[:3]]
+    views = []
+    for i, x in enumerate(qkv):
+        v = wide[:, 4096 * i:4096 * i + x[0].numel()].unflatten(1, tuple(x.shape[1:]))
+        v[before:] = x
+        views.append(v)
+    pad = lambda t: torch.cat([torch.zeros(before, 4), t]).cuda()  # noqa: E731
+    pool = c.states.cuda()
+    rule = q38.DeltaRule(gpu, 2, 4, 64, 64, c.scale)
+    batch = q38.DeltaBatch(pool, (c.off + before).cuda(), c.origin.cuda(), c.last.cuda(), before + c.rows, c.max_rows)
+    out = torch.zeros(before + c.rows, 4, 64, dtype=BF16, device="cuda")
+    rule.run(batch, *views, pad(c.g_log), pad(c.beta), out, G.workspace(max(16, rule.workspace_size(batch))), G.stream())
+    torch.cuda.synchronize()
+    assert torch.equal(out[before:].cpu(), want_out) and (out[:before] == 0).all()
+    at = c.last.long()
+    assert torch.equal(pool.cpu()[at], want[at])
+
+
+def test_two_calls_at_once(gpu, q38):
+    """The long and the short form on two streams over one pool, other slots: the same bits as alone."""
+    jobs = []
+    for rows in ([300, 65, 129], [1, 2, 1, 7]):
+        c = DeltaCase(rows, 2, 4, 128, 128, seed=17)
+        want = run(q38, gpu, c)
+        jobs.append((c, want))
+    n = jobs[0][0].slots
+    pool = torch.cat([c.states for c, _ in jobs]).cuda()
+    calls = []
+    for i, (c, _) in enumerate(jobs):
+        rule = q38.DeltaRule(gpu, 2, 4, 128, 128, c.scale)
+        batch = q38.DeltaBatch(pool, c.off.cuda(), c.origin.cuda() + i * n, c.last.cuda() + i * n, c.rows, c.max_rows)
+        out = torch.zeros(c.rows, 4, 128, dtype=BF16, device="cuda")
+        calls.append((rule, batch, c.operands("cuda"), out, G.workspace(max(16, rule.workspace_size(batch))), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for rule, batch, ops, out, ws, st in calls:
+            rule.run(batch, *ops, out, ws, st.cuda_stream)
+    torch.cuda.synchronize()
+    for i, ((c, (o, s)), call) in enumerate(zip(jobs, calls)):
+        at = c.last.long()
+        assert torch.equal(call[3].cpu(), o) and torch.equal(pool.cpu()[at + i * n], s[at])

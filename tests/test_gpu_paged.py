@@ -70,6 +70,82 @@ def test_attention(gpu, q38, geo, lengths, q8):
     check_attend(b, cache, q, scale, run_attend(q38, gpu, b, cache, q, scale))
 
 
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 128, 129, 256, 257])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attention_rows_around_a_tile(gpu, q38, rows, dim):
+    b = Batch([rows, 1], [rows + 30, 90], hkv=1, dim=dim, seed=rows)
+    cache = b.cache(False)
+    q = b.randn(b.rows, 1, dim).to(BF16)
+    check_attend(b, cache, q, 0.1, run_attend(q38, gpu, b, cache, q, 0.1))
+
+
+@pytest.mark.parametrize("rows,tokens", [([1, 2], [300, 77]), ([5], [700])])
+@pytest.mark.parametrize("hkv,group,dim", [(1, 128, 64), (2, 128, 128), (1, 128, 256), (2, 100, 256), (64, 4, 64), (64, 1, 128),
+                                           (5, 3, 128)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_attention_many_heads(gpu, q38, rows, tokens, hkv, group, dim, q8):
+    b = Batch(rows, tokens, hkv=hkv, dim=dim, seed=hkv + group)
+    cache = b.cache(q8)
+    q = b.randn(b.rows, hkv * group, dim).to(BF16)
+    check_attend(b, cache, q, dim ** -0.5, run_attend(q38, gpu, b, cache, q, dim ** -0.5))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q8", [False, True])
+def test_long_tiles_are_cut_and_joined(gpu, q38, dim, q8):
+    """Few tiles over long contexts: every workgroup takes a part of one."""
+    b = Batch([70, 3, 41], [6000, 2500, 41], page=32, hkv=1, dim=dim, seed=dim)
+    cache = b.cache(q8)
+    q = b.randn(b.rows, 2, dim).to(BF16)
+    check_attend(b, cache, q, dim ** -0.5, run_attend(q38, gpu, b, cache, q, dim ** -0.5))
+
+
+@pytest.mark.parametrize("seqs,rows", [(65, 1), (150, 3), (4096, 1), (130, 40)])
+def test_attention_many_sequences(gpu, q38, seqs, rows):
+    """More sequences than a wave has lanes; some without rows or tokens."""
+    lens = [(i * 7 % (rows + 1)) if i % 5 else rows for i in range(seqs)]
+    tokens = [n + i * 13 % 90 for i, n in enumerate(lens)]
+    tokens[3], tokens[64] = 2000, 777
+    b = Batch(lens, tokens, hkv=1, dim=64, seed=seqs)
+    cache = b.cache(False)
+    q = b.randn(b.rows, 2, 64).to(BF16)
+    check_attend(b, cache, q, 0.125, run_attend(q38, gpu, b, cache, q, 0.125))
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_attention_scale_zero(gpu, q38, rows):
+    b = Batch([rows], [rows + 200], hkv=2, dim=64, seed=17)
+    cache = b.cache(False)
+    q = b.randn(b.rows, 8, 64).to(BF16)
+    check_attend(b, cache, q, 0.0, run_attend(q38, gpu, b, cache, q, 0.0))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_row_offsets_beyond_32_bits(gpu, q38, rows):
+    """Row tensors of more than 2^31 elements whose last rows are the batch's."""
+    hkv, hq, dim = 2, 8, 64
+    stride = 1 << 20
+    b = Batch([rows], [rows + 100], hkv=hkv, dim=dim, seed=18)
+    before = (1 << 31) // stride + 5
+    dev = [t.cuda() for t in b.cache(False)[:2]]
+    wide = torch.zeros(before + rows, stride, dtype=BF16, device="cuda")
+    w = hkv * dim
+    q, k, v = b.randn(rows, hq, dim).to(BF16), b.randn(rows, hkv, dim).to(BF16), b.randn(rows, hkv, dim).to(BF16)
+    wide[before:, :hq * dim] = q.view(rows, -1).cuda()
+    wide[before:, 4096:4096 + w] = k.view(rows, -1).cuda()
+    wide[before:, 8192:8192 + w] = v.view(rows, -1).cuda()
+    view = lambda at, heads: wide[:, at:at + heads * dim].unflatten(1, (heads, dim))  # noqa: E731
+    B = q38.PagedBatch((b.off + before).cuda(), b.tokens.cuda(), b.table.cuda(), before + rows, rows)
+    C = q38.PagedCache(gpu, *dev)
+    C.append(B, view(4096, hkv), view(8192, hkv), G.stream())
+    C.attend(B, view(0, hq), view(16384, hq), 0.1, G.workspace(max(16, C.workspace_size(B, hq))), G.stream())
+    torch.cuda.synchronize()
+    p, o = b.places(0)
+    cache = [t.cpu() for t in dev] + [None, None]
+    assert torch.equal(cache[0][p, :, o][100:], k) and torch.equal(cache[1][p, :, o][100:], v)
+    check_attend(b, cache, q, 0.1, view(16384, hq)[before:].cpu())
+
+
 @pytest.mark.parametrize("page", [32, 64, 256, 1024])
 @pytest.mark.parametrize("q8", [False, True])
 def test_attention_page_sizes(gpu, q38, page, q8):
@@ -237,6 +313,25 @@ def test_append(gpu, q38, rows, tokens, hkv, dim, q8):
             assert torch.equal(got.cpu(), w)
 
 
+def test_append_many_sequences(gpu, q38):
+    lens = [i % 3 for i in range(4096)]
+    tokens = [n + i % 20 for i, n in enumerate(lens)]
+    b = Batch(lens, tokens, hkv=2, dim=64, seed=24)
+    want = list(b.cache(False, poison=3.0)[:2])
+    dev = [t.cuda() for t in want]
+    kv = b.randn(b.rows, 2, 2, 64).to(BF16)
+    for i, n in enumerate(lens):
+        if n:
+            p, o = (t[tokens[i] - n:] for t in b.places(i))
+            for j in range(2):
+                want[j][p, :, o] = kv[int(b.off[i]):int(b.off[i]) + n, j]
+    kvd = kv.cuda()
+    q38.PagedCache(gpu, *dev).append(batch_on_gpu(q38, b), kvd[:, 0], kvd[:, 1], G.stream())
+    torch.cuda.synchronize()
+    for got, w in zip(dev, want):
+        assert torch.equal(got.cpu(), w)
+
+
 def test_append_q8_extremes(gpu, q38):
     """Zeros, ties, the largest bf16, infinities and NaN."""
     big = torch.finfo(BF16).max
@@ -352,3 +447,23 @@ def test_repeated_calls_are_bit_identical(gpu, q38):
     first = run_attend(q38, gpu, b, cache, q, 0.06)
     for _ in range(3):
         assert torch.equal(run_attend(q38, gpu, b, cache, q, 0.06), first)
+
+
+def test_two_calls_at_once(gpu, q38):
+    """Calls on two streams with a workspace each: the same bits as one after the other."""
+    jobs = []
+    for seed, rows, tokens in ((41, [1] * 6, [4000, 700, 90, 1500, 3, 2222]), (42, [90, 33], [1200, 400])):
+        b = Batch(rows, tokens, hkv=2, dim=128, seed=seed)
+        C, B = q38.PagedCache(gpu, *[t.cuda() for t in b.cache(False)[:2]]), batch_on_gpu(q38, b)
+        q = b.randn(b.rows, 16, 128).to(BF16).cuda()
+        outs = [torch.zeros_like(q) for _ in range(2)]
+        jobs.append((C, B, q, outs, G.workspace(max(16, C.workspace_size(B, 16))), torch.cuda.Stream()))
+    for C, B, q, outs, ws, _ in jobs:
+        C.attend(B, q, outs[0], 0.09, ws, G.stream())
+        torch.cuda.synchronize()
+    for _ in range(5):
+        for C, B, q, outs, ws, st in jobs:
+            C.attend(B, q, outs[1], 0.09, ws, st.cuda_stream)
+    torch.cuda.synchronize()
+    for _, _, _, outs, _, _ in jobs:
+        assert torch.equal(*outs)
