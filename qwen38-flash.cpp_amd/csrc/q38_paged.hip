@@ -237,8 +237,8 @@ struct QueryTile {
     }
 };
 
-// The running softmax of a wave's queries and its sum of the values.
-template <int D, bool Q8, int MT>
+// The running softmax of a wave's queries and its sum of the values, the probabilities in P bf16 parts.
+template <int D, bool Q8, int MT, int P>
 struct AttnState {
     using Geo = AttnGeo<D, Q8>;
     floatx4 o[MT][Geo::E];
@@ -315,7 +315,7 @@ struct AttnState {
     }
 
     __device__ __forceinline__ void scores(const KeyTile<D, Q8>& k, const QueryTile<D, Q8, MT>& q, float c, int base,
-                                           bool masked, int lane, const floatx4 (&vs)[2], uintx4 (&b)[MT]) {
+                                           bool masked, int lane, const floatx4 (&vs)[2], uintx4 (&b)[MT][P]) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             floatx4 s[2];
@@ -339,14 +339,16 @@ struct AttnState {
             }
             float p[8];
             soften(m, s, k.s, c, base, masked, lane, p);
-            b[m] = weights(m, p, vs, base, lane);
+            weights(m, p, vs, base, lane, b[m]);
         }
     }
 
-    // O^T += V^T P^T; the probabilities, at most 1, are rounded to bf16 for it (with the value's
-    // scale in a Q8 cache): half a step of each against the value it multiplies, as the output's
-    // own rounding.
-    __device__ __forceinline__ uintx4 weights(int m, const float (&p)[8], const floatx4 (&vs)[2], int base, int lane) {
+    // O^T += V^T P^T; the probabilities (with the value's scale in a Q8 cache) are rounded to P bf16 parts
+    // for it. One: each is off by up to 2^-8 of itself, as the output by its own rounding (k_paged_tile, which
+    // a second set of products would slow down by a third). Two: by 2^-17 (k_paged_split, bound by bytes: at
+    // most 2.5% of its time).
+    __device__ __forceinline__ void weights(int m, const float (&p)[8], const floatx4 (&vs)[2], int base, int lane,
+                                            uintx4 (&b)[P]) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -354,14 +356,22 @@ struct AttnState {
             // (an unseen token's scale may be anything)
             if constexpr (Q8) x[j] = base + 8 * (lane >> 4) + j < lim[m] ? x[j] * vs[j >> 2][j & 3] : 0.0f;
         }
-        return (uintx4){pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+#pragma unroll
+        for (int n = 0; n < P; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                b[n][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+                if (n + 1 < P) x[2 * i] -= bflo(b[n][i]), x[2 * i + 1] -= bfhi(b[n][i]);
+            }
     }
     template <bool CODES>  // the values as 8-bit codes, not as bf16
-    __device__ __forceinline__ void products(const ValueTile<D, CODES>& t, const uintx4 (&b)[MT]) {
+    __device__ __forceinline__ void products(const ValueTile<D, CODES>& t, const uintx4 (&b)[MT][P]) {
         if constexpr (!Q8) {
             constexpr uint32_t one = 0x3f803f80u;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) all[m] = mfma((uintx4){one, one, one, one}, b[m], all[m]);
+            for (int n = 0; n < P; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) all[m] = mfma((uintx4){one, one, one, one}, b[m][n], all[m]);
         }
 #pragma unroll
         for (int o_ = 0; o_ < Geo::E; ++o_) {
@@ -375,7 +385,9 @@ struct AttnState {
                                                  o_ & 1 ? 0x07060302u : 0x05040100u);
             }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) o[m][o_] = mfma(a, b[m], o[m][o_]);
+            for (int n = 0; n < P; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) o[m][o_] = mfma(a, b[m][n], o[m][o_]);
             // (an operand or two at a time: formed all at once they would take the tile's size again)
             if (o_ & 1) __builtin_amdgcn_sched_barrier(0);
         }
@@ -547,7 +559,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         // tokens that every query of the tile sees: steps below need no mask
         const int all = attn_see(it, it.tile * S.rows());
         QueryTile<D, Q8, MT> qt;
-        AttnState<D, Q8, MT> st;
+        AttnState<D, Q8, MT, 2> st;
         qt.load(q, qs, it, S, head, 0, c < 0.0f, lane);
         st.clear(it, S, 0, lane);
         KeyTile<D, Q8> kt;
@@ -564,7 +576,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
         }
         for (; base < stop; base += kSplitTokens) {
             const bool more = base + kSplitTokens < stop, masked = base + 32 > all;
-            uintx4 b[MT];
+            uintx4 b[MT][2];
             st.scores(kt, qt, fabsf(c), base, masked, lane, vt.s, b);
             if (more) load_keys<D, Q8>(C, at, lane, kt);
             if constexpr (!Q8)
@@ -692,7 +704,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
         const int u = lane & 15, w = lane >> 4;
         AttnItem it = sw.item(S);
         QueryTile<D, false, MT> qt;
-        AttnState<D, Q8, MT> st;
+        AttnState<D, Q8, MT, 1> st;
         qt.load(q, qs, it, S, head, m0, negate, lane);
         st.clear(it, S, m0, lane);
         // tokens that all, and any, of the wave's queries see (a wave without queries has nothing to mask)
@@ -803,12 +815,12 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
                     ks[a] = *reinterpret_cast<const floatx4*>(sc + 32 * sub + 8 * w + 4 * a);
                     vs[a] = *reinterpret_cast<const floatx4*>(sc + TB + 32 * sub + 8 * w + 4 * a);
                 }
-            uintx4 b[MT];
+            uintx4 b[MT][1];
     #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float p[8];
                 st.soften(m, s[m], ks, c, base, masked, lane, p);
-                b[m] = st.weights(m, p, vs, base, lane);
+                st.weights(m, p, vs, base, lane, b[m]);
             }
             if constexpr (D == 256) read_values();
             if constexpr (!Q8)
@@ -885,16 +897,21 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
 }
 
 // Joins the pieces of the items that the shares' ends cut: a workgroup per (share that an item goes on
-// from, kv head, QB of the tile's queries), a wave per query, PB pieces in flight: few long tiles for
-// prompts (19 us for five), many pieces of one request's few queries (6.5 us for 4,001 tokens).
-template <int D, int QB, int PB>
+// from, kv head, QB of the tile's queries), WQ waves per query, each with every WQ-th run of PB pieces in
+// flight. Bound by the latency of its rounds. Prompts cut many queries into few pieces: a wave per query
+// (five prompts: 19 us). Long contexts cut few queries into many: four waves per query (three contexts of
+// up to 131,072 tokens 6.1 us, a wave per query 12.9; one of 4,001 3.8 us and 6.1).
+template <int D, int WQ, int QB, int PB>
 __global__ __launch_bounds__(256) void k_paged_join(AttnSplit S, int W, const float* __restrict__ part,
                                                     const CutItem* __restrict__ cuts, uint16_t* __restrict__ out,
                                                     int64_t os) {
+    static_assert(WQ == 1 || (WQ == 4 && QB == 1), "waves of a query meet once");
     constexpr int E = D / 64;
     typedef float vec_t __attribute__((ext_vector_type(E)));
+    __shared__ vec_t sums[WQ][64];
+    __shared__ float2 stats[WQ];
     const int lane = threadIdx.x & 63, head = blockIdx.y, G = S.G, M = S.M;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), place = head * W + blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), place = head * W + blockIdx.x, turn = wave % WQ;
     const CutItem cut = cuts[place];
     const int n = __builtin_amdgcn_readfirstlane(cut.pieces);
     if (n == 0) return;
@@ -907,13 +924,13 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnSplit S, int W, const fl
     // (it is the second slot of its first share and the first of the others)
     const float* first = part + (static_cast<int64_t>(place) * 2 + 1) * (M * (D + 2));
     auto piece = [&](int i) { return first + static_cast<int64_t>(2 * i - (i > 0)) * (M * (D + 2)); };
-#pragma unroll 2
-    for (int j = wave; j < QB; j += 4) {
+#pragma unroll(WQ > 1 ? 1 : 2)
+    for (int j = wave / WQ; j < QB; j += 4 / WQ) {
         const int i = blockIdx.z * QB + j, row = tile_row(S, it, i);
-        if (row < 0) continue;
+        if (WQ == 1 && row < 0) continue;
         float top = -INFINITY, sum = 0.0f;
         vec_t o = {};
-        for (int p0 = 0; p0 < n; p0 += PB) {
+        for (int p0 = turn * PB; p0 < n && row >= 0; p0 += WQ * PB) {
             float t[PB], l[PB], now = top;
             vec_t x[PB];
 #pragma unroll
@@ -935,6 +952,23 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnSplit S, int W, const fl
                 const float f = p0 + p < n ? __builtin_amdgcn_exp2f(t[p] - ref) : 0.0f;
                 sum = p0 + p < n ? fmaf(l[p], f, sum) : sum;
                 o = p0 + p < n ? o + x[p] * f : o;
+            }
+        }
+        if constexpr (WQ > 1) {
+            sums[wave][lane] = o;
+            if (lane == 0) stats[wave] = make_float2(top, sum);
+            __syncthreads();
+            if (turn || row < 0) return;
+#pragma unroll
+            for (int k = 1; k < WQ; ++k) top = fmaxf(top, stats[k].x);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            sum = 0.0f;
+            o = vec_t{};
+#pragma unroll
+            for (int k = 0; k < WQ; ++k) {
+                const float f = __builtin_amdgcn_exp2f(stats[k].x - ref);
+                sum = fmaf(stats[k].y, f, sum);
+                o += sums[k][lane] * f;
             }
         }
         const float inv = it.bad || attn_see(it, row) > 0 ? 1.0f / sum : 0.0f;
@@ -1007,9 +1041,8 @@ hipError_t launch_attention(const PagedCacheDev& C, const PagedBatchDev& B, cons
     if (e != hipSuccess || !p.joined) return e;
     const AttnSplit S{hq / C.hkv, p.M, kSplitTokens};
     if (p.tiles)
-        return launch(k_paged_join<D, 32, 2>, dim3(p.W - 1, C.hkv, p.M / 32), dim3(256), 0, st, S, p.W, part, cuts,
-                      out, os);
-    return launch(k_paged_join<D, 4, 16>, dim3(p.W - 1, C.hkv, p.M / 4), dim3(256), 0, st, S, p.W, part, cuts, out, os);
+        return launch(k_paged_join<D, 1, 32, 2>, dim3(p.W - 1, C.hkv, p.M / 32), dim3(256), 0, st, S, p.W, part, cuts, out, os);
+    return launch(k_paged_join<D, 4, 1, 8>, dim3(p.W - 1, C.hkv, p.M), dim3(256), 0, st, S, p.W, part, cuts, out, os);
 }
 
 } // namespace
