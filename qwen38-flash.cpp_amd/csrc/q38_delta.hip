@@ -404,21 +404,21 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 // The walk. A state wave holds 16 value columns of a head's state, transposed: S^T tile o (o < E =
 // DK / 16) has key dim E (4 w + r) + o in its result row 4 w + r and the value dim in its column. Lane
 // (u, w) thus holds key dims 4 E w .. 4 E (w + 1) - 1 of value dim u, eight of them in a row being an
-// operand of S k and S q with keys and queries read as stored, and the update's operand, K^T, is formed
-// from 16-byte runs of eight keys by byte permutes: no value moves between lanes. A sequence is one chain
-// of chunks per head, and a wave issues an instruction every four cycles at best, so what the chain does
-// not need is left to a second wave on another SIMD: an output wave per state wave takes the operands
-// of S and U through LDS a chunk later, and loads and stages the keys. A prompt of 4,001 rows: 160 us,
-// 1.27 us a chunk, bound by the state wave's own instructions (one wave doing all: 240 us); eight ragged
-// prompts, 16,192 rows: 345 us, two workgroups per CU, bound by the longest chains and by the systems,
-// which every group of 32 value dims reads.
+// operand of S k and S q with keys and queries read as stored: no value moves between lanes. A sequence is
+// one chain of chunks per head, and a wave issues an instruction every four cycles at best, so what the chain
+// does not need is left to a second wave on another SIMD: an output wave per state wave takes the operands of
+// S and U through LDS a chunk later, loads the keys and values and stages them as the state wave wants them
+// (the keys as stored and, pairs of rows interleaved, as operands of K^T). A prompt of 4,001 rows: 153 us, 1.2
+// us a chunk, bound by the state wave's own 400 instructions (one wave doing all: 240 us). Eight ragged
+// prompts, 16,192 rows, two workgroups per CU: 345 us, 2.0 to 2.9 us a chunk: a SIMD's matrix products (74 a
+// chunk) and vector instructions (some 420) take each other's time.
 template <int DK>
 struct WalkGeo {
     static constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8;
     static constexpr int NW = 2;                              // state waves of a workgroup, and output waves
-    static constexpr int PC = kChunk * CH / (64 * NW);        // 16-byte pieces of the keys per output thread
+    static constexpr int PC = kChunk * CH / (64 * NW);        // an output thread's rows of the keys, 16 bytes of each
     static constexpr int kKeys = kChunk * CH, kParts = NW * KS * 2 * 64, kUpd = NW * 2 * 64;
-    static constexpr size_t kLds = 2 * 16 * static_cast<size_t>(kKeys + kParts + kUpd);
+    static constexpr size_t kLds = 2 * 16 * static_cast<size_t>(2 * kKeys + kParts + kUpd);
 };
 
 template <int DK>
@@ -426,10 +426,11 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                                                                            const ChunkSystem* __restrict__ sys, int bound) {
     using Geo = WalkGeo<DK>;
     constexpr int E = Geo::E, KS = Geo::KS, CH = Geo::CH, NW = Geo::NW, PC = Geo::PC, KB = KS < 4 ? KS : 4;
-    extern __shared__ uintx4 walk_lds[];  // [2] of: keys, the state's parts, U
+    extern __shared__ uintx4 walk_lds[];  // [2] of: keys, K^T's operands, the state's parts, V and then U
     uintx4* const keys_lds = walk_lds;
-    uintx4* const parts_lds = walk_lds + 2 * Geo::kKeys;
-    floatx4* const upd_lds = reinterpret_cast<floatx4*>(walk_lds + 2 * (Geo::kKeys + Geo::kParts));
+    uintx4* const turned_lds = walk_lds + 2 * Geo::kKeys;
+    uintx4* const parts_lds = walk_lds + 4 * Geo::kKeys;
+    floatx4* const upd_lds = reinterpret_cast<floatx4*>(walk_lds + 2 * (2 * Geo::kKeys + Geo::kParts));
     const int lane = threadIdx.x & 63, u = lane & 15, w = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pair = wave % NW;
@@ -451,36 +452,67 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     auto system = [&](int n) -> const ChunkSystem& { return sys0[static_cast<size_t>(min(n, chunks - 1)) * D.hv]; };
     // keys: swizzled for reads down chunk_row()'s rows
     auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
+    // V and U: rows 8 w + 4 a .. of column u in a slot of their own, so that the writes of V, down the columns,
+    // get banks of their own
+    auto slot = [&](int column, int block, int a) { return (64 * a + 16 * block + (column ^ (2 * block + a))); };
     // Loads of a next chunk are made always, of the last one's again behind it, and their number is the same
     // on every path, so that a wait counts only the loads that it needs. Rows behind the sequence: its last
     // row again, whose update is nothing (its beta in the system is 0).
 
     if (outputs) {
         const char* const kb = reinterpret_cast<const char*>(D.k + begin * D.ks + hk * DK);
+        const char* const vb = reinterpret_cast<const char*>(D.v + begin * D.vs + h * D.dv + dv);
         const char* const qb = reinterpret_cast<const char*>(D.q + begin * D.qs + hk * DK);
         char* const ob = reinterpret_cast<char*>(D.out + (static_cast<size_t>(begin) * D.hv + h) * D.dv + dv);
         const int tid = pair * 64 + lane;
-        uintx4 kr[PC], qr[KS][2], mop[2][2];
+        uintx4 kr[PC], vr, qr[KS][2], mop[2][2];
         float eg[2];
+        // 16 bytes of a chunk's row: a uniform address and a lane's 32-bit offset (strides are below 2^24)
+        auto fetch = [&](const char* base, int64_t stride, int chunk, int row, int at) {
+            const char* from = base + 2 * (static_cast<int64_t>(chunk) * kChunk * stride);
+            const uint32_t r = min(row, length - 1 - chunk * kChunk);
+            return *reinterpret_cast<const uintx4*>(from + 2 * (__umul24(r, static_cast<uint32_t>(stride)) + at));
+        };
         auto fetch_keys = [&](int chunk) {
 #pragma unroll
-            for (int i = 0; i < PC; ++i) {
-                const int64_t row = min(chunk * kChunk + tid / CH + i * (64 * NW / CH), length - 1);
-                kr[i] = *reinterpret_cast<const uintx4*>(kb + 2 * row * D.ks + 16 * (tid % CH));
-            }
+            for (int i = 0; i < PC; ++i) kr[i] = fetch(kb, D.ks, chunk, tid / CH * PC + i, 8 * (tid % CH));
+            vr = fetch(vb, D.vs, chunk, lane / 2, 8 * (lane & 1));
         };
         auto stage_keys = [&](int buf) {
+            const int r0 = tid / CH * PC;
 #pragma unroll
-            for (int i = 0; i < PC; ++i) keys_lds[buf * Geo::kKeys + key_at(tid / CH + i * (64 * NW / CH), tid % CH)] = kr[i];
+            for (int i = 0; i < PC; ++i) keys_lds[buf * Geo::kKeys + key_at(r0 + i, tid % CH)] = kr[i];
+            // operand o of K^T: dim E u + o of rows 8 w ..
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = 8 * (tid % CH) + e;
+                typedef uint32_t pairs_t __attribute__((ext_vector_type(PC / 2)));
+                uint32_t x[PC / 2];
+#pragma unroll
+                for (int j = 0; j < PC / 2; ++j)
+                    x[j] = __builtin_amdgcn_perm(kr[2 * j + 1][e >> 1], kr[2 * j][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                uintx4* const at = turned_lds + buf * Geo::kKeys + d % E * 64 + r0 / 8 * 16 + d / E;
+                uint32_t* const to = reinterpret_cast<uint32_t*>(at) + r0 % 8 / 2;
+                if constexpr (PC == 2) {
+                    *to = x[0];
+                } else {
+                    pairs_t all;
+#pragma unroll
+                    for (int j = 0; j < PC / 2; ++j) all[j] = x[j];
+                    *reinterpret_cast<pairs_t*>(to) = all;
+                }
+            }
+            const int row = lane / 2;
+            float* to = reinterpret_cast<float*>(upd_lds + buf * Geo::kUpd + pair * 2 * 64) + (row & 3);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                to[4 * slot(8 * (lane & 1) + i, row >> 3, row >> 2 & 1)] = i & 1 ? bfhi(vr[i >> 1]) : bflo(vr[i >> 1]);
         };
         auto fetch_queries = [&](int chunk) {  // operands: row 16 a + u, dims 4 E w + 8 k ..
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int64_t row = min(chunk * kChunk + 16 * a + u, length - 1);
+            for (int a = 0; a < 2; ++a)
 #pragma unroll
-                for (int k = 0; k < KS; ++k)
-                    qr[k][a] = *reinterpret_cast<const uintx4*>(qb + 2 * row * D.qs + 16 * (KS * w + k));
-            }
+                for (int k = 0; k < KS; ++k) qr[k][a] = fetch(qb, D.qs, chunk, 16 * a + u, 8 * (KS * w + k));
         };
         auto fetch_scores = [&](const ChunkSystem& cs) {
 #pragma unroll
@@ -501,7 +533,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
             fetch_keys(min(n + 1, chunks - 1));
             if (n > 0) {
                 const uintx4* parts = parts_lds + ((n - 1) & 1) * Geo::kParts + pair * KS * 2 * 64 + lane;
-                const floatx4* upd = upd_lds + ((n - 1) & 1) * Geo::kUpd + pair * 2 * 64 + lane;
+                const floatx4* upd = upd_lds + ((n - 1) & 1) * Geo::kUpd + pair * 2 * 64;
                 // O^T = exp(G) S q + U^T M^T, transposed: value dims by chunk rows
                 floatx4 ot[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -510,7 +542,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                     for (int p = 1; p >= 0; --p)
 #pragma unroll
                         for (int a = 0; a < 2; ++a) ot[a] = mfma(parts[(k * 2 + p) * 64], qr[k][a], ot[a]);
-                const floatx4 un[2] = {upd[0], upd[64]};
+                const floatx4 un[2] = {upd[slot(u, w, 0)], upd[slot(u, w, 1)]};
                 Parts<2> up;
                 {
                     float x[8];
@@ -524,7 +556,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                 for (int p = 1; p >= 0; --p)
 #pragma unroll
                     for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[p], mop[0][a], ot[a]);
-                fetch_queries(n);
+                fetch_queries(min(n, chunks - 1));
                 fetch_scores(system(n));
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
@@ -557,22 +589,6 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
 #pragma unroll
             for (int e = 0; e < 4; ++e) st[o + e][r] = x[e];
         }
-    const char* const vb = reinterpret_cast<const char*>(D.v + begin * D.vs + h * D.dv + dv);
-    const uint32_t vo = 2 * (8 * w * static_cast<uint32_t>(D.vs) + u);
-    uint16_t vr[8];
-    auto fetch_v = [&](int chunk) {
-        if ((chunk + 1) * kChunk <= length) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                vr[j] = *reinterpret_cast<const uint16_t*>(vb + 2 * static_cast<int64_t>(chunk * kChunk + j) * D.vs + vo);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t row = min(chunk * kChunk + 8 * w + j, length - 1);
-                vr[j] = *reinterpret_cast<const uint16_t*>(vb + 2 * row * D.vs + 2 * u);
-            }
-        }
-    };
     // a chunk's system in registers, every part loaded anew as soon as its chunk is done with it
     uintx4 top[3][2];
     floatx4 into[2], left[2];
@@ -593,7 +609,6 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         whole = cs.into[kChunk - 1];
     };
     if (chunks > 0) {
-        fetch_v(0);
         load_into(system(0));
         load_t(system(0));
         load_left(system(0));
@@ -601,8 +616,9 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     lds_barrier();
     for (int n = 0; n < chunks; ++n) {
         const uintx4* kt = keys_lds + (n & 1) * Geo::kKeys;
+        const uintx4* turned = turned_lds + (n & 1) * Geo::kKeys + lane;
         uintx4* parts = parts_lds + (n & 1) * Geo::kParts + pair * KS * 2 * 64 + lane;
-        floatx4* upd = upd_lds + (n & 1) * Geo::kUpd + pair * 2 * 64 + lane;
+        floatx4* upd = upd_lds + (n & 1) * Geo::kUpd + pair * 2 * 64;
         const ChunkSystem& next = system(n + 1);
         // P = K S^T (chunk rows by value dims)
         floatx4 pr[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -630,22 +646,12 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        // K^T's rows and the state's decay, beside the products' end
-        uint32_t kv[8][E / 2];
+        // V, K^T and the state's decay, beside the products' end
+        const floatx4 vv[2] = {upd[slot(u, w, 0)], upd[slot(u, w, 1)]};
+        constexpr int KT = E < 8 ? E : 8;
+        uintx4 kv[KT];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (E == 4) {
-                const uint2 x = reinterpret_cast<const uint2*>(kt + key_at(8 * w + j, u >> 1))[u & 1];
-                kv[j][0] = x.x, kv[j][1] = x.y;
-            } else {
-#pragma unroll
-                for (int b = 0; b < E / 8; ++b) {
-                    const uintx4 x = kt[key_at(8 * w + j, E / 8 * u + b)];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) kv[j][4 * b + i] = x[i];
-                }
-            }
-        }
+        for (int o = 0; o < KT; ++o) kv[o] = turned[o * 64];
 #pragma unroll
         for (int o = 0; o < E; ++o) st[o] *= whole;
         // U = T diag(beta) Y, Y = V - exp(G) P (chains of products that add to one result wait for each
@@ -654,10 +660,9 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         {
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = bf2f(vr[j]) - into[j >> 2][j & 3] * pr[j >> 2][j & 3];
+            for (int j = 0; j < 8; ++j) y[j] = vv[j >> 2][j & 3] - into[j >> 2][j & 3] * pr[j >> 2][j & 3];
             yp.split(y);
         }
-        fetch_v(n + 1);
         load_into(next);
         floatx4 un[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -675,21 +680,16 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
             for (int j = 0; j < 8; ++j) z[j] = left[j >> 2][j & 3] * un[j >> 2][j & 3];
             zp.split(z);
         }
-        upd[0] = un[0];
-        upd[64] = un[1];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) upd[slot(u, w, a)] = un[a];
         load_left(next);
 #pragma unroll
         for (int o = 0; o < E; o += 2) {
-            uintx4 a[2];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                a[0][j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], 0x05040100u);
-                a[1][j] = __builtin_amdgcn_perm(kv[2 * j + 1][o >> 1], kv[2 * j][o >> 1], 0x07060302u);
-            }
 #pragma unroll
             for (int p = 2; p >= 0; --p)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) st[o + i] = mfma(a[i], zp.p[p], st[o + i]);
+                for (int i = 0; i < 2; ++i) st[o + i] = mfma(kv[(o + i) % KT], zp.p[p], st[o + i]);
+            if (o + KT < E) kv[o] = turned[(o + KT) * 64], kv[o + 1] = turned[(o + 1 + KT) * 64];
         }
         lds_barrier();  // (the next chunk's loads stay in flight)
     }
