@@ -408,7 +408,7 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 // one chain of chunks per head, and a wave issues an instruction every four cycles at best, so what the chain
 // does not need is left to a second wave on another SIMD: an output wave per state wave takes the operands of
 // S and U through LDS a chunk later, loads the keys and values and stages them as the state wave wants them
-// (the keys as stored and, pairs of rows interleaved, as operands of K^T). A prompt of 4,001 rows: 153 us, 1.2
+// (the keys as stored and, pairs of rows interleaved, as operands of K^T). A prompt of 4,001 rows: 149 us, 1.2
 // us a chunk, bound by the state wave's own 400 instructions (one wave doing all: 240 us). Eight ragged
 // prompts, 16,192 rows, two workgroups per CU: 345 us, 2.0 to 2.9 us a chunk: a SIMD's matrix products (74 a
 // chunk) and vector instructions (some 420) take each other's time.
@@ -467,16 +467,14 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         const int tid = pair * 64 + lane;
         uintx4 kr[PC], vr, qr[KS][2], mop[2][2];
         float eg[2];
-        // 16 bytes of a chunk's row: a uniform address and a lane's 32-bit offset (strides are below 2^24)
-        auto fetch = [&](const char* base, int64_t stride, int chunk, int row, int at) {
-            const char* from = base + 2 * (static_cast<int64_t>(chunk) * kChunk * stride);
-            const uint32_t r = min(row, length - 1 - chunk * kChunk);
-            return *reinterpret_cast<const uintx4*>(from + 2 * (__umul24(r, static_cast<uint32_t>(stride)) + at));
-        };
         auto fetch_keys = [&](int chunk) {
 #pragma unroll
-            for (int i = 0; i < PC; ++i) kr[i] = fetch(kb, D.ks, chunk, tid / CH * PC + i, 8 * (tid % CH));
-            vr = fetch(vb, D.vs, chunk, lane / 2, 8 * (lane & 1));
+            for (int i = 0; i < PC; ++i) {
+                const int64_t row = min(chunk * kChunk + tid / CH * PC + i, length - 1);
+                kr[i] = *reinterpret_cast<const uintx4*>(kb + 2 * row * D.ks + 16 * (tid % CH));
+            }
+            const int64_t row = min(chunk * kChunk + lane / 2, length - 1);
+            vr = *reinterpret_cast<const uintx4*>(vb + 2 * (row * D.vs + 8 * (lane & 1)));
         };
         auto stage_keys = [&](int buf) {
             const int r0 = tid / CH * PC;
@@ -510,9 +508,12 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         };
         auto fetch_queries = [&](int chunk) {  // operands: row 16 a + u, dims 4 E w + 8 k ..
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int a = 0; a < 2; ++a) {
+                const int64_t row = min(chunk * kChunk + 16 * a + u, length - 1);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) qr[k][a] = fetch(qb, D.qs, chunk, 16 * a + u, 8 * (KS * w + k));
+                for (int k = 0; k < KS; ++k)
+                    qr[k][a] = *reinterpret_cast<const uintx4*>(qb + 2 * row * D.qs + 16 * (KS * w + k));
+            }
         };
         auto fetch_scores = [&](const ChunkSystem& cs) {
 #pragma unroll
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                 for (int p = 1; p >= 0; --p)
 #pragma unroll
                     for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[p], mop[0][a], ot[a]);
-                fetch_queries(min(n, chunks - 1));
+                fetch_queries(n);
                 fetch_scores(system(n));
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
@@ -646,12 +647,14 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        // V, K^T and the state's decay, beside the products' end
+        // V, K^T and the state's decay, beside the products' end (the reads first: left to the compiler some
+        // came after the sums that need them, 2% of the walk)
         const floatx4 vv[2] = {upd[slot(u, w, 0)], upd[slot(u, w, 1)]};
         constexpr int KT = E < 8 ? E : 8;
         uintx4 kv[KT];
 #pragma unroll
         for (int o = 0; o < KT; ++o) kv[o] = turned[o * 64];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int o = 0; o < E; ++o) st[o] *= whole;
         // U = T diag(beta) Y, Y = V - exp(G) P (chains of products that add to one result wait for each
@@ -704,10 +707,13 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                 (floatx4){st[o][r], st[o + 1][r], st[o + 2][r], st[o + 3][r]};
 }
 
-// Sequences of up to so many rows go row by row. 16 rows of 32 heads, by rows and in chunks: one sequence
-// 17.4 and 18.4 us, eight 22.5 and 25.8, 64 117 and 130; 24 rows: 20.7 and 18.4, 29.3 and 25.8, 157 and 130.
-constexpr int kRowsForm = 16;
-bool by_rows(const DeltaBatchDev& B, int max_rows) { return B.ckpt || B.rows == 0 || max_rows <= kRowsForm; }
+// Sequences of up to so many rows go row by row. By rows and in chunks, 32 heads [128][128]: one sequence of
+// 24 rows 20.3 and 15.0 us, eight 29.6 and 28.9; 64 of 24 rows 158 and 170, of 32 rows 201 and 176 (16 heads
+// [256][256]: 321 and 379, 418 and 389; 8 heads [64][64]: 19.3 and 24.9, 24.0 and 25.5). 16 rows: within 1 us
+// of each other for one sequence and eight.
+bool by_rows(const DeltaBatchDev& B, int max_rows) {
+    return B.ckpt || B.rows == 0 || max_rows <= (B.seqs < 32 ? 16 : 28);
+}
 int chunk_bound(const DeltaBatchDev& B) { return B.rows / kChunk + (B.seqs < B.rows ? B.seqs : B.rows); }
 
 template <int DK>

@@ -223,7 +223,7 @@ def test_head_sizes_of_the_long_form(gpu, q38, dk, dv, hk, hv):
     check(c, *run(q38, gpu, c))
 
 
-@pytest.mark.parametrize("seqs,rows", [(65, 20), (64, 33), (130, 3), (200, 17)])
+@pytest.mark.parametrize("seqs,rows", [(65, 20), (64, 33), (130, 3), (200, 17), (65, 30), (130, 29), (31, 17), (32, 28)])
 def test_many_sequences(gpu, q38, seqs, rows):
     """More sequences than a wave has lanes, some of no rows."""
     lens = [i * 7 % (rows + 1) if i % 5 else rows for i in range(seqs)]
@@ -233,7 +233,7 @@ def test_many_sequences(gpu, q38, seqs, rows):
 
 def test_most_sequences(gpu, q38):
     """4096 sequences: as many alone in small batches, bit for bit."""
-    for max_rows in (2, 20):
+    for max_rows in (2, 20, 40):
         lens = [i % 3 for i in range(4096)]
         lens[1000] = max_rows
         c = DeltaCase(lens, 1, 1, 64, 64, seed=13, spare=0)
