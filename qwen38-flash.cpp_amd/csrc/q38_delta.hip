@@ -709,8 +709,8 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
 
 // Sequences of up to so many rows go row by row. By rows and in chunks, 32 heads [128][128]: one sequence of
 // 24 rows 20.3 and 15.0 us, eight 29.6 and 28.9; 64 of 24 rows 158 and 170, of 32 rows 201 and 176 (16 heads
-// [256][256]: 321 and 379, 418 and 389; 8 heads [64][64]: 19.3 and 24.9, 24.0 and 25.5). 16 rows: within 1 us
-// of each other for one sequence and eight.
+// [256][256]: 321 and 379, 418 and 389; 8 heads [64][64]: 19.3 and 24.9, 24.0 and 25.5). 16 rows by rows: 15.1,
+// 22.5 and 119.
 bool by_rows(const DeltaBatchDev& B, int max_rows) {
     return B.ckpt || B.rows == 0 || max_rows <= (B.seqs < 32 ? 16 : 28);
 }

@@ -443,36 +443,64 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {  // a value that every l
     const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32));
     return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-// The list's length and a share's size, and the item that holds step w * share (if the list is that
-// long). Every wave finds it by itself, 64 sequences a round (a scan over the workgroup took two barriers
-// and 2 us of the smallest calls); up to 64 sequences are weighed once.
+// (the 64-bit division's steps are worth avoiding in the smallest calls)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
+// The list's length and a share's size, and the item that holds step w * share with its sequence (if the
+// list is that long). Every wave finds it by itself, 64 sequences a round, from one load of their lengths (a
+// scan over the workgroup took two barriers and 2 us of the smallest calls); up to 64 sequences are weighed
+// once.
 __device__ __forceinline__ int64_t find_share(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t w, int64_t W,
-                                              AttnCursor* at, int64_t* share) {
+                                              AttnCursor* at, AttnItem* seq, int64_t* share) {
     const int lane = threadIdx.x & 63;
-    auto weight = [&](int s) { return s < B.seqs ? attn_weight(S, B, shift, s) : 0; };
-    int64_t mine = 0, sum = 0;
-    for (int s0 = 0; s0 < B.seqs; s0 += 64) sum += mine = weight(s0 + lane);
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
-    sum = uniform(sum);
-    *share = (sum + W - 1) / W;
-    const int64_t want = w * *share;
-    int64_t before = 0;
-    for (int s0 = 0; s0 < B.seqs && want < sum; s0 += 64) {
-        if (B.seqs > 64) mine = weight(s0 + lane);
-        int64_t upto = mine;
+    AttnItem it;
+    int64_t mine = 0, upto = 0, sum = 0;
+    auto weigh = [&](int s) {
+        mine = 0;
+        if (s < B.seqs) {
+            attn_sequence(B, shift, s, &it);
+            mine = attn_weight(S, it);
+        }
+    };
+    auto scan = [&] {
+        upto = mine;
         for (int d = 1; d < 64; d <<= 1) {
             const int64_t x = __shfl_up(upto, d);
             if (lane >= d) upto += x;
         }
+        return uniform(__shfl(upto, 63));
+    };
+    if (B.seqs <= 64) {
+        weigh(lane);
+        sum = scan();
+    } else {
+        for (int s0 = 0; s0 < B.seqs; s0 += 64) weigh(s0 + lane), sum += mine;
+        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+        sum = uniform(sum);
+    }
+    *share = quotient(sum + W - 1, W);
+    const int64_t want = w * *share;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < B.seqs && want < sum; s0 += 64) {
+        int64_t these = sum;
+        if (B.seqs > 64) {
+            weigh(s0 + lane);
+            these = scan();
+        }
         const uint64_t past = __ballot(before + upto > want);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const AttnCursor c = attn_seek(S, B, shift, __builtin_amdgcn_readfirstlane(s0 + l),
-                                           before + uniform(__shfl(upto - mine, l)), want);
+            seq->seq = __builtin_amdgcn_readfirstlane(s0 + l);
+            seq->first = __builtin_amdgcn_readlane(it.first, l);
+            seq->rows = __builtin_amdgcn_readlane(it.rows, l);
+            seq->tokens = __builtin_amdgcn_readlane(it.tokens, l);
+            seq->bad = __builtin_amdgcn_readlane(it.bad, l);
+            const AttnCursor c = attn_seek(S, *seq, before + uniform(__shfl(upto - mine, l)), want);
             *at = AttnCursor{c.seq, __builtin_amdgcn_readfirstlane(c.tile), uniform(c.start)};
             break;
         }
-        before += uniform(__shfl(upto, 63));
+        before += these;
     }
     return sum;
 }
@@ -486,10 +514,14 @@ struct ShareWalk {
     // false where the share is empty
     __device__ __forceinline__ bool open(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t w, int64_t W) {
         AttnCursor c{0, 0, 0};
+        AttnItem it;
         int64_t sh = 0;
-        const int64_t total = find_share(S, B, shift, w, W, &c, &sh);
+        const int64_t total = find_share(S, B, shift, w, W, &c, &it, &sh);
         if (w * sh >= total) return false;
-        if ((threadIdx.x & 63) == 0) at = c, share = sh, pos = w * sh, end = min(total, (w + 1) * sh);
+        if ((threadIdx.x & 63) == 0) {
+            at = c, share = sh, pos = w * sh, end = min(total, (w + 1) * sh);
+            seq_ = it.seq, first = it.first, rows = it.rows, tokens = it.tokens, bad = it.bad;
+        }
         return true;
     }
     // The next piece; the same for all lanes.
@@ -497,6 +529,7 @@ struct ShareWalk {
         AttnCursor c{__builtin_amdgcn_readfirstlane(at.seq), __builtin_amdgcn_readfirstlane(at.tile), uniform(at.start)};
         int64_t p = uniform(pos);
         AttnPiece pc;
+        pc.it = sequence();
         if (!attn_next(S, B, shift, uniform(end), &c, &p, &pc)) return false;
         if ((threadIdx.x & 63) == 0) {
             at = c, pos = p, start = pc.start, seq_ = pc.it.seq;
@@ -505,13 +538,17 @@ struct ShareWalk {
         }
         return true;
     }
-    __device__ __forceinline__ AttnItem item(const AttnSplit& S) const {
+    __device__ __forceinline__ AttnItem sequence() const {
         AttnItem it;
-        it.seq = 0;
+        it.seq = seq();
         it.first = __builtin_amdgcn_readfirstlane(first);
         it.rows = __builtin_amdgcn_readfirstlane(rows);
         it.tokens = __builtin_amdgcn_readfirstlane(tokens);
         it.bad = __builtin_amdgcn_readfirstlane(bad);
+        return it;
+    }
+    __device__ __forceinline__ AttnItem item(const AttnSplit& S) const {
+        AttnItem it = sequence();
         attn_tile(S, __builtin_amdgcn_readfirstlane(tile), &it);
         return it;
     }
@@ -524,7 +561,7 @@ struct alignas(32) CutItem {
     int pieces, first, rows, tokens, tile, bad;
 };
 __device__ __forceinline__ void note_cut(CutItem* cut, const ShareWalk& sw, const AttnItem& it) {
-    *cut = CutItem{static_cast<int>((sw.start + it.steps - 1) / sw.share - sw.start / sw.share) + 1, it.first, it.rows,
+    *cut = CutItem{static_cast<int>(quotient(sw.start + it.steps - 1, sw.share) - quotient(sw.start, sw.share)) + 1, it.first, it.rows,
                    it.tokens, it.tile, it.bad};
 }
 

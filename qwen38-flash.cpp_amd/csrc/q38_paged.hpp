@@ -73,7 +73,7 @@ struct AttnSplit {
     __host__ __device__ int rows() const { return M / G; }
 };
 struct AttnItem {
-    int seq, tile;
+    int seq = -1, tile;
     int rows;    // the sequence's rows
     int first;   // its first row in the tensors
     int tokens;  // its tokens (0 where they are negative or behind the table)
@@ -131,9 +131,8 @@ __host__ __device__ inline int64_t attn_before(const AttnSplit& S, const AttnIte
     const int blind = seen < 0 ? (-seen / R < n ? -seen / R : n) : 0;  // tiles that see nothing
     return sum + blind + floor_sum(n - blind, S.T, R, seen + (blind + 1) * R + S.T - 1);
 }
-__host__ __device__ inline int64_t attn_weight(const AttnSplit& S, const PagedBatchDev& B, int shift, int seq) {
-    AttnItem it;
-    attn_sequence(B, shift, seq, &it);
+// All steps of the sequence.
+__host__ __device__ inline int64_t attn_weight(const AttnSplit& S, const AttnItem& it) {
     return attn_before(S, it, attn_tiles(S, it.rows));
 }
 // A place in the list: an item and its first step.
@@ -141,21 +140,19 @@ struct AttnCursor {
     int seq, tile;
     int64_t start;
 };
-// The item that holds step pos, inside sequence seq, whose first step is seq_start.
-__host__ __device__ inline AttnCursor attn_seek(const AttnSplit& S, const PagedBatchDev& B, int shift, int seq,
-                                                int64_t seq_start, int64_t pos) {
-    AttnItem it;
-    attn_sequence(B, shift, seq, &it);
+// The item that holds step pos, inside the sequence of `it`, whose first step is seq_start.
+__host__ __device__ inline AttnCursor attn_seek(const AttnSplit& S, const AttnItem& it, int64_t seq_start, int64_t pos) {
     int lo = 0, hi = attn_tiles(S, it.rows);
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (seq_start + attn_before(S, it, mid) <= pos) lo = mid;
         else hi = mid;
     }
-    return AttnCursor{seq, lo, seq_start + (lo ? attn_before(S, it, lo) : 0)};
+    return AttnCursor{it.seq, lo, seq_start + (lo ? attn_before(S, it, lo) : 0)};
 }
 // A share's next piece: an item's steps [from, to), the item's first step at `start` of the list. The
-// cursor stands at the item that holds step *pos and moves with it.
+// cursor stands at the item that holds step *pos and moves with it. out->it: the piece before, whose
+// sequence need not be read again, or seq -1.
 struct AttnPiece {
     AttnItem it;
     int from, to;
@@ -164,7 +161,7 @@ struct AttnPiece {
 __host__ __device__ inline bool attn_next(const AttnSplit& S, const PagedBatchDev& B, int shift, int64_t end,
                                           AttnCursor* at, int64_t* pos, AttnPiece* out) {
     while (*pos < end && at->seq < B.seqs) {
-        attn_sequence(B, shift, at->seq, &out->it);
+        if (out->it.seq != at->seq) attn_sequence(B, shift, at->seq, &out->it);
         if (at->tile < attn_tiles(S, out->it.rows)) {
             attn_tile(S, at->tile, &out->it);
             const int64_t behind = at->start + out->it.steps;

@@ -78,13 +78,18 @@ static void split(std::mt19937& rng, int seqs, int max_rows, int max_tokens, con
             attn_tile(S, j, &it);
             sum += it.steps;
         }
-        CHECK(attn_weight(S, B, shift, i) == sum);
+        CHECK(attn_weight(S, it) == sum);
         start.push_back(start.back() + sum);
     }
     auto sequence_at = [&](int64_t pos) {
         int seq = 0;
         while (seq < seqs && start[static_cast<size_t>(seq) + 1] <= pos) ++seq;
         return seq;
+    };
+    auto seek = [&](int seq, int64_t pos) {
+        AttnItem it;
+        attn_sequence(B, shift, seq, &it);
+        return attn_seek(S, it, start[static_cast<size_t>(seq)], pos);
     };
     const int64_t total = start.back(), share = (total + W - 1) / W;
     std::map<std::pair<int, int>, int> seen;  // item -> steps so far
@@ -93,7 +98,7 @@ static void split(std::mt19937& rng, int seqs, int max_rows, int max_tokens, con
         const int64_t end = std::min(total, (w + 1) * share);
         int64_t pos = w * share, before = pos;
         const int seq = sequence_at(pos);
-        AttnCursor at = attn_seek(S, B, shift, seq, start[static_cast<size_t>(seq)], pos);
+        AttnCursor at = seek(seq, pos);
         std::set<int> slots;
         AttnPiece p;
         while (attn_next(S, B, shift, end, &at, &pos, &p)) {
@@ -125,7 +130,7 @@ static void split(std::mt19937& rng, int seqs, int max_rows, int max_tokens, con
     std::map<std::pair<int, int>, std::set<std::pair<int64_t, int>>> joined;
     for (int64_t w = 1; w < W && w * share < total; ++w) {
         const int seq = sequence_at(w * share);
-        const AttnCursor at = attn_seek(S, B, shift, seq, start[static_cast<size_t>(seq)], w * share);
+        const AttnCursor at = seek(seq, w * share);
         if (at.start == w * share || at.start / share + 1 != w) continue;
         AttnItem it;
         attn_sequence(B, shift, at.seq, &it);
