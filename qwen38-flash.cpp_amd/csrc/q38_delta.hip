@@ -406,19 +406,20 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 // (u, w) thus holds key dims 4 E w .. 4 E (w + 1) - 1 of value dim u, eight of them in a row being an
 // operand of S k and S q with keys and queries read as stored: no value moves between lanes. A sequence is
 // one chain of chunks per head, and a wave issues an instruction every four cycles at best, so what the chain
-// does not need is left to a second wave on another SIMD: an output wave per state wave takes the operands of
-// S and U through LDS a chunk later, loads the keys and values and stages them as the state wave wants them
-// (the keys as stored and, pairs of rows interleaved, as operands of K^T). A prompt of 4,001 rows: 149 us, 1.2
-// us a chunk, bound by the state wave's own 400 instructions (one wave doing all: 240 us). Eight ragged
-// prompts, 16,192 rows, two workgroups per CU: 345 us, 2.0 to 2.9 us a chunk: a SIMD's matrix products (74 a
-// chunk) and vector instructions (some 420) take each other's time.
+// does not need is left to a second wave on another SIMD: two state waves (32 value columns) go with two output
+// waves, of 16 rows of the chunk each, which take the operands of S and U through LDS a chunk later, load the
+// keys and values and stage them as the state waves want them (the keys as stored and, pairs of rows
+// interleaved, as operands of K^T). A prompt of 4,001 rows: 150 us, 1.2 us a chunk, bound by the state wave's
+// own 400 instructions (one wave doing all: 240 us). Eight ragged prompts, 16,192 rows, two workgroups per CU:
+// 317 us, bound by the vector memory path, which takes a cycle per row that neighbouring lanes do not share
+// (output waves by columns, each with all queries, scores and short stores of its own: 345 us).
 template <int DK>
 struct WalkGeo {
     static constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8;
     static constexpr int NW = 2;                              // state waves of a workgroup, and output waves
     static constexpr int PC = kChunk * CH / (64 * NW);        // an output thread's rows of the keys, 16 bytes of each
     static constexpr int kKeys = kChunk * CH, kParts = NW * KS * 2 * 64, kUpd = NW * 2 * 64;
-    static constexpr size_t kLds = 2 * 16 * static_cast<size_t>(2 * kKeys + kParts + kUpd);
+    static constexpr size_t kLds = 2 * 16 * static_cast<size_t>(2 * kKeys + kParts + 2 * kUpd);  // (128 dims: half a CU's)
 };
 
 template <int DK>
@@ -426,23 +427,24 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                                                                            const ChunkSystem* __restrict__ sys, int bound) {
     using Geo = WalkGeo<DK>;
     constexpr int E = Geo::E, KS = Geo::KS, CH = Geo::CH, NW = Geo::NW, PC = Geo::PC, KB = KS < 4 ? KS : 4;
-    extern __shared__ uintx4 walk_lds[];  // [2] of: keys, K^T's operands, the state's parts, V and then U
+    extern __shared__ uintx4 walk_lds[];  // [2] of: keys, K^T's operands, the state's parts, U, V
     uintx4* const keys_lds = walk_lds;
     uintx4* const turned_lds = walk_lds + 2 * Geo::kKeys;
     uintx4* const parts_lds = walk_lds + 4 * Geo::kKeys;
     floatx4* const upd_lds = reinterpret_cast<floatx4*>(walk_lds + 2 * (2 * Geo::kKeys + Geo::kParts));
+    floatx4* const val_lds = upd_lds + 2 * Geo::kUpd;
     const int lane = threadIdx.x & 63, u = lane & 15, w = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int pair = wave % NW;
+    const int part = wave % NW;  // a state wave's 16 columns, an output wave's 16 rows of the chunk
     const bool outputs = wave >= NW;
     // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: those of one head, which read the
-    // same chunk systems, keys and queries, are one XCD's (eight ragged prompts: 371 us with the groups
-    // spread over the XCDs, 345 so).
+    // same chunk systems, keys and queries, are one XCD's (spread over the XCDs eight ragged prompts took 7%
+    // longer).
     const int groups = D.dv / (16 * NW), turn = blockIdx.x / 8, chain = turn / groups * 8 + blockIdx.x % 8;
     if (chain >= D.hv * B.seqs) return;
     const int h = chain % D.hv, hk = h / (D.hv / D.hk);
     const int s = nth_sequence(B, chain / D.hv, max(1, 256 / (groups * D.hv)));
-    const int dv = (turn % groups * NW + pair) * 16;  // the wave's first value dim
+    const int dv = turn % groups * NW * 16;  // the workgroup's first value dim
     const RowSpan span = row_span(B.off, s, B.rows);
     const int length = __builtin_amdgcn_readfirstlane(span.end - span.begin), begin = __builtin_amdgcn_readfirstlane(span.begin);
     const int c0 = __builtin_amdgcn_readfirstlane(first_chunk(B, s));
@@ -454,7 +456,9 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     auto key_at = [](int row, int ch) { return row * CH + (ch ^ ((row & 3) | ((row >> 1) & 4))); };
     // V and U: rows 8 w + 4 a .. of column u in a slot of their own, so that the writes of V, down the columns,
     // get banks of their own
-    auto slot = [&](int column, int block, int a) { return (64 * a + 16 * block + (column ^ (2 * block + a))); };
+    auto slot = [](int columns, int column, int block, int a) {
+        return 128 * columns + 64 * a + 16 * block + (column ^ (2 * block + a) ^ (4 * columns));
+    };
     // Loads of a next chunk are made always, of the last one's again behind it, and their number is the same
     // on every path, so that a wait counts only the loads that it needs. Rows behind the sequence: its last
     // row again, whose update is nothing (its beta in the system is 0).
@@ -464,17 +468,17 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         const char* const vb = reinterpret_cast<const char*>(D.v + begin * D.vs + h * D.dv + dv);
         const char* const qb = reinterpret_cast<const char*>(D.q + begin * D.qs + hk * DK);
         char* const ob = reinterpret_cast<char*>(D.out + (static_cast<size_t>(begin) * D.hv + h) * D.dv + dv);
-        const int tid = pair * 64 + lane;
-        uintx4 kr[PC], vr, qr[KS][2], mop[2][2];
-        float eg[2];
+        const int tid = part * 64 + lane;
+        uintx4 kr[PC], vr, qr[KS], mop[2];
+        float eg;
         auto fetch_keys = [&](int chunk) {
 #pragma unroll
             for (int i = 0; i < PC; ++i) {
                 const int64_t row = min(chunk * kChunk + tid / CH * PC + i, length - 1);
                 kr[i] = *reinterpret_cast<const uintx4*>(kb + 2 * row * D.ks + 16 * (tid % CH));
             }
-            const int64_t row = min(chunk * kChunk + lane / 2, length - 1);
-            vr = *reinterpret_cast<const uintx4*>(vb + 2 * (row * D.vs + 8 * (lane & 1)));
+            const int64_t row = min(chunk * kChunk + 16 * part + lane / 4, length - 1);
+            vr = *reinterpret_cast<const uintx4*>(vb + 2 * (row * D.vs + 8 * (lane & 3)));
         };
         auto stage_keys = [&](int buf) {
             const int r0 = tid / CH * PC;
@@ -500,28 +504,22 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                     *reinterpret_cast<pairs_t*>(to) = all;
                 }
             }
-            const int row = lane / 2;
-            float* to = reinterpret_cast<float*>(upd_lds + buf * Geo::kUpd + pair * 2 * 64) + (row & 3);
+            const int row = 16 * part + lane / 4;
+            float* to = reinterpret_cast<float*>(val_lds + buf * Geo::kUpd) + (row & 3);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                to[4 * slot(8 * (lane & 1) + i, row >> 3, row >> 2 & 1)] = i & 1 ? bfhi(vr[i >> 1]) : bflo(vr[i >> 1]);
+                to[4 * slot(lane >> 1 & 1, 8 * (lane & 1) + i, row >> 3, row >> 2 & 1)] =
+                    i & 1 ? bfhi(vr[i >> 1]) : bflo(vr[i >> 1]);
         };
-        auto fetch_queries = [&](int chunk) {  // operands: row 16 a + u, dims 4 E w + 8 k ..
+        auto fetch_queries = [&](int chunk) {  // operands: row u of the wave's, dims 4 E w + 8 k ..
+            const int64_t row = min(chunk * kChunk + 16 * part + u, length - 1);
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const int64_t row = min(chunk * kChunk + 16 * a + u, length - 1);
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-                    qr[k][a] = *reinterpret_cast<const uintx4*>(qb + 2 * row * D.qs + 16 * (KS * w + k));
-            }
+            for (int k = 0; k < KS; ++k) qr[k] = *reinterpret_cast<const uintx4*>(qb + 2 * row * D.qs + 16 * (KS * w + k));
         };
         auto fetch_scores = [&](const ChunkSystem& cs) {
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-#pragma unroll
-                for (int p = 0; p < 2; ++p) mop[p][a] = cs.m[p][a][lane];
-                eg[a] = cs.into[16 * a + u];
-            }
+            for (int p = 0; p < 2; ++p) mop[p] = cs.m[p][part][lane];
+            eg = cs.into[16 * part + u];
         };
         if (chunks > 0) {
             fetch_keys(0);
@@ -533,40 +531,53 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         for (int n = 0; n <= chunks && chunks > 0; ++n) {  // the keys of chunk n + 1, the outputs of chunk n - 1
             fetch_keys(min(n + 1, chunks - 1));
             if (n > 0) {
-                const uintx4* parts = parts_lds + ((n - 1) & 1) * Geo::kParts + pair * KS * 2 * 64 + lane;
-                const floatx4* upd = upd_lds + ((n - 1) & 1) * Geo::kUpd + pair * 2 * 64;
-                // O^T = exp(G) S q + U^T M^T, transposed: value dims by chunk rows
-                floatx4 ot[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                const uintx4* parts = parts_lds + ((n - 1) & 1) * Geo::kParts + lane;
+                const floatx4* upd = upd_lds + ((n - 1) & 1) * Geo::kUpd;
+                // O^T = exp(G) S q + U^T M^T, transposed: value dims by the wave's rows
+                floatx4 ot[NW];
+#pragma unroll
+                for (int c = 0; c < NW; ++c) ot[c] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
 #pragma unroll
                     for (int p = 1; p >= 0; --p)
 #pragma unroll
-                        for (int a = 0; a < 2; ++a) ot[a] = mfma(parts[(k * 2 + p) * 64], qr[k][a], ot[a]);
-                const floatx4 un[2] = {upd[slot(u, w, 0)], upd[slot(u, w, 1)]};
-                Parts<2> up;
-                {
+                        for (int c = 0; c < NW; ++c) ot[c] = mfma(parts[((c * KS + k) * 2 + p) * 64], qr[k], ot[c]);
+                Parts<2> up[NW];
+#pragma unroll
+                for (int c = 0; c < NW; ++c) {
+                    const floatx4 un[2] = {upd[slot(c, u, w, 0)], upd[slot(c, u, w, 1)]};
                     float x[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[j] = un[j >> 2][j & 3];
-                    up.split(x);
+                    up[c].split(x);
                 }
 #pragma unroll
-                for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[0], mop[1][a], ot[a] * eg[a]);
+                for (int c = 0; c < NW; ++c) ot[c] = mfma(up[c].p[0], mop[1], ot[c] * eg);
 #pragma unroll
                 for (int p = 1; p >= 0; --p)
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) ot[a] = mfma(up.p[p], mop[0][a], ot[a]);
+                    for (int c = 0; c < NW; ++c) ot[c] = mfma(up[c].p[p], mop[0], ot[c]);
                 fetch_queries(n);
                 fetch_scores(system(n));
+                // lane L stores 16 bytes of row L / 4: what lanes (L / 4, 2 (L % 2)) and the next w have of its columns
+                uint32_t x[4];
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    ot[a] *= D.scale;
-                    const int row = (n - 1) * kChunk + 16 * a + u;
-                    if (row < length)
-                        *reinterpret_cast<uint2*>(ob + 2 * (static_cast<int64_t>(row) * D.hv * D.dv + 4 * w)) =
-                            make_uint2(pack_bf16(ot[a][0], ot[a][1]), pack_bf16(ot[a][2], ot[a][3]));
-                }
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        const int from = 4 * (lane / 4 + 16 * (2 * (lane & 1) + i));
+                        uint32_t y[NW];
+#pragma unroll
+                        for (int c = 0; c < NW; ++c)
+                            y[c] = __builtin_amdgcn_ds_bpermute(
+                                from, pack_bf16(ot[c][2 * d] * D.scale, ot[c][2 * d + 1] * D.scale));
+                        x[2 * i + d] = lane & 2 ? y[1] : y[0];
+                    }
+                const int row = (n - 1) * kChunk + 16 * part + lane / 4;
+                if (row < length)
+                    *reinterpret_cast<uintx4*>(ob + 2 * (static_cast<int64_t>(row) * D.hv * D.dv + 8 * (lane & 3))) =
+                        (uintx4){x[0], x[1], x[2], x[3]};
             }
             stage_keys((n + 1) & 1);
             lds_barrier();  // (the next chunk's loads stay in flight)
@@ -578,7 +589,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     const int from = B.origin ? uniform_load(B.origin + s) : -1;
     floatx4 st[E];
     auto state_at = [&](int slot, int r) {  // E consecutive key dims
-        return B.states + slot * elems + (static_cast<size_t>(h) * D.dv + dv + u) * DK + E * (4 * w + r);
+        return B.states + slot * elems + (static_cast<size_t>(h) * D.dv + dv + 16 * part + u) * DK + E * (4 * w + r);
     };
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -618,8 +629,9 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     for (int n = 0; n < chunks; ++n) {
         const uintx4* kt = keys_lds + (n & 1) * Geo::kKeys;
         const uintx4* turned = turned_lds + (n & 1) * Geo::kKeys + lane;
-        uintx4* parts = parts_lds + (n & 1) * Geo::kParts + pair * KS * 2 * 64 + lane;
-        floatx4* upd = upd_lds + (n & 1) * Geo::kUpd + pair * 2 * 64;
+        uintx4* parts = parts_lds + (n & 1) * Geo::kParts + part * KS * 2 * 64 + lane;
+        floatx4* upd = upd_lds + (n & 1) * Geo::kUpd;
+        const floatx4* val = val_lds + (n & 1) * Geo::kUpd;
         const ChunkSystem& next = system(n + 1);
         // P = K S^T (chunk rows by value dims)
         floatx4 pr[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -649,7 +661,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         __builtin_amdgcn_sched_barrier(0);
         // V, K^T and the state's decay, beside the products' end (the reads first: left to the compiler some
         // came after the sums that need them, 2% of the walk)
-        const floatx4 vv[2] = {upd[slot(u, w, 0)], upd[slot(u, w, 1)]};
+        const floatx4 vv[2] = {val[slot(part, u, w, 0)], val[slot(part, u, w, 1)]};
         constexpr int KT = E < 8 ? E : 8;
         uintx4 kv[KT];
 #pragma unroll
@@ -684,7 +696,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
             zp.split(z);
         }
 #pragma unroll
-        for (int a = 0; a < 2; ++a) upd[slot(u, w, a)] = un[a];
+        for (int a = 0; a < 2; ++a) upd[slot(part, u, w, a)] = un[a];
         load_left(next);
 #pragma unroll
         for (int o = 0; o < E; o += 2) {
