@@ -251,6 +251,25 @@ def test_most_sequences(gpu, q38):
             assert torch.equal(s[at], states[at])
 
 
+def test_most_rows(gpu, q38):
+    """A prompt of 2^19 rows: the bits of the same rows in sixteen calls (whole chunks each)."""
+    n, parts = 1 << 19, 16
+    c = DeltaCase([n], 1, 1, 64, 64, seed=18)
+    out, states = run(q38, gpu, c)
+    assert torch.isfinite(out.float()).all()
+    pool = c.states.cuda()
+    at = c.origin.clone()
+    for i in range(parts):
+        m = n // parts
+        d = DeltaCase([m], 1, 1, 64, 64)
+        d.qkv, d.g_log, d.beta = c.qkv[i * m:i * m + m], c.g_log[i * m:i * m + m], c.beta[i * m:i * m + m]
+        d.origin, d.last = at, c.last
+        o, s = run(q38, gpu, d, states=pool)
+        assert torch.equal(o, out[i * m:i * m + m]), i
+        at = c.last
+    assert torch.equal(s[int(c.last[0])], states[int(c.last[0])])
+
+
 def test_no_rows_copies_states(gpu, q38):
     c = DeltaCase([0, 0, 0], 2, 4, 64, 128, seed=14)
     c.origin[1] = -1

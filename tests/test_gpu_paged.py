@@ -272,6 +272,21 @@ def test_offsets_beyond_32_bits(gpu, q38):
     assert torch.equal(big[0][shift + p[-1], :, o[-1]].cpu(), k[0])
 
 
+def test_most_rows(gpu, q38):
+    """A prompt of 2^19 rows: a few of its rows against float64."""
+    n = 1 << 19
+    b = Batch([n], [n], page=1024, hkv=1, dim=64, seed=19)
+    cache = b.cache(False)
+    q = b.randn(n, 1, 64).to(BF16)
+    got = run_attend(q38, gpu, b, cache, q, 0.125)
+    assert torch.isfinite(got.float()).all()
+    rows = [0, 1, 255, 256, 131071, 300000, n - 257, n - 1]
+    for r in rows:  # each as the last row of a sequence of its own
+        one = Batch([1], [r + 1], page=1024, hkv=1, dim=64)
+        one.table, one.pages = b.table, b.pages
+        check_attend(one, cache, q[r:r + 1], 0.125, got[r:r + 1])
+
+
 # ------------------------------------------------------------------ append
 def quantised(x):
     """Codes and scales of head rows [..., dim] by exact arithmetic (integers in float64)."""
