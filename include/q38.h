@@ -779,12 +779,13 @@ int q38_paged_attention(q38_ctx* ctx, const q38_paged_cache* cache, const q38_pa
  * q, k: device bf16 [key_heads][key_dim] per row (value head h reads key head h / (value_heads /
  * key_heads)), v [value_heads][value_dim], each at its row stride (slices of one convolved row;
  * 16-byte aligned, strides multiples of 8); log_decay (g <= 0; -inf clears the state) and beta:
- * device float [rows][value_heads]; out: device bf16 [rows][value_heads][value_dim]. q and k are
- * taken as given (the layer normalises them before: |k| = 1 keeps the rule stable). Batches with
- * max_rows above 16 (28 from 32 sequences on) run in chunks of 32 rows on the matrix cores, with
- * states as exact as float ones (operands split into bf16 parts) and outputs as their own
- * rounding; others, and calls with checkpoints, run row by row. Infinities and NaN among a sequence's operands reach its later rows
- * and its state, in chunks also the earlier rows of their 32. The workspace is 16-byte aligned.
+ * device float [rows][value_heads]; out: device bf16 [rows][value_heads][value_dim], which may not
+ * overlap the operands. q and k are taken as given (the layer normalises them before: |k| = 1
+ * keeps the rule stable). Batches with max_rows above 16 (28 from 32 sequences on) run in chunks
+ * of 32 rows on the matrix cores, with states as exact as float ones (operands split into bf16
+ * parts) and outputs as their own rounding; others, and calls with checkpoints, run row by row.
+ * Infinities and NaN among a sequence's operands reach its later rows and its state, in chunks
+ * also the earlier rows of their 32. The workspace is 16-byte aligned.
  * States: a pool [slots][value_heads][value_dim][key_dim] of floats, 16-byte aligned. origin[i]:
  * the slot a sequence starts from, negative (or a null array) for the zero state; final_slots[i]:
  * the slot its last state goes to, negative (or null) for none, its own origin for an update in

@@ -252,12 +252,12 @@ __device__ __forceinline__ int first_chunk(const DeltaBatchDev& B, int seq) {
 
 // One wave per chunk and value head, or two value heads of one key head (N = 2): their products are the
 // same, and the substitution of one head's diagonal blocks fills half a wave (eight ragged prompts, 16,320
-// systems: 86 us with one, 75 with two, 2.3 TB/s of systems written). Bound by the chain of its steps, and
-// by LDS, which holds 8 waves a CU.
+// systems: 86 us with one, 75 with two). Bound by bytes where there are many chunks: those systems are 171 MB
+// behind 133 MB of queries and keys, 4.1 TB/s (half the LDS, for twice the waves, changed nothing).
 template <int DK, int N>
 __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B, ChunkSystem* __restrict__ sys) {
     constexpr int KS = DK / 32, LD = kChunk + 4;
-    __shared__ __align__(16) float As[N][kChunk][LD], Ts[N][kChunk][LD];
+    __shared__ __align__(16) float As[N][kChunk][LD];  // A, then T in its place, then the scores
     __shared__ double Gs[N][kChunk];
     __shared__ float Bs[N][kChunk];
     const int h0 = blockIdx.y * N, lane = threadIdx.x, u = lane & 15, w = lane >> 4, hk = h0 / (D.hv / D.hk);
@@ -335,21 +335,20 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            Ts[e][b + i][b + u] = t[i];
-            Ts[e][i][16 + u] = 0.0f;
+            As[e][b + i][b + u] = t[i];
         }
     }
     __syncthreads();
-    // the block below them: -T22 (A21 T11), float products (A21 T11 in place of A11, which is done with)
+    // the block below them: -T22 (A21 T11), float products (A21 T11 stands above for a while)
     floatx4 x[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         x[e] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < 16; k += 4)
-            x[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(As[e][16 + u][k + w], Ts[e][k + w][u], x[e], 0, 0, 0);
+            x[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(As[e][16 + u][k + w], As[e][k + w][u], x[e], 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) As[e][4 * w + r][u] = x[e][r];
+        for (int r = 0; r < 4; ++r) As[e][4 * w + r][16 + u] = x[e][r];
     }
     __syncthreads();
 #pragma unroll
@@ -357,12 +356,28 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
         x[e] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < 16; k += 4)
-            x[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Ts[e][16 + u][16 + k + w], As[e][k + w][u], x[e], 0, 0, 0);
+            x[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(As[e][16 + u][16 + k + w], As[e][k + w][16 + u], x[e], 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) Ts[e][16 + 4 * w + r][u] = -x[e][r];
+        for (int r = 0; r < 4; ++r) {
+            As[e][16 + 4 * w + r][u] = -x[e][r];
+            As[e][4 * w + r][16 + u] = 0.0f;
+        }
     }
     __syncthreads();
-    // the scores, where A was
+    ChunkSystem* const out0 = sys + static_cast<size_t>(blockIdx.x) * D.hv + h0;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            float row[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) row[j] = As[e][chunk_row(u, a)][8 * w + j] * Bs[e][8 * w + j];
+            Parts<3> t;
+            t.split(row);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) out0[e].t[p][a][lane] = t.p[p];
+        }
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < N; ++e)
 #pragma unroll
@@ -374,22 +389,13 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        ChunkSystem& out = sys[static_cast<size_t>(blockIdx.x) * D.hv + h0 + e];
-        float beta[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) beta[j] = Bs[e][8 * w + j];
+        ChunkSystem& out = out0[e];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             float row[8];
-            Parts<3> t;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) row[j] = Ts[e][chunk_row(u, a)][8 * w + j] * beta[j];
-            t.split(row);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) out.t[p][a][lane] = t.p[p];
-            Parts<2> m;
 #pragma unroll
             for (int j = 0; j < 8; ++j) row[j] = As[e][16 * a + u][8 * w + j];
+            Parts<2> m;
             m.split(row);
 #pragma unroll
             for (int p = 0; p < 2; ++p) out.m[p][a][lane] = m.p[p];
