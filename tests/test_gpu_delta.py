@@ -354,3 +354,32 @@ def test_two_calls_at_once(gpu, q38):
     for i, ((c, (o, s)), call) in enumerate(zip(jobs, calls)):
         at = c.last.long()
         assert torch.equal(call[3].cpu(), o) and torch.equal(pool.cpu()[at + i * n], s[at])
+
+
+@pytest.mark.parametrize("rows", [[3, 1, 5, 2], [40, 70, 33, 5]])
+def test_nan_stays_in_its_sequence(gpu, q38, rows):
+    """NaN in every operand of one sequence and in the rows of nobody: the others' bits stay."""
+    c = DeltaCase(rows, 2, 4, 64, 128, seed=19, gap=3)
+    want_out, want = run(q38, gpu, c)
+    a, b = int(c.off[1]), int(c.off[2])
+    bad = torch.ones(c.rows, dtype=torch.bool)
+    bad[int(c.off[0]):a] = False
+    bad[b:int(c.off[-1])] = False
+    for t in (c.qkv, c.g_log, c.beta):
+        t[bad] = math.nan
+    c.states[int(c.origin[1])] = math.nan
+    out, states = run(q38, gpu, c)
+    assert torch.equal(out[:a], want_out[:a]) and torch.equal(out[b:], want_out[b:])
+    for i in (0, 2, 3):
+        assert torch.equal(states[int(c.last[i])], want[int(c.last[i])])
+    assert torch.isnan(out[a:b].float()).all()
+
+
+@pytest.mark.parametrize("rows", [[5], [100]])
+def test_zero_beta_and_zero_rows_leave_the_state(gpu, q38, rows):
+    """beta 0 and no decay: the state as it was, bit for bit in both forms; the outputs S q."""
+    c = DeltaCase(rows, 1, 2, 64, 64, seed=20, decay=0.0)
+    c.beta[:] = 0
+    out, states = run(q38, gpu, c)
+    check(c, out, states)
+    assert torch.equal(states[int(c.last[0])], c.states[int(c.origin[0])])

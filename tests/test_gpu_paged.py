@@ -482,3 +482,36 @@ def test_two_calls_at_once(gpu, q38):
     torch.cuda.synchronize()
     for _, _, _, outs, _, _ in jobs:
         assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("rows", [[3, 1, 2], [40, 70, 33]])
+@pytest.mark.parametrize("q8", [False, True])
+def test_nan_stays_in_its_sequence(gpu, q38, rows, q8):
+    """NaN queries of one sequence and of the rows of nobody, NaN keys and values of its tokens: the
+    others' bits stay."""
+    b = Batch(rows, [200, 300, 90], hkv=2, dim=128, seed=43, gap=3)
+    cache = b.cache(q8)
+    q = b.randn(b.rows, 8, 128).to(BF16)
+    want = run_attend(q38, gpu, b, cache, q, 0.09)
+    a, e = int(b.off[1]), int(b.off[2])
+    q[:3], q[-3:], q[a:e] = math.nan, math.nan, math.nan
+    p, o = b.places(1)
+    for t in cache[2:] if q8 else cache[:2]:
+        t[p, :, o] = math.nan
+    got = run_attend(q38, gpu, b, cache, q, 0.09)
+    assert torch.equal(got[:a], want[:a]) and torch.equal(got[e:], want[e:])
+    assert torch.isnan(got[a:e].float()).all()
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_one_token_is_its_value(gpu, q38, rows):
+    """Rows that see one token, or tokens of one value, give that value exactly (softmax sums to 1)."""
+    b = Batch([rows], [rows], hkv=2, dim=64, seed=44)
+    cache = b.cache(False)
+    p, o = b.places(0)
+    cache[1][p, :, o] = cache[1][p[:1], :, o[:1]].clone()
+    q = b.randn(b.rows, 4, 64).to(BF16)
+    got = run_attend(q38, gpu, b, cache, q, 0.125)
+    v = cache[1][p[0], :, o[0]].repeat_interleave(2, 0)
+    assert torch.equal(got[0], v)
+    check_attend(b, cache, q, 0.125, got)
