@@ -970,7 +970,7 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnSplit S, int W, const fl
     // (it is the second slot of its first share and the first of the others)
     const float* first = part + (static_cast<int64_t>(place) * 2 + 1) * (M * (D + 2));
     auto piece = [&](int i) { return first + static_cast<int64_t>(2 * i - (i > 0)) * (M * (D + 2)); };
-#pragma unroll(WQ > 1 ? 1 : 2)
+#pragma unroll 2
     for (int j = wave / WQ; j < QB; j += 4 / WQ) {
         const int i = blockIdx.z * QB + j, row = tile_row(S, it, i);
         if (WQ == 1 && row < 0) continue;
