@@ -26,7 +26,7 @@ import torch
 
 own = False
 
-_held = {"ctx": None, "ws": None}
+_contexts = {}  # of the framework, one per device
 
 
 # ------------------------------------------------------------------ the cases
@@ -226,42 +226,43 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------ the framework's calls
-def _framework():
-    sys.path.insert(0, os.path.join(os.getcwd(), "qwen38-flash.cpp_amd"))
+def _framework(device):
+    path = os.path.join(os.getcwd(), "qwen38-flash.cpp_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
     import q38
-    if _held["ctx"] is None:
-        _held["ctx"] = q38.Ctx(torch.cuda.current_device())
-    return q38, _held["ctx"]
+    if device.index not in _contexts:
+        _contexts[device.index] = q38.Ctx(device.index)
+    return q38, _contexts[device.index]
 
 
-def _workspace(nbytes):
-    """One workspace serves the stream's calls one after the other."""
-    if _held["ws"] is None or _held["ws"].numel() < nbytes:
-        _held["ws"] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device="cuda")
-    return _held["ws"]
+def _workspace(s, nbytes):
+    """A prepared state's own: passes of other states may overlap, and a graph of this one keeps its address."""
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=s["off"].device)
 
 
 def _own(s):
-    st = torch.cuda.current_stream().cuda_stream
+    st = torch.cuda.current_stream(s["off"].device).cuda_stream
     op = s["case"]["op"]
     if "call" not in s:  # the handles and descriptions that a program keeps beside its buffers
-        q38, ctx = _framework()
+        q38, ctx = _framework(s["off"].device)
         if op == "delta":
             rule = q38.DeltaRule(ctx, s["case"]["hk"], s["case"]["hv"], s["case"]["dk"], s["case"]["dv"], s["scale"])
             batch = q38.DeltaBatch(s["states"], s["off"], s["origin"], s["final"], s["rows"], s["max_rows"],
                                    s["checkpoints"])
-            s["call"] = rule, batch, rule.workspace_size(batch)
+            s["call"] = rule, batch, _workspace(s, rule.workspace_size(batch))
         else:
             cache = q38.PagedCache(ctx, s["keys"], s["values"], s["keys_scale"], s["values_scale"])
             batch = q38.PagedBatch(s["off"], s["tokens"], s["table"], s["rows"], s["max_rows"])
-            s["call"] = cache, batch, cache.workspace_size(batch, s["case"]["hq"]) if op == "attend" else 0
-    handle, batch, nbytes = s["call"]
+            ws = _workspace(s, cache.workspace_size(batch, s["case"]["hq"])) if op == "attend" else None
+            s["call"] = cache, batch, ws
+    handle, batch, ws = s["call"]
     if op == "delta":
-        handle.run(batch, s["q"], s["k"], s["v"], s["g"], s["beta"], s["out"], _workspace(nbytes), st)
+        handle.run(batch, s["q"], s["k"], s["v"], s["g"], s["beta"], s["out"], ws, st)
     elif op == "append":
         handle.append(batch, s["k"], s["v"], st)
     else:
-        handle.attend(batch, s["q"], s["out"], s["scale"], _workspace(nbytes), st)
+        handle.attend(batch, s["q"], s["out"], s["scale"], ws, st)
 
 
 # ------------------------------------------------------------------ the plain forms
