@@ -287,7 +287,7 @@ class Ctx:
     def __init__(self, device: int = 0):
         h = P()
         check(lib.q38_ctx_create(device, C.byref(h)))
-        self.h = h
+        self.h, self.device = h, device
 
     def close(self):
         if self.h:
@@ -442,6 +442,21 @@ def _int32(what: str, *tensors):
             raise ValueError(f"{what} must be contiguous int32 tensors")
 
 
+def _same_device(*tensors) -> int:
+    """The device index of tensors that belong together (-1: host memory)."""
+    devices = {t.get_device() for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"tensors lie on several devices: {sorted(devices)} (-1: the host)")
+    return devices.pop() if devices else -1
+
+
+def _on_device(ctx, *devices):
+    """Addresses of the host or of another device would be followed by the kernels: refused here, where they
+    are still tensors. (Without a context the library refuses the call itself.)"""
+    if ctx is not None and any(d != ctx.device for d in devices):
+        raise ValueError(f"a tensor is not on the context's device {ctx.device}")
+
+
 def _row_stride(t, rows: int, heads: int, dim: int) -> int:
     """Row stride in elements of a [rows or more, heads, dim] bf16 tensor whose rows are contiguous."""
     stride, (n, h, d) = t.stride(), t.shape
@@ -462,7 +477,7 @@ class PagedBatch:
         n = tokens.numel()
         if row_offsets.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("row_offsets [n + 1], tokens [n] and page_table [n, pages] disagree")
-        self._keep, self.rows = (row_offsets, tokens, page_table), rows
+        self._keep, self.rows, self._device = (row_offsets, tokens, page_table), rows, _same_device(row_offsets, tokens, page_table)
         self.desc = PagedBatchDesc(n, rows, max_rows, page_table.shape[1], ptr(row_offsets), ptr(tokens),
                                    ptr(page_table))
 
@@ -483,6 +498,7 @@ class PagedCache:
             if q8 and (t.shape != keys.shape[:3] or not _is(t, "float32") or not t.is_contiguous()):
                 raise ValueError("scales must be contiguous float32 [pages, kv_heads, page_tokens] tensors")
         self._ctx, self._keep = ctx, (keys, values, key_scales, value_scales)
+        _on_device(ctx, _same_device(*self._keep))
         pages, self._heads, page, self._dim = keys.shape
         self.desc = PagedCacheDesc(ptr(keys), ptr(values), _opt(key_scales), _opt(value_scales),
                                    Q38_KV_Q8 if q8 else Q38_KV_BF16, pages, page, self._heads, self._dim)
@@ -491,6 +507,7 @@ class PagedCache:
         """k, v: [rows, kv_heads, head_dim] bf16, any row stride."""
         ks = _row_stride(k, batch.rows, self._heads, self._dim)
         vs = _row_stride(v, batch.rows, self._heads, self._dim)
+        _on_device(self._ctx, batch._device, k.get_device(), v.get_device())
         check(lib.q38_paged_append(self._ctx and self._ctx.h, self.desc, batch.desc, k.data_ptr(), ks, v.data_ptr(), vs,
                                    st))
 
@@ -501,6 +518,9 @@ class PagedCache:
         """q, out: [rows, q_heads, head_dim] bf16, any row stride."""
         heads = q.shape[1]
         qs, os_ = _row_stride(q, batch.rows, heads, self._dim), _row_stride(out, batch.rows, heads, self._dim)
+        _on_device(self._ctx, batch._device, q.get_device(), out.get_device())
+        if ws is not None:
+            _on_device(self._ctx, ws.get_device())
         check(lib.q38_paged_attention(self._ctx and self._ctx.h, self.desc, batch.desc, q.data_ptr(), qs, heads, scale,
                                       out.data_ptr(), os_, _opt(ws), 0 if ws is None else ws.nbytes, st))
 
@@ -520,6 +540,7 @@ class DeltaBatch:
         if states is not None and (states.dim() != 4 or not _is(states, "float32") or not states.is_contiguous()):
             raise ValueError("states must be a contiguous float32 [slots, value_heads, value_dim, key_dim] tensor")
         self._keep, self.rows = (states, row_offsets, origin, final_slots, checkpoints), rows
+        self._device = _same_device(*self._keep)
         self._state_shape = None if states is None else tuple(states.shape[1:])
         self.desc = DeltaBatchDesc(n, rows, max_rows, 0 if states is None else states.shape[0], ptr(row_offsets),
                                    _opt(origin), _opt(final_slots), _opt(checkpoints), _opt(states))
@@ -547,6 +568,10 @@ class DeltaRule:
         for t in (log_decay, beta):
             if t.shape[1:] != (hv,) or t.shape[0] < rows or not _is(t, "float32") or not t.is_contiguous():
                 raise ValueError("log_decay and beta must be contiguous float32 [rows, value_heads] tensors")
+        _on_device(self._ctx, batch._device, q.get_device(), k.get_device(), v.get_device(), log_decay.get_device(),
+                   beta.get_device(), out.get_device())
+        if ws is not None:
+            _on_device(self._ctx, ws.get_device())
         check(lib.q38_delta_rule(self._ctx and self._ctx.h, self.desc, batch.desc, q.data_ptr(), qs, k.data_ptr(), ks,
                                  v.data_ptr(), vs, log_decay.data_ptr(), beta.data_ptr(), out.data_ptr(), _opt(ws),
                                  0 if ws is None else ws.nbytes, st))

@@ -181,3 +181,61 @@ def test_binding_refuses_what_the_abi_cannot_see(q38):
     f = t(3, 2, dt=torch.float32)
     with pytest.raises(ValueError):
         rule.run(db, t(3, 1, 64), t(3, 1, 64), t(3, 2, 64), f, f, t(3, 2, 64), None)
+
+
+def test_binding_refuses_tensors_of_another_device(q38):
+    """Host tensors (here for every operand in turn) never reach a kernel: the binding refuses them before the
+    library is called. A context of the host's "device" -1 stands for tensors that are where they should be."""
+    import types
+
+    import torch
+    gpu, here = (types.SimpleNamespace(h=None, device=d) for d in (0, -1))
+    t = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)  # noqa: E731
+    i32 = lambda *s: t(*s, dt=torch.int32)  # noqa: E731
+
+    class Elsewhere:  # a tensor that names device 0 as its own
+        def __init__(self, x):
+            self.x = x
+
+        def __getattr__(self, name):
+            return getattr(self.x, name)
+
+        def get_device(self):
+            return 0
+
+    keys = t(4, 2, 16, 64)
+    with pytest.raises(ValueError, match="device"):
+        q38.PagedCache(gpu, keys, keys)
+    with pytest.raises(ValueError, match="device"):
+        q38.PagedCache(gpu, Elsewhere(keys), keys)
+    with pytest.raises(ValueError, match="device"):
+        q38.PagedBatch(Elsewhere(i32(4)), i32(3), i32(3, 4), 3, 1)
+    batch, cache = q38.PagedBatch(i32(4), i32(3), i32(3, 4), 3, 1), q38.PagedCache(here, keys, keys)
+    ws = t(1 << 22, dt=torch.uint8)
+    k, q = t(3, 2, 64), t(3, 4, 64)
+    for bad in range(2):
+        ops = [Elsewhere(k) if i == bad else k for i in range(2)]
+        with pytest.raises(ValueError, match="device"):
+            cache.append(batch, *ops)
+    for bad in range(3):
+        ops = [Elsewhere(x) if i == bad else x for i, x in enumerate((q, q, ws))]
+        with pytest.raises(ValueError, match="device"):
+            cache.attend(batch, ops[0], ops[1], 0.1, ops[2])
+    moved = q38.PagedBatch(Elsewhere(i32(4)), Elsewhere(i32(3)), Elsewhere(i32(3, 4)), 3, 1)
+    with pytest.raises(ValueError, match="device"):
+        cache.append(moved, k, k)
+    with pytest.raises(q38.Q38Error, match="null context"):  # nothing else is wrong with the call
+        cache.append(batch, k, k)
+
+    f, pool = t(3, 2, dt=torch.float32), t(4, 2, 64, 64, dt=torch.float32)
+    with pytest.raises(ValueError, match="device"):
+        q38.DeltaBatch(Elsewhere(pool), i32(3), i32(2), i32(2), 3, 1)
+    rule, db = q38.DeltaRule(here, 1, 2, 64, 64, 1.0), q38.DeltaBatch(pool, i32(3), i32(2), i32(2), 3, 1)
+    good = (t(3, 1, 64), t(3, 1, 64), t(3, 2, 64), f, f, t(3, 2, 64), ws)
+    for bad in range(len(good)):
+        with pytest.raises(ValueError, match="device"):
+            rule.run(db, *(Elsewhere(x) if i == bad else x for i, x in enumerate(good)))
+    with pytest.raises(ValueError, match="device"):
+        q38.DeltaRule(gpu, 1, 2, 64, 64, 1.0).run(db, *good)
+    with pytest.raises(q38.Q38Error, match="null context"):
+        rule.run(db, *good)
