@@ -556,10 +556,11 @@ struct ShareWalk {
     int seq_;
 };
 // What a share leaves for the join: the item that goes on behind it, if it began in it, and the
-// number of its pieces (0: none).
-struct alignas(32) CutItem {
-    int pieces, first, rows, tokens, tile, bad;
+// number of its pieces (0: none). They lie at the workspace's start, which is 16-byte aligned.
+struct alignas(16) CutItem {
+    int pieces, first, rows, tokens, tile, bad, unused[2];
 };
+static_assert(sizeof(CutItem) == 32 && alignof(CutItem) <= 16, "the partial sums behind them keep the workspace's alignment");
 __device__ __forceinline__ void note_cut(CutItem* cut, const ShareWalk& sw, const AttnItem& it) {
     *cut = CutItem{static_cast<int>(quotient(sw.start + it.steps - 1, sw.share) - quotient(sw.start, sw.share)) + 1, it.first, it.rows,
                    it.tokens, it.tile, it.bad};

@@ -383,3 +383,16 @@ def test_zero_beta_and_zero_rows_leave_the_state(gpu, q38, rows):
     out, states = run(q38, gpu, c)
     check(c, out, states)
     assert torch.equal(states[int(c.last[0])], c.states[int(c.origin[0])])
+
+
+def test_workspace_is_aligned_to_16_bytes_only(gpu, q38):
+    c = DeltaCase([90, 40], 2, 4, 128, 128, seed=21)
+    want = run(q38, gpu, c)
+    need = q38.DeltaRule(gpu, 2, 4, 128, 128, c.scale).workspace_size(
+        q38.DeltaBatch(c.states.cuda(), c.off.cuda(), c.origin.cuda(), c.last.cuda(), c.rows, c.max_rows))
+    ws = torch.full((need + 64,), 0xff, dtype=torch.uint8, device="cuda")
+    at = 48 - ws.data_ptr() % 32
+    got = run(q38, gpu, c, ws=ws[at:at + need])
+    last = c.last.long()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1][last], want[1][last])
+    assert (ws[:at] == 0xff).all() and (ws[at + need:] == 0xff).all()

@@ -515,3 +515,19 @@ def test_one_token_is_its_value(gpu, q38, rows):
     v = cache[1][p[0], :, o[0]].repeat_interleave(2, 0)
     assert torch.equal(got[0], v)
     check_attend(b, cache, q, 0.125, got)
+
+
+@pytest.mark.parametrize("rows,tokens", [([1, 2], [3000, 700]), ([60, 1], [2500, 900])])
+def test_workspace_is_aligned_to_16_bytes_only(gpu, q38, rows, tokens):
+    """A workspace 16 bytes behind a multiple of 32 (what the call asks for and no more), with items cut across
+    workgroups: the bits of any other workspace."""
+    b = Batch(rows, tokens, hkv=2, dim=128, seed=45)
+    cache = b.cache(False)
+    q = b.randn(b.rows, 8, 128).to(BF16)
+    want = run_attend(q38, gpu, b, cache, q, 0.09)
+    need = q38.PagedCache(gpu, *[t.cuda() for t in cache[:2]]).workspace_size(batch_on_gpu(q38, b), 8)
+    ws = torch.full((need + 64,), 0xff, dtype=torch.uint8, device="cuda")
+    view = ws[48 - ws.data_ptr() % 32:][:need]
+    assert view.data_ptr() % 32 == 16
+    assert torch.equal(run_attend(q38, gpu, b, cache, q, 0.09, ws=view), want)
+    assert (ws[:48 - ws.data_ptr() % 32] == 0xff).all() and (ws[48 - ws.data_ptr() % 32 + need:] == 0xff).all()
