@@ -145,11 +145,12 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B)
 //
 // The products run on the bf16 matrix cores. q, k and v are bf16 already: k . k and q . k are exact
 // products with float sums. Float operands are split into bf16 parts, x = hi + mid + lo: three parts
-// (24 bits) of Y, U and T, which the state's new terms are made of, multiplied part by part (for two
-// split operands the six products down to 2^-24); two (16 bits) of the state where it is multiplied with
-// k and q (the state itself stays in float), of the scores and of U in the outputs. Against 64 bits
-// the states are off by 1.2e-7 (7e-8 row by row in float, 4e-6 with two parts everywhere), the
-// outputs by their own rounding.
+// (24 bits) of all that the state is made of, T, Y, U and the state itself in S k, whose error Y takes into U
+// and so back into the state, multiplied part by part (for two split operands the six products down to
+// 2^-24); two (16 bits) of what only the outputs, rounded to bf16, are made of: the state in S q, the scores
+// and U beside them. The states are as far from 64 bits as those of float rows: of 128 rows without decay
+// 1.1e-7 of their norm (float rows 2.4e-7; the state in two parts 9e-7, U in two 5e-6). The third part of the
+// state costs 4 to 5% of a prompt's time (4,001 rows 188 -> 196 us, eight ragged prompts 337 -> 354).
 constexpr int kChunk = 32;
 constexpr double kFloor = -1e4;  // exp() of it is 0; log decays below (-inf) are taken as this
 
@@ -654,11 +655,11 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = st[(8 * (k0 + k) + j) % E][(8 * (k0 + k) + j) / E];
-                Parts<2> sp;
+                Parts<3> sp;
                 sp.split(x);
 #pragma unroll
-                for (int p = 1; p >= 0; --p) {
-                    parts[((k0 + k) * 2 + p) * 64] = sp.p[p];
+                for (int p = 2; p >= 0; --p) {
+                    if (p < 2) parts[((k0 + k) * 2 + p) * 64] = sp.p[p];
 #pragma unroll
                     for (int a = 0; a < 2; ++a) pr[a] = mfma(kb[k][a], sp.p[p], pr[a]);
                 }

@@ -104,3 +104,37 @@ class DeltaCase:
         A = (beta.T[..., None] * kk * torch.exp((G[:, :, None] - G[:, None, :]).clamp_max(0))).tril(-1)
         T = torch.linalg.inv(torch.eye(A.shape[-1], dtype=A.dtype) + A)
         return torch.linalg.matrix_norm(T.abs() @ A.abs(), 2)
+
+
+def final_states(c, dt):
+    """The states after the last rows by the recurrence in one type, on the CPU: [sequences, hv, dv, dk]."""
+    q, k, v, g, beta = (t.to(dt) for t in c.operands("cpu"))
+    k = k.repeat_interleave(c.hv // c.hk, 1)
+    out = []
+    for i, n in enumerate(c.lens):
+        S = c.states[int(c.origin[i])].to(dt)
+        for r in range(int(c.off[i]), int(c.off[i]) + n):
+            S = S * torch.exp(g[r])[:, None, None]
+            u = beta[r][:, None] * (v[r] - (S * k[r][:, None, :]).sum(-1))
+            S = S + u[..., None] * k[r][:, None, :]
+        out.append(S)
+    return torch.stack(out)
+
+
+def concentrate_keys(c):
+    """Keys with all their weight on one of four dims: a row's error in them meets no other that cancels it."""
+    at = torch.randint(0, 4, (c.rows, c.hk), generator=c.g)
+    c.qkv[:, c.hk * c.dk:2 * c.hk * c.dk] = torch.nn.functional.one_hot(at, c.dk).view(c.rows, -1).to(BF16)
+
+
+def state_error(states, exact):
+    """[sequences, hv]: the error relative in a head's norm."""
+    return (states.double() - exact).flatten(2).norm(dim=-1) / exact.flatten(2).norm(dim=-1)
+
+
+def state_limit(c, exact):
+    """The error that the chunked form may make in a head's norm. It rounds an element of the state
+    once per chunk and product of operand parts (24 bits) where the recurrence in float rounds it
+    twice per row: twice the recurrence's error covers it, with two float steps where the recurrence
+    happens to be exact (keys of one dim make exact products)."""
+    return 2 * state_error(final_states(c, torch.float32), exact) + 2 * 2 * HALF_F32

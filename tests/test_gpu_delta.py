@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import gpu_util as G
-from delta_cases import BF16, DeltaCase
+from delta_cases import BF16, DeltaCase, concentrate_keys, final_states, state_error, state_limit
 
 pytestmark = pytest.mark.gpu
 
@@ -396,3 +396,19 @@ def test_workspace_is_aligned_to_16_bytes_only(gpu, q38):
     last = c.last.long()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1][last], want[1][last])
     assert (ws[:at] == 0xff).all() and (ws[at + need:] == 0xff).all()
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.001, 0.05, 1.0])
+@pytest.mark.parametrize("keys", ["spread", "concentrated"])
+@pytest.mark.parametrize("heads", list(HEADS))
+def test_chunked_states_are_as_exact_as_float_rows(gpu, q38, heads, keys, decay):
+    """The final states against the recurrence's in 64 bits: delta_cases.state_limit."""
+    hk, hv, dk, dv = HEADS[heads]
+    c = DeltaCase([128, 70], hk, hv, dk, dv, seed=22, decay=decay)
+    if keys == "concentrated":
+        concentrate_keys(c)
+    _, states = run(q38, gpu, c)
+    exact = final_states(c, torch.float64)
+    got = state_error(states[c.last.long()], exact)
+    limit = state_limit(c, exact)
+    assert bool((got <= limit).all()), (got.max().item(), (got / limit).max().item())
