@@ -33,11 +33,10 @@ __device__ __forceinline__ T uniform_load(const T* p) {
 // and 4.9 us for one request. Longer sequences are a chain of two sums over lanes per row; the next row's
 // operands are in flight during a row.
 template <int DK, int R>
-__global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B) {
+__device__ __forceinline__ void walk_rows(const DeltaDev& D, const DeltaBatchDev& B, int s, int h, int dv0) {
     constexpr int C = DK / 32;
-    const int s = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63, sub = lane & 7;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int dv = (blockIdx.x * 4 + wave) * 8 * R + (lane >> 3);  // the lane's first value row, the next 8 on
+    const int lane = threadIdx.x & 63, sub = lane & 7;
+    const int dv = dv0 + (lane >> 3);  // the lane's first value row, the next 8 on
     const int hk = h / (D.hv / D.hk);
     const int first = uniform_load(B.off + s), behind = uniform_load(B.off + s + 1);
     const int from = B.origin ? uniform_load(B.origin + s) : -1, last = B.last ? uniform_load(B.last + s) : -1;
@@ -134,6 +133,12 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B)
     store(last);
 }
 
+template <int DK, int R>
+__global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    walk_rows<DK, R>(D, B, blockIdx.z, blockIdx.y, (blockIdx.x * 4 + wave) * 8 * R);
+}
+
 // ---- the chunked form. Within a chunk of C rows, with G_i the sums of its log decays up to row i,
 // A_ij = beta_i (k_i . k_j) exp(G_i - G_j) for j < i and T = (I + A)^-1, the rows' updates
 // u_i = beta_i (v_i - S k_i) solve a triangular system:
@@ -149,7 +154,7 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B)
 // and so back into the state, multiplied part by part (for two split operands the six products down to
 // 2^-24); two (16 bits) of what only the outputs, rounded to bf16, are made of: the state in S q, the scores
 // and U beside them. The states are as far from 64 bits as those of float rows: of 128 rows without decay
-// 1.1e-7 of their norm (float rows 2.4e-7; the state in two parts 9e-7, U in two 5e-6). The third part of the
+// 1.5e-7 of their norm (float rows 2.3e-7; the state in two parts 9e-7, U in two 5e-6). The third part of the
 // state costs 4 to 5% of a prompt's time (4,001 rows 188 -> 196 us, eight ragged prompts 337 -> 354).
 constexpr int kChunk = 32;
 constexpr double kFloor = -1e4;  // exp() of it is 0; log decays below (-inf) are taken as this
@@ -470,6 +475,23 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     // on every path, so that a wait counts only the loads that it needs. Rows behind the sequence: its last
     // row again, whose update is nothing (its beta in the system is 0).
 
+    // A row's products with the matrices' zeros do not hide an infinity or NaN of a later row of its chunk: U, and
+    // with it the outputs, would be NaN from the chunk's first row on, where the rule is causal. Such a U is in the
+    // state for good, so the state tells at the end: the workgroup then runs its part of the sequence again from
+    // the origin, which nothing has overwritten, row by row (in a healthy model never; 20 times a walk's time).
+    int* const flags = reinterpret_cast<int*>(upd_lds + (chunks & 1) * Geo::kUpd);  // (not in use at the end)
+    auto again = [&] {
+        if (chunks == 0) return false;
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) any |= flags[i];
+        if (__builtin_amdgcn_readfirstlane(any) == 0) return false;
+        __threadfence();  // (the outputs so far are behind those that replace them)
+        __syncthreads();
+        walk_rows<DK, 1>(D, B, s, h, dv + 8 * wave);
+        return true;
+    };
+
     if (outputs) {
         const char* const kb = reinterpret_cast<const char*>(D.k + begin * D.ks + hk * DK);
         const char* const vb = reinterpret_cast<const char*>(D.v + begin * D.vs + h * D.dv + dv);
@@ -589,6 +611,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
             stage_keys((n + 1) & 1);
             lds_barrier();  // (the next chunk's loads stay in flight)
         }
+        again();
         return;
     }
 
@@ -715,7 +738,17 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
         }
         lds_barrier();  // (the next chunk's loads stay in flight)
     }
-    if (chunks > 0) lds_barrier();  // the output waves' last chunk
+    if (chunks > 0) {
+        float sum = 0.0f;  // 0 or NaN
+#pragma unroll
+        for (int o = 0; o < E; ++o)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum = fmaf(st[o][r], 0.0f, sum);
+        const bool strange = __any(sum != 0.0f) && from < B.slots;  // (an origin out of range: NaN as it is)
+        if (lane == 0) flags[part] = strange;
+        lds_barrier();  // the output waves' last chunk
+    }
+    if (again()) return;
     const int to = B.last ? uniform_load(B.last + s) : -1;
     if (to < 0 || to >= B.slots) return;
 #pragma unroll

@@ -412,3 +412,54 @@ def test_chunked_states_are_as_exact_as_float_rows(gpu, q38, heads, keys, decay)
     got = state_error(states[c.last.long()], exact)
     limit = state_limit(c, exact)
     assert bool((got <= limit).all()), (got.max().item(), (got / limit).max().item())
+
+
+@pytest.mark.parametrize("at", [0, 20, 45, 69])
+@pytest.mark.parametrize("what", ["q nan", "q inf", "k nan", "k inf", "v nan", "v inf", "g nan", "beta nan", "beta inf"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_non_finite_operands_reach_only_later_rows(gpu, q38, what, at, in_place):
+    """One element of one row of a prompt is infinite or NaN: what the recurrence in 64 bits keeps finite, the rows
+    before it, other heads and, for a value, other value dims, is as exact as without it, also among the rows
+    of its chunk; the rest is not finite. The other sequence's bits stay."""
+    hk, hv, dk, dv = 2, 4, 64, 128
+    c = DeltaCase([70, 40], hk, hv, dk, dv, seed=23)
+    if in_place:
+        c.last = c.origin.clone()
+    clean_out, clean = run(q38, gpu, c)
+    _, ob, _, sb = c.exact(CHUNK)
+    x = math.nan if what.endswith("nan") else math.inf
+    if what[0] == "q":
+        c.qkv[at, dk + 5] = x                   # of key head 1
+    elif what[0] == "k":
+        c.qkv[at, hk * dk + 5] = x              # of key head 0
+    elif what[0] == "v":
+        c.qkv[at, 2 * hk * dk + dv + 9] = x     # of value head 1
+    elif what[0] == "g":
+        c.g_log[at, 2] = x
+    else:
+        c.beta[at, 3] = x
+    want, _, S, _ = c.exact()
+    out, states = run(q38, gpu, c)
+    assert torch.equal(out[70:], clean_out[70:]) and torch.equal(states[int(c.last[1])], clean[int(c.last[1])])
+    fine = torch.isfinite(want[:70])
+    assert bool(fine.any()) and not bool(fine.all())
+    assert torch.equal(torch.isfinite(out[:70]), fine)
+    assert bool(((out[:70].double() - want[:70]).abs() <= ob[:70])[fine].all())
+    got, want = states[int(c.last[0])].double(), S[69]
+    whole = torch.isfinite(want).all(-1)
+    assert not bool(torch.isfinite(got[~whole]).any())
+    assert bool(((got - want).norm(dim=-1) <= sb[69])[whole].all())
+
+
+def test_non_finite_origin_stays_in_its_value_rows(gpu, q38):
+    c = DeltaCase([50, 33], 1, 2, 64, 64, seed=24)
+    want, ob, S, sb = c.exact(CHUNK)
+    c.states[int(c.origin[0]), 1, 7, 3] = math.nan
+    out, states = run(q38, gpu, c)
+    bad = torch.zeros(c.rows, 2, 64, dtype=torch.bool)
+    bad[:50, 1, 7] = True
+    assert torch.isnan(out[bad].float()).all()
+    assert bool(((out.double() - want).abs() <= ob)[~bad].all())
+    for i, r in ((0, 49), (1, 82)):
+        off = (states[int(c.last[i])].double() - S[r]).norm(dim=-1)
+        assert bool((off <= sb[r])[~bad[r]].all()) and torch.isnan(off[bad[r]]).all()
