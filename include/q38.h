@@ -761,10 +761,12 @@ int q38_paged_append(q38_ctx* ctx, const q38_paged_cache* cache, const q38_paged
  * scale * (q . k_t); query head h reads kv head h / (q_heads / kv_heads); q_heads is at most 256, and
  * 128 per kv head. q and out: device bf16, [q_heads][head_dim] per row at their strides (alignment
  * as for k); they may not overlap. Scores, softmax sums and the output's sums are float, p (in a Q8
- * cache p times the value's scale) is rounded for the product with V, to 16 bits for max_rows *
- * q_heads / kv_heads up to 32 and to bf16 above, out is rounded once; in a bf16 cache the sum that
+ * cache p times the value's scale) is rounded for the product with V, to 16 bits in sequences of
+ * up to 32 queries per kv head (rows * q_heads / kv_heads), whatever the others of the batch are,
+ * and to bf16 or better in longer ones, out is rounded once; in a bf16 cache the sum that
  * divides is of the rounded p. A row that sees no token gives
- * zeros; what unseen places of the cache hold, infinities and NaN too, has no effect. All rows of a
+ * zeros; what unseen places of the cache hold, infinities and NaN too, has no effect; a seen value's
+ * reach its dim of the outputs, as one or the other. All rows of a
  * sequence with tokens behind its table are NaN; a page out of range makes the rows that see it
  * NaN, and may make others of its sequence NaN too. Results do not depend on the other sequences'
  * values, but on their lengths within float rounding (they move the points where the cache is

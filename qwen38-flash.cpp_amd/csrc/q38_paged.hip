@@ -344,11 +344,12 @@ struct AttnState {
     }
 
     // O^T += V^T P^T; the probabilities (with the value's scale in a Q8 cache) are rounded to P bf16 parts
-    // for it. One: each is off by up to 2^-8 of itself, as the output by its own rounding (k_paged_tile, which
-    // a second set of products would slow down by a third). Two: by 2^-17 (k_paged_split, bound by bytes: at
-    // most 2.5% of its time).
+    // for it. One: each is off by up to 2^-8 of itself, as the output by its own rounding (k_paged_tile, many
+    // queries of a sequence; a second part took five ragged prompts from 432 to 535 us). Two: by 2^-17
+    // (sequences of few queries: k_paged_split, bound by bytes, at most 2.5% of its time, and in k_paged_tile a
+    // second wave, whose one part is what the first part leaves: `low`).
     __device__ __forceinline__ void weights(int m, const float (&p)[8], const floatx4 (&vs)[2], int base, int lane,
-                                            uintx4 (&b)[P]) {
+                                            uintx4 (&b)[P], bool low = false) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -363,6 +364,9 @@ struct AttnState {
                 b[n][i] = pack_bf16(x[2 * i], x[2 * i + 1]);
                 if (n + 1 < P) x[2 * i] -= bflo(b[n][i]), x[2 * i + 1] -= bfhi(b[n][i]);
             }
+        if (low)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[0][i] = pack_bf16(x[2 * i] - bflo(b[0][i]), x[2 * i + 1] - bfhi(b[0][i]));
     }
     template <bool CODES>  // the values as 8-bit codes, not as bf16
     __device__ __forceinline__ void products(const ValueTile<D, CODES>& t, const uintx4 (&b)[MT][P]) {
@@ -435,6 +439,7 @@ __device__ __forceinline__ floatx4 add_special(const PagedCacheDev& C, const int
     return x;
 }
 
+constexpr int kSplitQueries = 32;              // queries per sequence and kv head that it is for
 constexpr int kSplitWaves = 4;                 // waves of a workgroup
 constexpr int kSplitTokens = 32 * kSplitWaves; // tokens of a step
 
@@ -719,6 +724,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     using Geo = AttnGeo<D, false>;
     using TG = TileGeo<D>;
     constexpr int TB = TG::TB, NT = 64 * TG::WAVES, CH = TG::CH, PC = TG::PIECES, MT = TG::MT;
+    constexpr int F = kSplitQueries / (16 * MT);
     extern __shared__ uintx4 tiles[];  // [2][keys, values][TB][CH], then [2][key, value scales][TB]
     float* const scales = reinterpret_cast<float*>(tiles + 4 * TB * CH);
     const AttnSplit S{G, TG::M, kSplitTokens};
@@ -727,7 +733,6 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
     const int per_xcd = gridDim.x / 8, n = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
     if (n >= shares * C.hkv) return;
     const int head = n / shares, place = n % shares, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int m0 = wave * 16 * MT;
     const bool negate = c < 0.0f;
     c = fabsf(c);
     __shared__ ShareWalk walks[TG::WAVES];
@@ -741,6 +746,13 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
         asm volatile("" : "+v"(lane));
         const int u = lane & 15, w = lane >> 4;
         AttnItem it = sw.item(S);
+        // A sequence of few queries, beside a longer one that brought the batch here, has its probabilities in two
+        // bf16 parts as in k_paged_split (its error must not grow when a prompt joins its batch): the first F waves
+        // hold its queries, the next F, idle otherwise, the same queries with the parts that the first ones'
+        // rounding leaves, and the sums are added at the end (33 requests of a row or two in a batch that came
+        // here: 100 -> 113 us; both parts in one wave's loop 120 us, and the prompts' loop 5% slower).
+        const bool few = it.rows * G <= kSplitQueries, low = few && wave >= F && wave < 2 * F;
+        const int m0 = (low ? wave - F : wave) * 16 * MT;
         QueryTile<D, false, MT> qt;
         AttnState<D, Q8, MT, 1> st;
         qt.load(q, qs, it, S, head, m0, negate, lane);
@@ -858,7 +870,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
             for (int m = 0; m < MT; ++m) {
                 float p[8];
                 st.soften(m, s[m], ks, c, base, masked, lane, p);
-                st.weights(m, p, vs, base, lane, b[m]);
+                st.weights(m, p, vs, base, lane, b[m], low);
             }
             if constexpr (D == 256) read_values();
             if constexpr (!Q8)
@@ -890,6 +902,29 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
             }
         }
         const bool bad = __syncthreads_or(it.bad || (it.see > 0 && walk.bad));
+        if (few) {
+            static_assert(F * MT * (Geo::E + 1) * 64 <= 4 * TB * CH, "the staged tiles' place holds the sums");
+            uintx4* const place = tiles + (low ? wave - F : wave) * MT * (Geo::E + 1) * 64 + lane;
+            if (low)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                    for (int o = 0; o < Geo::E; ++o)
+                        place[(m * (Geo::E + 1) + o) * 64] = __builtin_bit_cast(uintx4, st.o[m][o]);
+                    place[(m * (Geo::E + 1) + Geo::E) * 64] = __builtin_bit_cast(uintx4, st.all[m]);
+                }
+            __syncthreads();
+            if (wave < F)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                    for (int o = 0; o < Geo::E; ++o)
+                        st.o[m][o] += __builtin_bit_cast(floatx4, place[(m * (Geo::E + 1) + o) * 64]);
+                    // (in a Q8 cache the sum is of the probabilities themselves)
+                    if constexpr (!Q8) st.all[m] += __builtin_bit_cast(floatx4, place[(m * (Geo::E + 1) + Geo::E) * 64]);
+                }
+            __syncthreads();
+        }
         asm volatile("" ::: "memory");  // (read anew: see ShareWalk)
         it = sw.item(S);
         const bool whole = sw.to - sw.from == it.steps;
@@ -903,7 +938,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
         for (int m = 0; m < MT; ++m) {
             float sum = st.total(m);
             if (bad) sum = kNan;
-            const int i = m0 + 16 * m + u, row = tile_row(S, it, i);
+            const int i = m0 + 16 * m + u, row = low ? -1 : tile_row(S, it, i);
             if (row < 0) continue;
             const float inv = bad || st.lim[m] > 0 ? 1.0f / sum : 0.0f;
             uint16_t* dst = out + (it.first + row) * os + (head * G + i % G) * D;
@@ -921,7 +956,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
             if (!whole && w == 0) pd[TG::M * D + i] = st.top[m], pd[TG::M * D + TG::M + i] = sum;
         }
         if constexpr (!Q8)
-            if (special) {  // to what the lane has just written
+            if (special && !low) {  // to what the lane has just written
     #pragma unroll 1
                 for (int n = 0; n < MT * Geo::E; ++n) {
                     const int i = m0 + 16 * (n / Geo::E) + u, row = tile_row(S, it, i);
@@ -1051,7 +1086,7 @@ AttnPlan attn_plan(const PagedCacheDev& C, const PagedBatchDev& B, int max_rows,
     AttnPlan p{};
     const int G = hq / C.hkv;
     const int64_t queries = static_cast<int64_t>(max_rows) * G;
-    p.tiles = queries > 32;
+    p.tiles = queries > kSplitQueries;
     p.mt = queries <= 16 ? 1 : 2;
     p.M = !p.tiles ? 16 * p.mt : C.d == 256 ? TileGeo<256>::M : TileGeo<128>::M;
     p.W = std::max(1, 256 * (p.tiles || C.d == 256 ? 1 : 2) / C.hkv);  // the chip's 256 CUs at the kernels' occupancy

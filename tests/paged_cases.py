@@ -9,6 +9,7 @@ import torch
 BF16 = torch.bfloat16
 HALF_BF16 = torch.finfo(BF16).eps / 2   # the largest relative error of one rounding to bf16
 HALF_F32 = torch.finfo(torch.float32).eps / 2
+HALF_16 = 2.0 ** -17                    # of a rounding to two bf16 parts, 16 bits
 
 
 class Batch:
@@ -69,8 +70,9 @@ def values64(x, scales):
     return x.double() if scales is None else x.double() * scales.double()[..., None]
 
 
-def attention64(b: Batch, keys, values, ks, vs, q, scale):
+def attention64(b: Batch, keys, values, ks, vs, q, scale, half=HALF_BF16):
     """(out, bound) in float64 for every row of the batch, NaN for rows that no sequence owns.
+    half: the probabilities' half step, HALF_16 where a sequence has few queries.
     bound: half a bf16 step of the result, half a step of every probability against what it
     multiplies, and the float sums (D products per score, relative in the probabilities; one
     sum over the tokens)."""
@@ -96,5 +98,27 @@ def attention64(b: Batch, keys, values, ks, vs, q, scale):
                 # (twice the first-order float error of a score: its own and that of the maximum)
                 err = 2 * abs(scale) * (k.abs() @ x.abs()).max() * (D + 8) * 2 * HALF_F32 + 2 * s.abs().max() * HALF_F32 * 4
                 size = w @ v.abs()
-                bound[row, h] = HALF_BF16 * out[row, h].abs() + size * (HALF_BF16 * 1.01 + 2 * err + (see + 64) * HALF_F32)
+                bound[row, h] = HALF_BF16 * out[row, h].abs() + size * (half * 1.01 + 2 * err + (see + 64) * HALF_F32)
     return out, bound
+
+
+def cancel_values(b: Batch, cache, q, scale):
+    """Sets the value of every sequence's last token so that the outputs of its last row nearly vanish beside
+    the terms that they are sums of (exactly, but for its own rounding, for the first query of each kv
+    head; the others' probabilities are close where the scale is small): then the rounding of an output hides
+    nothing of the probabilities'."""
+    keys, values, ks, vs = cache
+    G = q.shape[1] // b.hkv
+    for i in range(len(b.lens)):
+        p, o = b.places(i)
+        if b.lens[i] == 0 or len(p) < 2:
+            continue
+        K = values64(keys[p, :, o], None if ks is None else ks[p, :, o])
+        V = values64(values[p, :, o], None if vs is None else vs[p, :, o])
+        for h in range(b.hkv):
+            w = torch.softmax((K[:, h] @ q[int(b.off[i + 1]) - 1, h * G].double()) * scale, 0)
+            v = -(w[:-1] @ V[:-1, h]) / w[-1]
+            if vs is not None:
+                vs[p[-1], h, o[-1]] = v.abs().max() / 127
+                v = torch.round(v / vs[p[-1], h, o[-1]].double())
+            values[p[-1], h, o[-1]] = v.to(values.dtype)

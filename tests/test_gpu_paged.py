@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import gpu_util as G
-from paged_cases import BF16, HALF_F32, Batch, attention64
+from paged_cases import BF16, HALF_16, HALF_F32, Batch, attention64, cancel_values
 
 pytestmark = pytest.mark.gpu
 
@@ -531,3 +531,30 @@ def test_workspace_is_aligned_to_16_bytes_only(gpu, q38, rows, tokens):
     assert view.data_ptr() % 32 == 16
     assert torch.equal(run_attend(q38, gpu, b, cache, q, 0.09, ws=view), want)
     assert (ws[:48 - ws.data_ptr() % 32] == 0xff).all() and (ws[48 - ws.data_ptr() % 32 + need:] == 0xff).all()
+
+
+@pytest.mark.parametrize("lengths", ["decode", "verify", "beside_a_prompt", "hint"])
+@pytest.mark.parametrize("geo", ["family", "gqa4_128", "mha_64", "mqa_wide"])
+@pytest.mark.parametrize("q8", [False, True])
+def test_few_queries_have_16_bit_probabilities(gpu, q38, geo, lengths, q8):
+    """Sequences of up to 32 queries per kv head, alone and where a prompt of the batch (or a hint of one)
+    brings the kernel for many queries: outputs that nearly cancel show the probabilities' rounding."""
+    hkv, group, dim = GEOS[geo]
+    few = 32 // group
+    rows = {"decode": [1, 1, 1], "verify": [few, 1, few], "beside_a_prompt": [1, few, 150, 1], "hint": [few, 1, 1]}[lengths]
+    tokens = [30, 200, 777, 1500][:len(rows)]
+    b = Batch(rows, tokens, hkv=hkv, dim=dim, seed=62)
+    if lengths == "hint":
+        b.max_rows = b.rows
+    cache, scale = b.cache(q8), 0.005
+    q = b.randn(b.rows, hkv * group, dim).to(BF16)
+    cancel_values(b, cache, q, scale)
+    got = run_attend(q38, gpu, b, cache, q, scale).double()
+    for i, n in enumerate(rows):
+        if n * group > 32:
+            continue
+        a, e = int(b.off[i]), int(b.off[i + 1])
+        one = Batch([n], [tokens[i]], hkv=hkv, dim=dim)
+        one.table = b.table[i:i + 1]
+        want, bound = attention64(one, *cache, q[a:e], scale, HALF_16)
+        assert bool(((got[a:e] - want).abs() <= bound).all()), (i, float(((got[a:e] - want).abs() / bound).max()))
