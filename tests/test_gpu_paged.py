@@ -558,3 +558,25 @@ def test_few_queries_have_16_bit_probabilities(gpu, q38, geo, lengths, q8):
         one.table = b.table[i:i + 1]
         want, bound = attention64(one, *cache, q[a:e], scale, HALF_16)
         assert bool(((got[a:e] - want).abs() <= bound).all()), (i, float(((got[a:e] - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("rows,tokens", [([6], 3000), ([1], 1700), ([16], 1029), ([90], 4000)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("back", [0, 1, 5, 200, 600])
+def test_non_finite_values_in_pieces(gpu, q38, rows, tokens, dim, back):
+    """An infinite and a NaN value, `back` tokens before the last one, of a sequence whose tokens are cut into
+    many workgroups' pieces: in the last step, among the new rows, and in pieces that every row sees whole."""
+    n = rows[0]
+    b = Batch(rows, [tokens], hkv=2, dim=dim, seed=46)
+    cache = b.cache(False)
+    q = b.randn(b.rows, 4, dim).to(BF16)
+    clean = run_attend(q38, gpu, b, cache, q, 0.1)
+    page, at = b.places(0)
+    cache[1][page[-1 - back], :, at[-1 - back], 3] = math.inf
+    cache[1][page[-1 - back], :, at[-1 - back], dim - 1] = math.nan
+    got = run_attend(q38, gpu, b, cache, q, 0.1)
+    sees = torch.arange(n) >= n - 1 - back  # the rows that see the token
+    assert torch.equal(got[~sees], clean[~sees])
+    assert not torch.isfinite(got[sees][..., [3, dim - 1]].float()).any()
+    keep = [i for i in range(dim) if i not in (3, dim - 1)]
+    assert torch.equal(got[sees][..., keep], clean[sees][..., keep])
