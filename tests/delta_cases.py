@@ -138,3 +138,14 @@ def state_limit(c, exact):
     twice per row: twice the recurrence's error covers it, with two float steps where the recurrence
     happens to be exact (keys of one dim make exact products)."""
     return 2 * state_error(final_states(c, torch.float32), exact) + 2 * 2 * HALF_F32
+
+
+def output_error(out, want):
+    """[hv]: the norm of a head's error over all rows."""
+    return (out.double() - want).transpose(0, 1).flatten(1).norm(dim=-1)
+
+
+def output_limit(want):
+    """The norm of the error that rounding the exact outputs makes, and 5% for what is off before it:
+    16-bit operands, 2^-9 of a rounding, turn a few roundings the other way."""
+    return 1.05 * output_error(want.to(BF16), want)

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import gpu_util as G
-from delta_cases import BF16, DeltaCase, concentrate_keys, final_states, state_error, state_limit
+from delta_cases import (BF16, DeltaCase, concentrate_keys, final_states, output_error, output_limit, state_error,
+                         state_limit)
 
 pytestmark = pytest.mark.gpu
 
@@ -463,3 +464,16 @@ def test_non_finite_origin_stays_in_its_value_rows(gpu, q38):
     for i, r in ((0, 49), (1, 82)):
         off = (states[int(c.last[i])].double() - S[r]).norm(dim=-1)
         assert bool((off <= sb[r])[~bad[r]].all()) and torch.isnan(off[bad[r]]).all()
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.05, 1.0])
+@pytest.mark.parametrize("keys", ["spread", "concentrated"])
+@pytest.mark.parametrize("heads", list(HEADS))
+def test_chunked_outputs_are_off_by_their_rounding(gpu, q38, heads, keys, decay):
+    c = DeltaCase([128, 70], *HEADS[heads], seed=25, decay=decay)
+    if keys == "concentrated":
+        concentrate_keys(c)
+    out, _ = run(q38, gpu, c)
+    want = c.exact()[0]
+    got, limit = output_error(out, want), output_limit(want)
+    assert bool((got <= limit).all()), float((got / limit).max())
