@@ -265,7 +265,14 @@ struct AttnState {
     // second product's B operand, and their sum. MASKED steps: some query does not see all tokens.
     __device__ __forceinline__ void soften(int m, const floatx4 (&s)[2], const floatx4 (&ks)[2], float c, int base,
                                            bool masked, int lane, float (&p)[8]) {
-        const int first = base + 8 * (lane >> 4);
+        // (opaque: the compiler would share the comparisons of the two masks and make them in front of the branches, in
+        // every step, or not, by what else the kernel holds: five ragged prompts 453 us in place of 430. With 256
+        // dims, 16 queries per wave, sharing is better: ragged prompts 341 us against 344, in 8 bits 319 against 322.)
+        auto seen_from = [&] {
+            int first = base + 8 * (lane >> 4) - lim[m];
+            if constexpr (D < 256) asm volatile("" : "+v"(first));
+            return first;
+        };
         float best = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -273,8 +280,9 @@ struct AttnState {
             if constexpr (Q8) p[j] *= ks[j >> 2][j & 3];
         }
         if (masked) {
+            const int first = seen_from();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = first + j < lim[m] ? p[j] : -INFINITY;
+            for (int j = 0; j < 8; ++j) p[j] = first + j < 0 ? p[j] : -INFINITY;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) best = fmaxf(best, p[j]);
@@ -296,8 +304,9 @@ struct AttnState {
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], c, -ref));
         if (masked) {
+            const int first = seen_from();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = first + j < lim[m] ? p[j] : 0.0f;
+            for (int j = 0; j < 8; ++j) p[j] = first + j < 0 ? p[j] : 0.0f;
         }
         if constexpr (Q8) {
 #pragma unroll
