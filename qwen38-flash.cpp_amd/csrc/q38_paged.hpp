@@ -102,22 +102,29 @@ __host__ __device__ inline void attn_tile(const AttnSplit& S, int tile, AttnItem
     it->see = attn_see(*it, (behind < it->rows ? behind : it->rows) - 1);
     it->steps = it->see > S.T ? (it->see + S.T - 1) / S.T : 1;
 }
-// sum over i < n of floor((a i + b) / m), by Euclid's steps (the lattice points under a line)
+// sum over i < n of floor((a i + b) / m). Whole parts of a / m and b / m come out of the sum; what is left, a and
+// b below m, counts for every height j = 1 .. top (the last term) the i with a i + b >= m j, n - ceil((m j - b) / a)
+// of them, so it is n top less a sum of the same kind over the heights, with a and m exchanged as in Euclid's
+// algorithm (counting the points under a line by rows in place of columns: Graham, Knuth, Patashnik,
+// Concrete Mathematics, chapter 3).
 __host__ __device__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     int64_t sum = 0;
-    while (n) {
-        sum += static_cast<int64_t>(n - 1) * n / 2 * (a / m) + static_cast<int64_t>(n) * (b / m);
+    for (bool less = false;; less = !less) {
+        const int64_t pairs = static_cast<int64_t>(n) * (static_cast<int64_t>(n) - 1) / 2;
+        int64_t part = pairs * (a / m) + static_cast<int64_t>(n) * (b / m);
         a %= m;
         b %= m;
-        const uint32_t top = a * n + b;
-        if (top < m) break;
-        n = top / m;
-        b = top % m;
-        const uint32_t t = m;
-        m = a;
-        a = t;
+        const uint32_t top = n ? (a * (n - 1) + b) / m : 0;
+        part += static_cast<int64_t>(n) * top;
+        sum += less ? -part : part;
+        if (top == 0) return sum;
+        // (j = heights + 1: ceil((m (heights + 1) - b) / a) = floor((m heights + m - b + a - 1) / a))
+        b = m - b + a - 1;
+        const uint32_t columns = a;
+        a = m;
+        m = columns;
+        n = top;
     }
-    return sum;
 }
 // Steps of the sequence's tiles 0 .. n - 1 (n <= its tiles; all but its last tile have their R rows).
 __host__ __device__ inline int64_t attn_before(const AttnSplit& S, const AttnItem& it, int n) {
