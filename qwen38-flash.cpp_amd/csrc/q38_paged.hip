@@ -785,7 +785,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
         raw_t kr[PC], vr[PC];
         float sr[2] = {0.0f, 0.0f};
         auto fetch = [&](int t0) {
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < PC; ++i) {
                 const int64_t at = walk.half(t0 + i * (NT / CH) + wt) * (D * EL);
                 kr[i] = *reinterpret_cast<const raw_t*>(static_cast<const char*>(C.keys) + at + lane_off);
@@ -805,7 +805,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
                 return x;
         };
         auto stage = [&](int buf) {
-    #pragma unroll
+#pragma unroll
             for (int i = 0; i < PC; ++i) {
                 const int at = tile_at<D>(i * (NT / CH) + wt + lane / CH, ch);
                 tiles[(2 * buf) * TB * CH + at] = widen(kr[i]);
@@ -823,59 +823,59 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
             auto key = [&](int a, int i) { return kt[tile_at<D>(32 * sub + 8 * (u >> 2) + 4 * a + (u & 3), 4 * i + w)]; };
             ValueTile<D, false> v;
             auto read_values = [&] {
-    #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int t = 32 * sub + 8 * w + j;
                     if constexpr (D == 64) {
                         const uint2 x = reinterpret_cast<const uint2*>(vt + tile_at<D>(t, u >> 1))[u & 1];
                         v.v[j][0] = x.x, v.v[j][1] = x.y;
                     } else {
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < D / 128; ++b) {
                             const uintx4 x = vt[tile_at<D>(t, 16 * b + u)];
-    #pragma unroll
+#pragma unroll
                             for (int i = 0; i < 4; ++i) v.v[j][4 * b + i] = x[i];
                         }
                     }
                 }
             };
             floatx4 s[MT][2], ks[2], vs[2];
-    #pragma unroll
+#pragma unroll
             for (int a = 0; a < 2; ++a)
-    #pragma unroll
+#pragma unroll
                 for (int m = 0; m < MT; ++m) s[m][a] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (D < 256) {  // all reads in flight before the first product, the values' before the softmax
                 uintx4 k[2][Geo::KS];
-    #pragma unroll
+#pragma unroll
                 for (int a = 0; a < 2; ++a)
-    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < Geo::KS; ++i) k[a][i] = key(a, i);
                 __builtin_amdgcn_sched_barrier(0);
-    #pragma unroll
+#pragma unroll
                 for (int a = 0; a < 2; ++a)
-    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < Geo::KS; ++i)
-    #pragma unroll
+#pragma unroll
                         for (int m = 0; m < MT; ++m) s[m][a] = mfma(k[a][i], qt.q[m][i], s[m][a]);
                 read_values();
             } else {  // (256 dims: no registers for them)
-    #pragma unroll
+#pragma unroll
                 for (int a = 0; a < 2; ++a)
-    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < Geo::KS; ++i) {
                         const uintx4 k = key(a, i);
-    #pragma unroll
+#pragma unroll
                         for (int m = 0; m < MT; ++m) s[m][a] = mfma(k, qt.q[m][i], s[m][a]);
                     }
             }
             if constexpr (Q8)
-    #pragma unroll
+#pragma unroll
                 for (int a = 0; a < 2; ++a) {
                     ks[a] = *reinterpret_cast<const floatx4*>(sc + 32 * sub + 8 * w + 4 * a);
                     vs[a] = *reinterpret_cast<const floatx4*>(sc + TB + 32 * sub + 8 * w + 4 * a);
                 }
             uintx4 b[MT][1];
-    #pragma unroll
+#pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float p[8];
                 st.soften(m, s[m], ks, c, base, masked, lane, p);
@@ -943,7 +943,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
             pd = part + (static_cast<int64_t>(n) * 2 + slot) * (TG::M * (D + 2));
             if (slot && threadIdx.x == 0) note_cut(cut, sw, it);
         }
-    #pragma unroll
+#pragma unroll
         for (int m = 0; m < MT; ++m) {
             float sum = st.total(m);
             if (bad) sum = kNan;
@@ -951,9 +951,9 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
             if (row < 0) continue;
             const float inv = bad || st.lim[m] > 0 ? 1.0f / sum : 0.0f;
             uint16_t* dst = out + (it.first + row) * os + (head * G + i % G) * D;
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 4; ++r)
-    #pragma unroll
+#pragma unroll
                 for (int o = 0; o < Geo::E; o += 4) {
                     const int d = Geo::dim(4 * w + r, o);
                     const floatx4 x = {st.o[m][o][r], st.o[m][o + 1][r], st.o[m][o + 2][r], st.o[m][o + 3][r]};
@@ -966,7 +966,7 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
         }
         if constexpr (!Q8)
             if (special && !low) {  // to what the lane has just written
-    #pragma unroll 1
+#pragma unroll 1
                 for (int n = 0; n < MT * Geo::E; ++n) {
                     const int i = m0 + 16 * (n / Geo::E) + u, row = tile_row(S, it, i);
                     if (row < 0) continue;
