@@ -477,3 +477,38 @@ def test_chunked_outputs_are_off_by_their_rounding(gpu, q38, heads, keys, decay)
     want = c.exact()[0]
     got, limit = output_error(out, want), output_limit(want)
     assert bool((got <= limit).all()), float((got / limit).max())
+
+
+@pytest.mark.parametrize("dk", [64, 128, 256])
+@pytest.mark.parametrize("dv", [64, 128, 256])
+def test_sequences_run_again_at_every_size(gpu, q38, dk, dv):
+    """A NaN value and, in another sequence, an infinite key: rows before them as without them, whatever the
+    sizes; captured, and replayed over the same slots."""
+    c = DeltaCase([50, 33, 90], 2, 4, dk, dv, seed=26)
+    want, ob, S, sb = c.exact(CHUNK)
+    clean_out, clean = run(q38, gpu, c)
+    c.qkv[40, 2 * 2 * dk + 3 * dv + dv - 1] = math.nan
+    c.qkv[50 + 33 + 77, 2 * dk + dk - 1] = math.inf        # of key head 0: value heads 0 and 1
+    bad = torch.zeros(c.rows, 4, dv, dtype=torch.bool)
+    bad[40:50, 3, dv - 1] = True
+    bad[160:, :2] = True
+    states = c.states.cuda()
+    rule = q38.DeltaRule(gpu, 2, 4, dk, dv, c.scale)
+    batch = q38.DeltaBatch(states, c.off.cuda(), c.origin.cuda(), c.last.cuda(), c.rows, c.max_rows)
+    ops, out = c.operands("cuda"), torch.zeros(c.rows, 4, dv, dtype=BF16, device="cuda")
+    ws = G.workspace(max(16, rule.workspace_size(batch)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rule.run(batch, *ops, out, ws, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        out.fill_(3.0)
+        states[c.last.long().cuda()] = 5.0
+        graph.replay()
+        torch.cuda.synchronize()
+        got, now = out.cpu(), states.cpu()
+        assert torch.equal(torch.isfinite(got), ~bad)
+        assert bool(((got.double() - want).abs() <= ob)[~bad].all())
+        for i, r in enumerate((49, 82, 172)):
+            off = (now[int(c.last[i])].double() - S[r]).norm(dim=-1)
+            assert bool((off <= sb[r])[~bad[r]].all()) and not bool(torch.isfinite(off[bad[r]]).any())
+        assert torch.equal(got[50:83], clean_out[50:83]) and torch.equal(now[int(c.last[1])], clean[int(c.last[1])])

@@ -580,3 +580,32 @@ def test_non_finite_values_in_pieces(gpu, q38, rows, tokens, dim, back):
     assert not torch.isfinite(got[sees][..., [3, dim - 1]].float()).any()
     keep = [i for i in range(dim) if i not in (3, dim - 1)]
     assert torch.equal(got[sees][..., keep], clean[sees][..., keep])
+
+
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 8), (256, 8), (256, 16)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_few_queries_beside_a_prompt_with_bad_tokens(gpu, q38, dim, group, q8):
+    """Sequences of few queries in the kernel for many: an infinity that only the last row sees, a NaN that all
+    see, a page out of range and tokens behind the table; over several pieces."""
+    n = 32 // group
+    b = Batch([n, n, n, n, 120, 1], [900, 700, 800, 30, 300, 5], hkv=2, dim=dim, seed=47)
+    cache = b.cache(q8)
+    q = b.randn(b.rows, 2 * group, dim).to(BF16)
+    clean = run_attend(q38, gpu, b, cache, q, 0.1)
+    check_attend(b, cache, q, 0.1, clean)
+    bad = cache[3] if q8 else cache[1][..., 7]   # a token's value scales, or one dim of its values
+    p, o = b.places(0)
+    bad[p[-1], :, o[-1]] = math.inf
+    p, o = b.places(1)
+    bad[p[40], :, o[40]] = math.nan
+    b.table[2, 3] = b.pages
+    b.tokens[3] = b.width * b.page + 1
+    got = run_attend(q38, gpu, b, cache, q, 0.1)
+    off = b.off.tolist()
+    dims = list(range(dim)) if q8 else [7]
+    keep = [] if q8 else [i for i in range(dim) if i != 7]
+    assert torch.equal(got[:n - 1], clean[:n - 1]) and torch.equal(got[off[4]:], clean[off[4]:])
+    for rows in (slice(n - 1, n), slice(off[1], off[2])):
+        assert not torch.isfinite(got[rows][..., dims].float()).any()
+        assert torch.equal(got[rows][..., keep], clean[rows][..., keep])
+    assert torch.isnan(got[off[2]:off[4]].float()).all()
