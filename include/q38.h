@@ -787,7 +787,7 @@ int q38_paged_attention(q38_ctx* ctx, const q38_paged_cache* cache, const q38_pa
  * of 32 rows on the matrix cores, with states as exact as float ones (operands split into bf16
  * parts) and outputs as their own rounding; others, and calls with checkpoints, run row by row.
  * Infinities and NaN among a sequence's operands reach its later rows and its state and nothing
- * else (a chunked sequence whose state ends with one is run again row by row, at 20 times the
+ * else (a chunked sequence whose state ends with one is run again row by row, at 12 times the
  * time). The workspace is 16-byte aligned.
  * States: a pool [slots][value_heads][value_dim][key_dim] of floats, 16-byte aligned. origin[i]:
  * the slot a sequence starts from, negative (or a null array) for the zero state; final_slots[i]:

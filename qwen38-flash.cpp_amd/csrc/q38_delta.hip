@@ -30,7 +30,7 @@ __device__ __forceinline__ T uniform_load(const T* p) {
 // A wave takes 8 R value rows of one head of one sequence: 8 lanes per value row, lane `sub` of them
 // key dims 32 c + 4 sub .. + 3 (16-byte state accesses, 128 bytes together per row). Single tokens are
 // bound by the states' bytes: 104 us for 128 requests of 32 heads [128][128], 5.2 TB/s, a copy's rate,
-// and 4.9 us for one request. Longer sequences are a chain of two sums over lanes per row; the next row's
+// and 4.8 us for one request. Longer sequences are a chain of two sums over lanes per row; the next row's
 // operands are in flight during a row.
 template <int DK, int R>
 __device__ __forceinline__ void walk_rows(const DeltaDev& D, const DeltaBatchDev& B, int s, int h, int dv0) {
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaDev D, DeltaBatchDev B)
 // 2^-24); two (16 bits) of what only the outputs, rounded to bf16, are made of: the state in S q, the scores
 // and U beside them. The states are as far from 64 bits as those of float rows: of 128 rows without decay
 // 1.5e-7 of their norm (float rows 2.3e-7; the state in two parts 9e-7, U in two 5e-6). The third part of the
-// state costs 4 to 5% of a prompt's time (4,001 rows 188 -> 196 us, eight ragged prompts 337 -> 354).
+// state costs about 4% of a prompt's time (4,001 rows 188 -> 196 us in a pass).
 constexpr int kChunk = 32;
 constexpr double kFloor = -1e4;  // exp() of it is 0; log decays below (-inf) are taken as this
 
@@ -226,9 +226,10 @@ __device__ __forceinline__ bool find_chunk(const DeltaBatchDev& B, int want, int
     return false;
 }
 // The sequence that the slot-th group of workgroups takes. A walk is one chain per head, so the longest
-// sequences begin first; where all groups are on the chip at once, two workgroups per CU, those of the
-// second half join the first half's in the opposite order, the shortest beside the longest (eight ragged
-// prompts in their own order: 377 us, so: 352). Up to 64 sequences; more fill the chip in any order.
+// sequences begin first (eight ragged prompts of 32 heads in their own order 368 us, so 348); where all
+// groups are on the chip at once, two workgroups per CU, those of the second half join the first half's in
+// the opposite order, the shortest beside the longest (eight of 16 heads in their own order 168 us, longest
+// first 158, so 156). Up to 64 sequences; more fill the chip in any order.
 __device__ __forceinline__ int nth_sequence(const DeltaBatchDev& B, int slot, int groups_per_round) {
     if (B.seqs > 64 || B.seqs == 1) return slot;
     const int lane = threadIdx.x & 63;
@@ -421,10 +422,11 @@ __global__ __launch_bounds__(64) void k_delta_system(DeltaDev D, DeltaBatchDev B
 // does not need is left to a second wave on another SIMD: two state waves (32 value columns) go with two output
 // waves, of 16 rows of the chunk each, which take the operands of S and U through LDS a chunk later, load the
 // keys and values and stage them as the state waves want them (the keys as stored and, pairs of rows
-// interleaved, as operands of K^T). A prompt of 4,001 rows: 150 us, 1.2 us a chunk, bound by the state wave's
-// own 400 instructions (one wave doing all: 240 us). Eight ragged prompts, 16,192 rows, two workgroups per CU:
-// 317 us, bound by the vector memory path, which takes a cycle per row that neighbouring lanes do not share
-// (output waves by columns, each with all queries, scores and short stores of its own: 345 us).
+// interleaved, as operands of K^T). A prompt of 4,001 rows: 170 us, 1.35 us a chunk, bound by the state wave's
+// own 500 instructions (161 us with two parts of the state; one wave doing all, before, took 80 us more). Eight
+// ragged prompts, 16,192 rows, two workgroups per CU: 339 us with their systems, bound by the vector memory
+// path, which takes a cycle per row that neighbouring lanes do not share (output waves by columns, each with
+// all queries, scores and short stores of its own, took 8% longer).
 template <int DK>
 struct WalkGeo {
     static constexpr int E = DK / 16, KS = DK / 32, CH = DK / 8;
@@ -450,8 +452,8 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     const int part = wave % NW;  // a state wave's 16 columns, an output wave's 16 rows of the chunk
     const bool outputs = wave >= NW;
     // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: those of one head, which read the
-    // same chunk systems, keys and queries, are one XCD's (spread over the XCDs eight ragged prompts took 7%
-    // longer).
+    // same chunk systems, keys and queries, are one XCD's (spread over the XCDs eight ragged prompts take
+    // 393 us in place of 348).
     const int groups = D.dv / (16 * NW), turn = blockIdx.x / 8, chain = turn / groups * 8 + blockIdx.x % 8;
     if (chain >= D.hv * B.seqs) return;
     const int h = chain % D.hv, hk = h / (D.hv / D.hk);
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
     // A row's products with the matrices' zeros do not hide an infinity or NaN of a later row of its chunk: U, and
     // with it the outputs, would be NaN from the chunk's first row on, where the rule is causal. Such a U is in the
     // state for good, so the state tells at the end: the workgroup then runs its part of the sequence again from
-    // the origin, which nothing has overwritten, row by row (in a healthy model never; 20 times a walk's time).
+    // the origin, which nothing has overwritten, row by row (in a healthy model never; 4,001 rows 2.4 ms).
     int* const flags = reinterpret_cast<int*>(upd_lds + (chunks & 1) * Geo::kUpd);  // (not in use at the end)
     auto again = [&] {
         if (chunks == 0) return false;
@@ -759,10 +761,12 @@ __global__ __launch_bounds__(128 * WalkGeo<DK>::NW, 2) void k_delta_chunks(Delta
                 (floatx4){st[o][r], st[o + 1][r], st[o + 2][r], st[o + 3][r]};
 }
 
-// Sequences of up to so many rows go row by row. By rows and in chunks, 32 heads [128][128]: one sequence of
-// 24 rows 20.3 and 15.0 us, eight 29.6 and 28.9; 64 of 24 rows 158 and 170, of 32 rows 201 and 176 (16 heads
-// [256][256]: 321 and 379, 418 and 389; 8 heads [64][64]: 19.3 and 24.9, 24.0 and 25.5). 16 rows by rows: 15.1,
-// 22.5 and 119.
+// Sequences of up to so many rows go row by row. By rows and in chunks, us, 32 heads [128][128] / 16 [256][256] /
+// 8 [64][64]: one sequence of 24 rows 18.6 and 15.2 / 26.5 and 18.2 / 13.1 and 13.3; eight of 16 rows 21.9 and
+// 27.7 / 33.0 and 49.2 / 9.7 and 14.4, of 24 rows 28.0 and 28.0 / 43.4 and 49.8 / 13.1 and 14.2; 64 of 24 rows
+// 158 and 172 / 318 and 391 / 18.3 and 27.5, of 28 rows 178 and 175 / 358 and 393 / 20.8 and 27.5, of 32 rows
+// 196 and 179 / 398 and 395 / 23.2 and 27.7. (Few small heads would go by rows a little longer: 4 us of one call,
+// which the rule leaves out.)
 bool by_rows(const DeltaBatchDev& B, int max_rows) {
     return B.ckpt || B.rows == 0 || max_rows <= (B.seqs < 32 ? 16 : 28);
 }

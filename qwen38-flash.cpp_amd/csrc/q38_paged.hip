@@ -706,12 +706,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_split(PagedCach
 // converted on the way: its codes are exact in bf16), and every wave multiplies them with its own 32
 // queries. Bound by the matrix cores, by the exponentials beside them (8 per lane for 16 products of 128
 // dims) and by LDS reads, which 32 queries per wave bring to the matrix cores' own time: five ragged
-// prompts, 5,647 rows of 32 heads of 128 over 20,306 tokens, in 473 us, 633 TFLOP/s (4.9 ms with k_paged_split).
+// prompts, 5,647 rows of 32 heads of 128 over 20,306 tokens, in 430 us with their join, 697 TFLOP/s (4.9 ms
+// with k_paged_split).
 template <int D>
 struct TileGeo {
     // One workgroup of two waves per SIMD fills a CU: two workgroups of one each share it unevenly (the
     // older one's waves go first: done after 430 us, the other's after 525) and leave it half empty at the
-    // end, 588 us against 473 for five ragged prompts. 16-query groups per wave (MT): 256 dims take the
+    // end, 24% longer for five ragged prompts. 16-query groups per wave (MT): 256 dims take the
     // registers of two.
     static constexpr int MT = D == 256 ? 1 : 2, WAVES = 8, M = 16 * MT * WAVES;
     static constexpr int TB = D == 256 ? 32 : 64;
@@ -889,7 +890,8 @@ __global__ __launch_bounds__(64 * TileGeo<D>::WAVES, 2) void k_paged_tile(
         fetch(from * TB);
         stage(0);
         __syncthreads();
-        // a wave without queries only stages (33 requests of a row or two in a batch that came here: 133 -> 100 us)
+        // a wave without queries only stages (33 requests of a row or two in a batch that came here: 133 -> 100 us;
+        // ragged prompts of 256 dims, which gain nothing, 325 -> 329)
         if (r0 < 0) {
             for (int step = from; step < to; ++step) {
                 fetch(min(step + 1, to - 1) * TB);
